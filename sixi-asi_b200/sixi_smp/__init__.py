@@ -9,7 +9,8 @@ Entry points mirror the engine's sampler/verifier interface (include/sixi_smp.h)
   candidates       DeterministicSampler::compute_sampling_candidates  (:449-584)
   greedy_argmax    DeterministicSampler::sample_greedy_argmax  (:394-407)
   verify           SpeculativeDecoder::step verification       src/speculative/speculative.cpp:589-916
-and the device-side producer of JSON-object grammar masks (include/sixi_json.h, json_grammar.py).
+and the device-side producer of JSON-object grammar masks (include/sixi_json.h, json_grammar.py) and
+the 8-bit paged key/value cache with its attention (include/sixi_kv.h, kv_cache.py).
 """
 
 from __future__ import annotations
@@ -134,6 +135,18 @@ SIGNATURES = {
     "sixi_schema_check_text": (_I32, [_P, _P, ctypes.c_size_t]),
 }
 
+# include/sixi_kv.h: the 8-bit paged key/value cache (sixi_smp.kv_cache)
+KV_SIGNATURES = {
+    "sixi_kv_create": (_I32, [_I32, _P, _P, _P, _P, _P, ctypes.POINTER(_P)]),
+    "sixi_kv_destroy": (_I32, [_P]),
+    "sixi_kv_rope_create": (_I32, [_I32, _P, ctypes.POINTER(_P)]),
+    "sixi_kv_rope_destroy": (_I32, [_P]),
+    "sixi_kv_rope_apply": (_I32, [_P, _P, _P, _U32, _U32, _U32, _P, _P]),
+    "sixi_kv_append": (_I32, [_P, _P, _P, _P, _P, _P, _P]),
+    "sixi_kv_read": (_I32, [_P, _P, _P, _P, _P, _P]),
+    "sixi_kv_attend": (_I32, [_P, _P, _P, ctypes.c_float, _U32, _U32, _P, _P, _P, _P, _P]),
+}
+
 
 def load(path: Path | str = LIB_PATH) -> ctypes.CDLL:
     path = Path(path)
@@ -142,7 +155,7 @@ def load(path: Path | str = LIB_PATH) -> ctypes.CDLL:
             f"{path} is missing: build it with `python sixi-asi_b200/build_lib.py` "
             "(there is no CPU fallback)")
     lib = ctypes.CDLL(str(path))
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -1,0 +1,252 @@
+"""The 8-bit paged key/value cache (include/sixi_kv.h) over torch CUDA tensors.
+
+A serving step on a batch of streams, before the sampler or the verifier sees its logits:
+
+    rope = Rope(rot_dim=128, base=1e6)
+    cache = KvCache(n_pages, page_size=64, n_kv_heads=8, head_dim=128)
+    batch = KvBatch(page_table, offsets, lens, n_tokens, max_new)
+    cache.append(k, v, batch, rope=rope)                 # the new tokens' keys and values
+    out, lse, status = cache.attend(q, batch, rope=rope)  # their queries over all cached tokens
+
+`batch` names each sequence's last offsets[s + 1] - offsets[s] positions: one token a stream for a
+decode step, 1 + k for speculative verification, a chunk of a prompt. After the verifier has accepted
+a of k drafts, lens for the next batch continues from lens - k + a.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+from . import BF16, F32, _check, _lib, _ptr
+
+_P = ctypes.c_void_p
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+ATTEND_ALL = 1  # SIXI_KV_ATTEND_ALL
+
+
+class KvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim", "max_seqs", "reserved")]
+
+
+class KvTensor(ctypes.Structure):
+    _fields_ = [("data", _P), ("dtype", ctypes.c_uint32), ("n_heads", ctypes.c_uint32),
+                ("token_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64)]
+
+
+class KvBatchStruct(ctypes.Structure):
+    _fields_ = [("page_table", _P), ("table_stride", ctypes.c_uint64), ("offsets", _P), ("lens", _P),
+                ("n_seqs", ctypes.c_uint32), ("max_pages", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32),
+                ("max_new", ctypes.c_uint32)]
+
+
+class RopeConfig(ctypes.Structure):
+    _fields_ = [("rot_dim", ctypes.c_uint32), ("layout", ctypes.c_uint32), ("scaling", ctypes.c_uint32),
+                ("original_max_position", ctypes.c_uint32), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
+
+
+def _dev_index(device) -> int:
+    import torch
+
+    if device is None:
+        return torch.cuda.current_device()
+    d = torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
+    return d.index if d.index is not None else torch.cuda.current_device()
+
+
+def _stream(stream) -> int:
+    import torch
+
+    return int((stream if stream is not None else torch.cuda.current_stream()).cuda_stream)
+
+
+def _view(t, device: int, dim: int, what: str) -> KvTensor:
+    """[tokens, heads, dim] rows of a torch tensor with unit stride along dim."""
+    import torch
+
+    if t.dtype not in (torch.float32, torch.bfloat16) or t.dim() != 3 or t.shape[2] != dim:
+        raise ValueError(f"{what}: fp32 or bf16 [tokens, heads, {dim}] expected, got {t.dtype} {tuple(t.shape)}")
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{what}: on {t.device}, not cuda:{device}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{what}: the last dimension must have unit stride")
+    return KvTensor(t.data_ptr(), F32 if t.dtype == torch.float32 else BF16, t.shape[1], t.stride(0), t.stride(1))
+
+
+class Rope:
+    """Rotary frequencies on one device (sixi_kv_rope_create). layout "half" or "interleaved"; scaling
+    "none", "linear", "ntk" or "yarn" (factor; yarn also original_max_position and the betas)."""
+
+    def __init__(self, rot_dim: int, base: float = 10000.0, layout: str = "half", scaling: str = "none",
+                 factor: float = 1.0, original_max_position: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 device=None):
+        if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+            raise ValueError(f"unknown rotary layout {layout!r} or scaling {scaling!r}")
+        self.h = None
+        self.device = _dev_index(device)
+        self.rot_dim = rot_dim
+        c = RopeConfig(rot_dim, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], original_max_position, base, factor,
+                       beta_fast, beta_slow)
+        h = _P()
+        _check("sixi_kv_rope_create", _lib().sixi_kv_rope_create(self.device, ctypes.byref(c), ctypes.byref(h)))
+        self.h = h
+
+    def close(self) -> None:
+        if self.h:
+            _lib().sixi_kv_rope_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def apply(self, x, positions, inverse: bool = False, out=None, stream=None):
+        """x [tokens, heads, dim] turned by positions [tokens] (int32); inverse turns back (the gradient).
+        out may be x."""
+        import torch
+
+        if positions.dtype != torch.int32 or positions.shape != (x.shape[0],) or not positions.is_contiguous():
+            raise ValueError("positions: contiguous int32 [tokens] expected")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape:
+            raise ValueError(f"out: {tuple(x.shape)} expected, got {tuple(out.shape)}")
+        xv, ov = _view(x, self.device, x.shape[2], "x"), _view(out, self.device, x.shape[2], "out")
+        st = _lib().sixi_kv_rope_apply(self.h, ctypes.byref(xv), _ptr(positions), x.shape[0], x.shape[2],
+                                       1 if inverse else 0, ctypes.byref(ov), _stream(stream))
+        _check("sixi_kv_rope_apply", st)
+        return out
+
+
+class KvBatch:
+    """The positions a call works on (sixi_kv_batch): page_table int32 [seqs, max_pages], offsets int64
+    [seqs + 1], lens int32 [seqs] (device tensors, kept alive here), and on the host the total number of
+    tokens and the most of one sequence."""
+
+    def __init__(self, page_table, offsets, lens, n_tokens: int, max_new: int):
+        import torch
+
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+            raise ValueError("page_table: int32 [seqs, max_pages] with unit stride along pages expected")
+        n = page_table.shape[0]
+        if offsets.dtype != torch.int64 or offsets.shape != (n + 1,) or not offsets.is_contiguous():
+            raise ValueError(f"offsets: contiguous int64 [{n + 1}] expected")
+        if lens.dtype != torch.int32 or lens.shape != (n,) or not lens.is_contiguous():
+            raise ValueError(f"lens: contiguous int32 [{n}] expected")
+        self.page_table, self.offsets, self.lens = page_table, offsets, lens
+        self.n_seqs, self.n_tokens, self.max_new = n, int(n_tokens), int(max_new)
+        self.struct = KvBatchStruct(page_table.data_ptr(), page_table.stride(0), offsets.data_ptr(), lens.data_ptr(), n,
+                                    page_table.shape[1], self.n_tokens, self.max_new)
+
+
+class KvCache:
+    """A cache on one device (sixi_kv_create). The pages are torch tensors: uint8 or float8_e4m3fn
+    [n_pages, n_kv_heads, page_size, head_dim] and fp32 scales [n_pages, n_kv_heads], allocated here
+    unless given."""
+
+    def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, k_pages=None, v_pages=None,
+                 k_scales=None, v_scales=None, max_seqs: int = 4096, device=None):
+        import torch
+
+        self.h = None
+        given = next((t for t in (k_pages, v_pages, k_scales, v_scales) if t is not None), None)
+        self.device = _dev_index(given.device if device is None and given is not None else device)
+        dev = torch.device("cuda", self.device)
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+
+        def buffer(t, shape, dtypes, what):
+            if t is None:
+                return torch.empty(shape, dtype=dtypes[0], device=dev)
+            if tuple(t.shape) != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{what}: contiguous {dtypes[0]} {shape} on {dev} expected, got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+            return t
+
+        by = (torch.uint8, torch.float8_e4m3fn)
+        self.k_pages, self.v_pages = buffer(k_pages, shape, by, "k_pages"), buffer(v_pages, shape, by, "v_pages")
+        self.k_scales = buffer(k_scales, shape[:2], (torch.float32,), "k_scales")
+        self.v_scales = buffer(v_scales, shape[:2], (torch.float32,), "v_scales")
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = shape[0], page_size, n_kv_heads, head_dim
+        c = KvConfig(n_pages, page_size, n_kv_heads, head_dim, max_seqs, 0)
+        h = _P()
+        st = _lib().sixi_kv_create(self.device, ctypes.byref(c), _ptr(self.k_pages), _ptr(self.v_pages),
+                                   _ptr(self.k_scales), _ptr(self.v_scales), ctypes.byref(h))
+        _check("sixi_kv_create", st)
+        self.h = h
+
+    def close(self) -> None:
+        if self.h:
+            _lib().sixi_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _tensor(self, t, batch: KvBatch, what: str) -> KvTensor:
+        if t.dim() != 3 or t.shape[0] != batch.n_tokens:
+            raise ValueError(f"{what}: [{batch.n_tokens}, heads, {self.head_dim}] expected, got {tuple(t.shape)}")
+        return _view(t, self.device, self.head_dim, what)
+
+    def _status(self, status, batch: KvBatch):
+        import torch
+
+        if status is None:
+            return torch.empty(batch.n_seqs, dtype=torch.int32, device=torch.device("cuda", self.device))
+        if status.dtype != torch.int32 or status.shape != (batch.n_seqs,) or not status.is_contiguous():
+            raise ValueError(f"status: contiguous int32 [{batch.n_seqs}] expected")
+        return status
+
+    def append(self, k, v, batch: KvBatch, rope: Rope | None = None, status=None, stream=None):
+        """Writes k, v [tokens, n_kv_heads, head_dim] at the batch's positions, the keys turned by rope.
+        Returns the status of each sequence (int32, device)."""
+        kv, vv = self._tensor(k, batch, "k"), self._tensor(v, batch, "v")
+        status = self._status(status, batch)
+        st = _lib().sixi_kv_append(self.h, ctypes.byref(kv), ctypes.byref(vv), ctypes.byref(batch.struct),
+                                   rope.h if rope is not None else None, _ptr(status), _stream(stream))
+        _check("sixi_kv_append", st)
+        return status
+
+    def read(self, batch: KvBatch, dtype=None, k=None, v=None, status=None, stream=None):
+        """The batch's positions as values: k, v [tokens, n_kv_heads, head_dim] (dtype bf16 or fp32)."""
+        import torch
+
+        if k is None or v is None:
+            dt = dtype or torch.bfloat16
+            shape, dev = (batch.n_tokens, self.n_kv_heads, self.head_dim), torch.device("cuda", self.device)
+            k = torch.empty(shape, dtype=dt, device=dev) if k is None else k
+            v = torch.empty(shape, dtype=dt, device=dev) if v is None else v
+        kv, vv = self._tensor(k, batch, "k"), self._tensor(v, batch, "v")
+        status = self._status(status, batch)
+        st = _lib().sixi_kv_read(self.h, ctypes.byref(batch.struct), ctypes.byref(kv), ctypes.byref(vv), _ptr(status),
+                                 _stream(stream))
+        _check("sixi_kv_read", st)
+        return k, v
+
+    def attend(self, q, batch: KvBatch, scale: float | None = None, window: int = 0, causal: bool = True,
+               rope: Rope | None = None, out=None, lse=None, status=None, stream=None):
+        """Attention of q [tokens, n_q_heads, head_dim] over the cache: (out like q, lse fp32 [tokens,
+        n_q_heads], status int32 [seqs]). scale defaults to head_dim ** -0.5; window 0 is none."""
+        import torch
+
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape:
+            raise ValueError(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
+        if lse is None:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        elif lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
+            raise ValueError(f"lse: contiguous fp32 {tuple(q.shape[:2])} expected")
+        qv, ov = self._tensor(q, batch, "q"), self._tensor(out, batch, "out")
+        status = self._status(status, batch)
+        st = _lib().sixi_kv_attend(self.h, ctypes.byref(qv), ctypes.byref(batch.struct),
+                                   self.head_dim ** -0.5 if scale is None else scale, window,
+                                   0 if causal else ATTEND_ALL, rope.h if rope is not None else None, ctypes.byref(ov),
+                                   _ptr(lse), _ptr(status), _stream(stream))
+        _check("sixi_kv_attend", st)
+        return out, lse, status
