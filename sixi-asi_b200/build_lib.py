@@ -60,7 +60,7 @@ def build(jobs: int | None = None, force: bool = False, verbose: bool = True) ->
             units.append((CSRC / "smp_inst.cu", BUILD / f"inst_{mname}_{dname}.o",
                           [f"-DSIXI_INST_MODE={m}", f"-DSIXI_INST_DT={d}"]))
     for name in ("smp_launch", "smp_abi", "smp_shard", "smp_dist", "smp_json", "smp_numeric", "smp_suffix", "smp_schema",
-                 "smp_kv", "smp_kv_attn"):
+                 "smp_kv", "smp_kv_attn", "smp_kv_mma"):
         units.append((CSRC / f"{name}.cu", BUILD / f"{name}.o", []))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         futs = [ex.submit(_compile, s, o, d, force) for s, o, d in units]

@@ -481,6 +481,7 @@ struct sixi_kv {
     uint32_t* counter;    // [kAttnMaxCtas], zero between calls
     float* part;          // attention's partial results
     uint64_t part_stride;
+    CUtensorMap k_map, v_map;  // pages as attention copies them
 };
 
 struct sixi_kv_rope {
@@ -609,6 +610,8 @@ int32_t sixi_kv_create(int32_t device, const sixi_kv_config* c, void* k_pages, v
         e = cudaMalloc(reinterpret_cast<void**>(&h->part), sizeof(float) * 2u * kAttnMaxCtas * h->part_stride);
     if (e == cudaSuccess) e = cudaMemset(h->seq_state, 0, sizeof(uint32_t) * 2u * c->max_seqs);
     if (e == cudaSuccess) e = cudaMemset(h->counter, 0, sizeof(uint32_t) * kAttnMaxCtas);
+    if (e == cudaSuccess) e = make_page_map(k_pages, h->g, &h->k_map);
+    if (e == cudaSuccess) e = make_page_map(v_pages, h->g, &h->v_map);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e != cudaSuccess) {
         sixi_kv_destroy(h);
@@ -746,8 +749,10 @@ int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch*
     a.part = h->part;
     a.counter = h->counter;
     a.part_stride = h->part_stride;
-    return kv_from_cuda(
-        launch_attend_f32(a, h->n_sms, q->dtype == SIXI_SMP_BF16, static_cast<cudaStream_t>(stream)));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return kv_from_cuda(q->dtype == SIXI_SMP_BF16
+                            ? launch_attend_bf16(a, h->k_map, h->v_map, b->max_new, h->n_sms, s)
+                            : launch_attend_f32(a, h->n_sms, s));
 }
 
 }  // extern "C"

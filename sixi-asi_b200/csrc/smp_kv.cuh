@@ -451,6 +451,9 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
                              cudaStream_t stream);
 cudaError_t launch_kv_read(const KvGeom& g, const KvBatchView& b, const sixi_kv_tensor* k, const sixi_kv_tensor* v,
                            int32_t* status, cudaStream_t stream);
-cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, bool bf16, cudaStream_t stream);
+cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, cudaStream_t stream);
+cudaError_t make_page_map(void* pages, const KvGeom& g, CUtensorMap* out);
+cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, const CUtensorMap& v_map, uint32_t max_new,
+                               uint32_t n_sms, cudaStream_t stream);
 
 }  // namespace sixi_b200

@@ -38,8 +38,10 @@ struct Smem {
     float* red;     // [4096] sums over token groups
 };
 
-// One tile's bytes and scales into stage st; tokens outside the sequence (or with a bad page) are zero.
-__device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, const Piece& pc, int32_t tile, uint32_t st) {
+// One tile's bytes and scales into stage st; tokens outside the sequence, before the window of the unit's
+// first row (lo) or in a bad page are zero.
+__device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, const Piece& pc, int32_t lo, int32_t tile,
+                                          uint32_t st) {
     const uint32_t D = a.g.head_dim, row = D + 16u, per = D / 16u;
     uint8_t* dst = sm.kv + static_cast<uint64_t>(st) * 2u * kT * row;
     const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
@@ -47,7 +49,7 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, con
         const uint32_t kv = i / (kT * per), j = i - kv * (kT * per);
         const uint32_t t = j / per, c = j - t * per;
         const int32_t pos = tile * kT + static_cast<int32_t>(t);
-        bool on = pos < pc.plan.len;
+        bool on = pos < pc.plan.len && pos >= lo;
         uint64_t off = 0;
         if (on) {
             const int32_t id = table[static_cast<uint32_t>(pos) >> a.g.page_shift];
@@ -62,7 +64,7 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, con
         const uint32_t kv = threadIdx.x >> kTileShift, t = threadIdx.x & (kT - 1u);
         const int32_t pos = tile * kT + static_cast<int32_t>(t);
         float f = 0.0f;
-        if (pos < pc.plan.len) {
+        if (pos < pc.plan.len && pos >= lo) {
             const int32_t id = table[static_cast<uint32_t>(pos) >> a.g.page_shift];
             if (static_cast<uint32_t>(id) < a.g.n_pages)
                 f = (kv ? a.g.v_scales : a.g.k_scales)[static_cast<uint64_t>(id) * a.g.n_heads + pc.head];
@@ -107,7 +109,10 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
     while (next_piece(a.shape, a.b, a.g.page_shift, walk, &pc)) {
         const uint32_t r_base = pc.row_tile * kRt;
         __syncthreads();
-        load_tile(a, sm, pc, pc.t0, 0);
+        const int32_t lo = a.shape.window ? pc.plan.p0 + static_cast<int32_t>(r_base / a.shape.group) -
+                                                static_cast<int32_t>(a.shape.window) + 1
+                                          : 0;
+        load_tile(a, sm, pc, lo, pc.t0, 0);
         // queries, turned and rounded to their type, then scaled; a NaN or Inf makes the row NaN
         for (uint32_t i = tid; i < kRt * D; i += kNT) {
             const uint32_t r = i / D, d = i - r * D;
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
         for (int32_t tile = pc.t0; tile < pc.t1; ++tile) {
             const uint32_t st = static_cast<uint32_t>(tile - pc.t0) & 1u;
             if (tile + 1 < pc.t1) {
-                load_tile(a, sm, pc, tile + 1, st ^ 1u);
+                load_tile(a, sm, pc, lo, tile + 1, st ^ 1u);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -287,13 +292,13 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
             const uint32_t r = i / D, d = i - r * D;
             float M = kNegInf, l = 0.0f, o = 0.0f;
             for (uint32_t c = c0; c <= c1; ++c)
-                M = fmaxf(M, a.part[(2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r]);
+                M = fmaxf(M, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r));
             for (uint32_t c = c0; c <= c1; ++c) {
                 const float* p = a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride;
-                const float m = p[kPartRows * D + r];
+                const float m = __ldcg(p + kPartRows * D + r);
                 const float f = m == M ? 1.0f : exp2f(m - M);
-                l += p[kPartRows * (D + 1u) + r] * f;
-                o += p[r * D + d] * f;
+                l += __ldcg(p + kPartRows * (D + 1u) + r) * f;
+                o += __ldcg(p + r * D + d) * f;
             }
             const uint32_t rr = r_base + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
             T* p = static_cast<T*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
@@ -309,13 +314,13 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
 
 }  // namespace
 
-cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, bool bf16, cudaStream_t stream) {
+cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, cudaStream_t stream) {
     a.shape.rt = kRt;
     a.shape.tile_shift = kTileShift;
     const uint32_t D = a.g.head_dim;
     const size_t smem = sizeof(float) * (static_cast<size_t>(kRt) * D + 4u * kT * (D + 16u) / 4u + 4u * kT + 2u * kRt * kT +
                                          4096u + 3u * kRt);
-    auto fn = bf16 ? attend_f32_kernel<__nv_bfloat16> : attend_f32_kernel<float>;
+    auto fn = attend_f32_kernel<float>;
     cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     const uint32_t ctas = 2u * n_sms < kAttnMaxCtas ? 2u * n_sms : kAttnMaxCtas;
