@@ -418,11 +418,6 @@ cudaError_t launch_rope_apply(const RopeView& r, const sixi_kv_tensor* x, const 
                : rope_dispatch<float, 4>(r, x, positions, n_tokens, head_dim, out, stream);
 }
 
-// whether 8 consecutive elements are turned (or passed through) together
-static bool rope_by_8(const RopeView& r) {
-    return r.turns == nullptr || (r.interleaved ? r.rot_dim % 8 == 0 : (r.rot_dim / 2) % 8 == 0);
-}
-
 cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_kv_tensor* k, const sixi_kv_tensor* v,
                              const RopeView& rope, uint32_t max_new, int32_t* status, uint32_t* seq_state,
                              cudaStream_t stream) {

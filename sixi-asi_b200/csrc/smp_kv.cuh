@@ -439,6 +439,11 @@ struct AttnArgs {
     uint64_t part_stride;
 };
 
+// whether 8 consecutive elements (at a multiple of 8) are turned, or passed through, together
+inline bool rope_by_8(const RopeView& r) {
+    return r.turns == nullptr || (r.interleaved ? r.rot_dim % 8 == 0 : (r.rot_dim / 2) % 8 == 0);
+}
+
 // Partial results: two per CTA (a unit that the CTA continues, and one that it leaves to the next), each
 // kPartRows rows of head_dim unnormalised fp32 sums, then the rows' maxima (base 2) and sums.
 constexpr uint32_t kAttnMaxCtas = 512;

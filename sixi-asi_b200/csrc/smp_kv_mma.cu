@@ -2,7 +2,7 @@
 // queries): the cached bytes go from memory to tcgen05.mma as they are, nothing is widened on the way.
 //
 // Mathematics. Both products are fp8 products with fp32 accumulation, and the 16-bit side of each is
-// split into two e4m3 terms that are multiplied one after the other into the same accumulator:
+// split into two e4m3 terms that are multiplied side by side:
 //   S^T = K (q_hi + q_lo)^T       a bf16 value has 8 significant bits, an e4m3 one has 4: after a row is
 //                                 scaled by a power of two the split is exact (but for elements below
 //                                 1/1792 of the row's largest, which err by 2^-19 of it at most)
@@ -17,14 +17,20 @@
 //
 // Layout. Tokens are the M side of the scores (128 of them a tile, one per TMEM lane), query rows the N
 // side (16 to 64: the query heads of one key head times new tokens); head elements are the M side of the
-// output. So a decode step's 8 rows do not pad a 128-row tile, the softmax has one token per thread with
-// all threads busy, and K and V are both the A operand as they lie in memory: K is K-major, V MN-major,
-// each a 128-byte-swizzled tile that TMA copies page by page (whatever the page size) into 128 x 128 bytes.
+// output. So a decode step's 8 rows do not pad a 128-row tile, and K and V are both the A operand as they lie
+// in memory: K is K-major, V MN-major, each a 128-byte-swizzled tile that TMA copies page by page (whatever
+// the page size) into 128 x 128 bytes. The softmax reads scores in 16x256b fragments: a thread has 4 tokens of
+// a quarter of the rows, so most of a row's maximum and sum is taken within a thread. The columns of the
+// weights are dealt such that a thread's rows are neighbours there (row 8 j + 2 q + e is column
+// q * R / 4 + 2 j + e), and go out in one store a token.
 //
-// Roles, one CTA per SM: warp 0 copies pages, warp 1 issues the products, warps 2-3 stage queries (turned,
-// split) and check page tables, warps 4-7 keep the output's sums (one head element a thread), warps 8-11
-// (8-15 for 64 rows) are the softmax. Scores, weights and output tiles are double-buffered, so the
-// products of one tile overlap the softmax of another; copies run up to 6 tiles ahead and across units.
+// A product of up to 128 columns takes about as long as one of 16 (40 to 66 cycles measured), so hi and lo are
+// side by side in one operand of twice the rows, not two products.
+//
+// Roles, one CTA per SM: warp 0 copies pages, warps 1 and 2 issue the two products, warp 3 stages queries
+// (turned, split) and checks page tables, warps 4-7 keep the output's sums (one head element a thread), warps 8-11
+// and 12-15 are two softmax groups that take every other tile, each with its own running maximum. A tile's
+// softmax is a chain of waits; two at a time, with the scores of the next ready before it ends, hide it.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -41,26 +47,27 @@ constexpr int kTileShift = 7;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait (never expected to run out)
+constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
 constexpr int kQSlots = 8;  // pieces whose row records are kept: softmax lags the staging by fewer than 5
 
 // R rows of a row tile, DC 128-element chunks of a head
 template <int R, int DC>
 struct Cfg {
-    static constexpr int kGroups = R > 32 ? 2 : 1;        // softmax warpgroups
-    static constexpr int kCols = R / kGroups;             // rows of one softmax warpgroup
-    static constexpr int kThreads = 256 + 128 * kGroups;
-    static constexpr uint32_t kChunk = kTile * 128u;      // bytes of a tile's chunk
-    static constexpr uint32_t kStage = 2u * DC * kChunk;  // K then V
+    static constexpr int kThreads = 512;
+    static constexpr int V = R / 4;                       // rows of a softmax thread
+    static constexpr uint32_t kChunk = kTile * 128u;      // bytes of a tile's chunk of keys or values
+    static constexpr uint32_t kBuf = DC * kChunk;
     static constexpr uint32_t kQ = DC * 2u * R * 128u;    // hi rows, lo rows, chunk by chunk
     static constexpr uint32_t kW = 2u * R * kTile;        // hi, lo
     static constexpr uint32_t kFixed = 2u * kQ + 2u * kW;
-    static constexpr uint32_t kMax = 227u * 1024u - 1024u - 8192u;  // less alignment and the small arrays
-    static constexpr int kFit = static_cast<int>((kMax - kFixed) / kStage);
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
-    static constexpr uint32_t kDyn = kFixed + kStages * kStage + 1024u;
-    static constexpr uint32_t kColsUsed = 2u * R + 4u * DC * R;  // scores; hi and lo outputs; two of each
+    static constexpr uint32_t kSmall = 2048u + 320u * R;  // bound of the small arrays
+    static constexpr int kBufs = static_cast<int>((227u * 1024u - 1024u - kSmall - kFixed) / kBuf);
+    static constexpr int kNK = kBufs / 2 > 6 ? 6 : kBufs / 2;            // tiles of keys in flight
+    static constexpr int kNV = kBufs - kNK > 6 ? 6 : kBufs - kNK;        // and of values
+    static constexpr uint32_t kDyn = kFixed + (kNK + kNV) * kBuf + 1024u;
+    static constexpr uint32_t kColsUsed = 4u * R + 4u * DC * R;  // scores and outputs, hi and lo, two of each
     static constexpr uint32_t kTmem = kColsUsed <= 64 ? 64u : (kColsUsed <= 128 ? 128u : (kColsUsed <= 256 ? 256u : 512u));
-    static_assert(kStages >= 2 && kColsUsed <= 512, "does not fit");
+    static_assert(kNK >= 2 && kNV >= 2 && kColsUsed <= 512, "does not fit");
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -88,24 +95,28 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait of a whole warp, with one answer for all its lanes: false when the bound ran out or
-// another role of the CTA gave up.
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
-    for (uint32_t i = 0; i < kWaitIters; ++i) {
-        if (__all_sync(0xFFFFFFFFu, bar_try(b, parity))) return true;
-        if (__any_sync(0xFFFFFFFFu, *gave_up != 0u)) return false;
+// Bounded wait of a whole warp. When a bound runs out anywhere in the CTA, no further wait waits and no further
+// copy or product is issued: every role runs through its tiles and ends, and the results are reported as bad.
+__device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
+    if (!bar_try(b, parity)) {
+        bool ok = false;
+        for (uint32_t i = 0; i < kWaitIters && !ok; ++i) ok = bar_try(b, parity) || *gave_up != 0u;
+        if (!ok) *gave_up = 1u;
     }
-    *gave_up = 1u;
-    return false;
-}
-// A bounded barrier of the warps that `b` counts (one arrival a warp); *phase is the caller's count.
-__device__ __forceinline__ bool warps_meet(uint64_t* b, uint32_t* phase, volatile uint32_t* gave_up) {
     __syncwarp();
-    if ((threadIdx.x & 31u) == 0) bar_arrive(b);
-    const bool ok = bar_wait(b, *phase & 1u, gave_up);
-    ++*phase;
-    return ok;
 }
+// one lane of the (converged) warp: with it the compiler keeps the operands of a product uniform, which halves
+// the cost of issuing one (40 cycles against 63 for a lane picked by its number)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0u;
+}
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
 __device__ __forceinline__ void tma_page(const CUtensorMap* map, void* dst, uint64_t* bar, int32_t x, int32_t z) {
     asm volatile(
@@ -138,6 +149,15 @@ __device__ __forceinline__ void tmem_ld8(uint32_t addr, float* x) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v[i]);
 }
+// a 16-lane, 8-column fragment: x[0..1] of lane (thread / 4), x[2..3] of lane 8 + (thread / 4), columns 2 * (thread % 4)..
+__device__ __forceinline__ void tmem_ld_frag(uint32_t addr, float* x) {
+    uint32_t v[4];
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // shared-memory matrix descriptors: 128-byte swizzle (rows of 128 bytes, 8-row groups 1,024 bytes apart)
@@ -155,87 +175,216 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float warp_max(float x) {
-    float y;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-    return y;
+// two fp32 operations at a time
+struct F2 {
+    uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 un2(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
 }
 
-// Two weights in [0, 256] as e4m3 bytes: hi = the nearest, lo = what hi leaves, times 16. The rest is
-// taken in f16 (11 significant bits; exact there, as hi is one of its values).
+// Two weights in [0, 1] as e4m3 codes of 256 times their value: hi = the nearest, lo = 16 times what hi leaves.
+// In f16, w has the exponent field that 256 w has in e4m3 (and subnormals have the same steps times 2^-7), so
+// hi's code is w's f16 pattern rounded at bit 7. hi: the codes in bytes 0 and 2; lo: in bytes 0 and 1.
 constexpr float kLoInv = 1.0f / 16.0f;
-__device__ __forceinline__ void split2(float w0, float w1, uint32_t* hi, uint32_t* lo) {
-    const __half2 w = __floats2half2_rn(w0, w1);
-    const __half2_raw wr = w;
-    const __nv_fp8x2_storage_t h = __nv_cvt_halfraw2_to_fp8x2(wr, __NV_SATFINITE, __NV_E4M3);
-    const __half2 back = __half2(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3));
-    const __half2_raw rest = __hmul2(__hsub2(w, back), __float2half2_rn(16.0f));
-    *hi = h;
+__device__ __forceinline__ void split2(F2 w, uint32_t* hi, uint32_t* lo) {
+    const float2 f = un2(w);
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    const uint32_t top = (*reinterpret_cast<const uint32_t*>(&h) + 0x00400040u) & 0xFF80FF80u;
+    const __half2_raw rest = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&top)), __float2half2_rn(4096.0f));
+    *hi = top >> 7;
     *lo = __nv_cvt_halfraw2_to_fp8x2(rest, __NV_SATFINITE, __NV_E4M3);
+}
+
+// Over the 8 lanes of one lane % 4 (a thread's tokens): N values each, reduced to N / 8 (at least 1) a lane, value
+// `first_of(lane)` on. Halves are exchanged and folded, so it takes N shuffles instead of 3 N.
+template <int N, typename Op>
+__device__ __forceinline__ void fold_lanes(float* x, uint32_t lane, Op op) {
+    int n = N;
+#pragma unroll
+    for (int o = 16; o >= 4; o >>= 1) {
+        const bool up = (lane & o) != 0u;
+        if (n > 1) {
+            n >>= 1;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                if (i >= n) break;
+                const float send = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+                x[i] = op(keep, __shfl_xor_sync(0xFFFFFFFFu, send, o));
+            }
+        } else {
+            x[0] = op(x[0], __shfl_xor_sync(0xFFFFFFFFu, x[0], o));
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ uint32_t first_of(uint32_t lane) {
+    if constexpr (N == 4) return (lane >> 3) & 3u;
+    if constexpr (N == 8) return lane >> 2;
+    return (lane >> 2) * (N / 8);
 }
 
 // ---------------------------------------------------------------------------------------------
 
 template <int R, int DC>
 struct Shared {
-    static constexpr int kS = Cfg<R, DC>::kStages;
-    uint64_t kfull[kS], vfull[kS], empty[kS];
-    uint64_t sfull[2], sempty[2], wfull[2], ofull[2], oempty[2], qfull[2], qempty[2], rfull[kQSlots], lfull, lempty, meet[3], done;
+    static constexpr int kNK = Cfg<R, DC>::kNK, kNV = Cfg<R, DC>::kNV;
+    uint64_t kfull[kNK], vfull[kNV], scfull[kNV];
+    uint64_t sfull[kRing], ofull[kRing];  // of tile n at n % kRing: its scores, its output are done
+    uint64_t sempty[2], wfull[2], oempty[2], qfull[2], qempty[2], rfull[kQSlots], lfull, lempty, done;
     unsigned long long scratch[Cfg<R, DC>::kThreads / 32 + 2];
     uint32_t tmem, gave_up, last_flag, pad;
-    float kscale[kS][8], vscale[kS][8];     // by page of the tile
-    float frow[kQSlots][R];                 // a row's factor from the product to the score, base 2
-    int32_t qpos[kQSlots][R];               // a row's position; INT_MIN beyond the valid rows
-    float wmax[2][R / Cfg<R, DC>::kCols][4][Cfg<R, DC>::kCols];
-    float wmax2[Cfg<R, DC>::kGroups][4][Cfg<R, DC>::kCols];  // the same of weight times value scale
-    float2 ref[Cfg<R, DC>::kGroups * 4][Cfg<R, DC>::kCols];  // per warp: running maximum, weight factor
-    float osc[2][R], alpha[2][R];           // a tile's factor, and the older sums'
-    uint32_t changed[2][2];                 // [buffer][group] some alpha is not 1
-    float lsum[4][R], mfin[R];
+    float kscale[kNV][8], vscale[kNV][8];   // by page of the tile
+    // by column of the weights:
+    alignas(16) float frow[kQSlots][R];                 // a row's factor from the product to the score, base 2; positive
+    int32_t qpos[kQSlots][R];               // a row's position
+    float wmax[2][2][4][R];                 // [group][its tiles' parity][warp] a tile's maxima
+    alignas(16) float2 ref[8][R];                       // [softmax warp] running maximum, weight factor
+    float rescale[8][R];                    // [softmax warp] factor of the older sums
+    float osc[2][R], mgrp[2][R];            // a tile's factor, and the running maximum that its weights are under
+    alignas(16) float fac[4][R], facold[4][R];  // [output warp] a tile's factor, the older sums' factor
+    float lsum[2][4][R], mfin[2][R];        // [group][warp] a piece's sums; [group] maxima
 };
 
 struct MmaArgs {
     AttnArgs a;
     uint32_t pages_per_tile;
+    uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
 };
+
+// A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle), 8 elements a lane, DC * 16 lanes a row;
+// this warp takes rows `at`, `at` + `step`, ... in units of the rows that it handles at once, U units at a time.
+template <int R, int DC, int U>
+__device__ __forceinline__ void stage_queries(const MmaArgs& args, const Piece& pc, uint8_t* dst, float* frow, int32_t* qpos,
+                                              uint32_t at, uint32_t step) {
+    constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC>::V;
+    const AttnArgs& a = args.a;
+    const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
+    const uint32_t sub = lane / kRowLanes, d0 = (lane % kRowLanes) * 8u;
+    const float sign = a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : 0.0f);
+    for (uint32_t rb = at * kAtOnce; rb < pc.rows; rb += step * kAtOnce * U) {
+        float x[U][8], m[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = rb + u * step * kAtOnce + sub;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
+            if (r < pc.rows && d0 < D) {
+                const uint32_t rr = pc.row_tile * R + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
+                const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                                         (pc.head * a.shape.group + g) * a.q.head_stride;
+                const int32_t pos = pc.plan.p0 + static_cast<int32_t>(tok);
+                if (args.q_vec) {
+                    load_turned<__nv_bfloat16, 8>(a.rope, p, d0, pos, x[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) load_turned<__nv_bfloat16, 1>(a.rope, p, d0 + j, pos, &x[u][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            m[u] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // a turned query is rounded to its type, as a rotation of its own would be
+                x[u][j] = __bfloat162float(__float2bfloat16_rn(x[u][j]));
+                const float ab = fabsf(x[u][j]);
+                m[u] = ab < __builtin_huge_valf() ? fmaxf(m[u], ab) : __builtin_huge_valf();
+            }
+        }
+#pragma unroll
+        for (uint32_t o = kRowLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o));
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = rb + u * step * kAtOnce + sub;
+            if (r >= pc.rows) continue;
+            const bool bad = m[u] == __builtin_huge_valf();
+            const int e = bad ? 0 : kv_scale_exp(m[u]);
+            const float mul = exp2_int(-e) * sign;  // the sign of the scale is the query's here
+            uint32_t h[2], l[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float v0 = x[u][4 * j] * mul, v1 = x[u][4 * j + 1] * mul;
+                const float v2 = x[u][4 * j + 2] * mul, v3 = x[u][4 * j + 3] * mul;
+                h[j] = e4m3x2(v0, v1) | (e4m3x2(v2, v3) << 16);
+                const float2 h01 = e4m3x2_to_float2(h[j]), h23 = e4m3x2_to_float2(h[j] >> 16);
+                l[j] = e4m3x2(v0 - h01.x, v1 - h01.y) | (e4m3x2(v2 - h23.x, v3 - h23.y) << 16);
+                if (bad) h[j] = 0x7F7F7F7Fu, l[j] = 0u;  // a NaN or Inf makes the row NaN
+            }
+            const uint32_t to = (d0 >> 7) * (2u * R * 128u) + r * 128u + ((((d0 & 127u) >> 4) ^ (r & 7u)) << 4) + (d0 & 8u);
+            *reinterpret_cast<uint2*>(dst + to) = make_uint2(h[0], h[1]);
+            *reinterpret_cast<uint2*>(dst + to + R * 128u) = make_uint2(l[0], l[1]);
+            if (d0 == 0u) {
+                const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
+                // (positive, so that a masked score stays -inf; at 1e-30 scores are zero all the same)
+                frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
+                qpos[col] = pc.plan.p0 + static_cast<int32_t>((pc.row_tile * R + r) / a.shape.group);
+            }
+        }
+    }
+    fence_async_smem();
+}
 
 template <int R, int DC>
 __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
     attend_mma_kernel(const __grid_constant__ MmaArgs args, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<R, DC>;
-    constexpr int NS = C::kStages;
+    constexpr int NK = C::kNK, NV = C::kNV, V = C::V;
+    constexpr uint32_t kFull = 0xFFFFFFFFu;
     extern __shared__ uint8_t raw[];
     __shared__ Shared<R, DC> sh;
+    static_assert(sizeof(Shared<R, DC>) <= C::kSmall, "small arrays");
     const AttnArgs& a = args.a;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t shift = a.g.page_shift, D = a.g.head_dim;
     uint8_t* dyn = raw + ((1024u - (s32(raw) & 1023u)) & 1023u);
-    uint8_t* stages = dyn;
-    uint8_t* qbuf = dyn + NS * C::kStage;
+    uint8_t* kbuf = dyn;
+    uint8_t* vbuf = kbuf + NK * C::kBuf;
+    uint8_t* qbuf = vbuf + NV * C::kBuf;
     uint8_t* wbuf = qbuf + 2u * C::kQ;
     volatile uint32_t* gave_up = &sh.gave_up;
 
     if (tid == 0) {
-        for (int i = 0; i < NS; ++i) {
-            bar_init(&sh.kfull[i], 33);  // the expected bytes, and the 32 lanes that copy scales
-            bar_init(&sh.vfull[i], 1);
-            bar_init(&sh.empty[i], 1);
-        }
+        for (int i = 0; i < NK; ++i) bar_init(&sh.kfull[i], 1);
+        for (int i = 0; i < NV; ++i) bar_init(&sh.vfull[i], 1), bar_init(&sh.scfull[i], 32);
+        for (int i = 0; i < kRing; ++i) bar_init(&sh.sfull[i], 1), bar_init(&sh.ofull[i], 1);
         for (int i = 0; i < 2; ++i) {
-            bar_init(&sh.sfull[i], 1);
-            bar_init(&sh.sempty[i], 4 * C::kGroups);
-            bar_init(&sh.wfull[i], 4 * C::kGroups);
-            bar_init(&sh.ofull[i], 1);
+            bar_init(&sh.sempty[i], 4);
+            bar_init(&sh.wfull[i], 4);
             bar_init(&sh.oempty[i], 4);
-            bar_init(&sh.qfull[i], 2);
+            bar_init(&sh.qfull[i], 1);
             bar_init(&sh.qempty[i], 1);
         }
-        for (int i = 0; i < kQSlots; ++i) bar_init(&sh.rfull[i], 2);
-        for (int i = 0; i < 3; ++i) bar_init(&sh.meet[i], 4);
-        bar_init(&sh.lfull, 4 * C::kGroups);
+        for (int i = 0; i < kQSlots; ++i) bar_init(&sh.rfull[i], 1);
+        bar_init(&sh.lfull, 8);
         bar_init(&sh.lempty, 4);
-        bar_init(&sh.done, 1);
+        bar_init(&sh.done, 2);
         sh.gave_up = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -252,21 +401,27 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
     PieceWalk walk;
     uint64_t total;
     uint32_t ctas;
-    const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &walk, &total, &ctas);
     tc_before();
-    __syncthreads();
-    tc_after();
+    const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &walk, &total, &ctas);
+    tc_after();  // (walk_init's barriers have ordered the allocation and the barriers' set-up)
     const uint32_t tmem = sh.tmem;
 
     if (busy) {
         Piece pc;
+        if (warp != 0) {
+            // the first piece's queries: by every warp but the copying one, which starts at once
+            PieceWalk w = walk;
+            if (next_piece(a.shape, a.b, shift, w, &pc))
+                stage_queries<R, DC, (R * DC / 2 + 14) / 15>(args, pc, qbuf, sh.frow[0], sh.qpos[0], warp - 1u, 15u);
+            asm volatile("bar.sync 4, 480;" ::: "memory");
+        }
         if (warp == 0) {
-            // ---- pages: one lane per page of a tile ----
-            const uint32_t ppt = args.pages_per_tile;
+            // ---- pages: lanes 0-7 copy a tile's pages of keys, 8-15 of values, the others their scales ----
+            const uint32_t ppt = args.pages_per_tile, per_window = 32u / ppt;
             const uint32_t none = a.g.n_pages * a.g.n_heads;  // a coordinate past the end: zeros
+            const uint32_t slot = lane & 7u;
             uint32_t n = 0;
-            bool on = true;
-            while (on && next_piece(a.shape, a.b, shift, walk, &pc)) {
+            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
                 const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
                 const uint32_t n_pg = (static_cast<uint32_t>(pc.plan.len) + a.g.page_size - 1u) >> shift;
                 uint32_t lo_pg = 0;  // pages wholly before the window of the unit's first row are not read
@@ -275,195 +430,182 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                                        static_cast<int32_t>(a.shape.window) + 1;
                     lo_pg = lo > 0 ? static_cast<uint32_t>(lo) >> shift : 0u;
                 }
-                // page ids a tile ahead
-                const uint32_t slot = lane & 7u;
-                uint32_t idx = static_cast<uint32_t>(pc.t0) * ppt + slot;
-                int32_t id = slot < ppt && idx < n_pg && idx >= lo_pg ? table[idx] : -1;
+                // 32 page ids at a time, the next 32 asked for before they are needed
+                uint32_t idx = static_cast<uint32_t>(pc.t0) * ppt + lane;
+                int32_t ids = -1, ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t st = n % NS;
+                    const uint32_t in = static_cast<uint32_t>(t - pc.t0) % per_window;
+                    if (in == 0) {
+                        ids = ids_next;
+                        idx += 32u;
+                        ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
+                    }
+                    const int32_t id = __shfl_sync(kFull, ids, in * ppt + (slot & (ppt - 1u)));
                     const bool good = static_cast<uint32_t>(id) < a.g.n_pages;
                     const uint32_t z = good ? static_cast<uint32_t>(id) * a.g.n_heads + pc.head : none;
-                    idx += ppt;
-                    id = t + 1 < pc.t1 && slot < ppt && idx < n_pg && idx >= lo_pg ? table[idx] : -1;
-                    if (n >= NS && !bar_wait(&sh.empty[st], ((n / NS) - 1u) & 1u, gave_up)) {
-                        on = false;
+                    const uint32_t ks = n % NK, vs = n % NV;
+                    if (n >= NK) bar_wait(&sh.sfull[(n - NK) % kRing], ((n - NK) / kRing) & 1u, gave_up);
+                    if (*gave_up) break;
+                    if (lane == 0) bar_expect(&sh.kfull[ks], C::kBuf);
+                    __syncwarp();
+                    if (lane < ppt) {
+#pragma unroll
+                        for (int c = 0; c < DC; ++c)
+                            tma_page(&k_map, kbuf + ks * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &sh.kfull[ks],
+                                     c * 128, z);
+                    }
+                    if (n >= NV) bar_wait(&sh.ofull[(n - NV) % kRing], ((n - NV) / kRing) & 1u, gave_up);
+                    if (*gave_up) {
+                        ++n;  // the keys' copy is in flight
                         break;
                     }
-                    uint8_t* dst = stages + st * C::kStage;
-                    if (lane == 0) {
-                        bar_expect(&sh.kfull[st], DC * C::kChunk);
-                        bar_expect(&sh.vfull[st], DC * C::kChunk);
-                    }
+                    if (lane == 0) bar_expect(&sh.vfull[vs], C::kBuf);
                     __syncwarp();
-                    if (lane < 8u) {
-                        if (slot < ppt) {
+                    if (lane >= 8u && lane < 8u + ppt) {
 #pragma unroll
-                            for (int c = 0; c < DC; ++c)
-                                tma_page(&k_map, dst + c * C::kChunk + slot * a.g.page_size * 128u, &sh.kfull[st], c * 128, z);
-                        }
-                    } else if (lane < 16u) {
-                        if (slot < ppt) {
-#pragma unroll
-                            for (int c = 0; c < DC; ++c)
-                                tma_page(&v_map, dst + (DC + c) * C::kChunk + slot * a.g.page_size * 128u, &sh.vfull[st],
-                                         c * 128, z);
-                        }
-                    } else {
+                        for (int c = 0; c < DC; ++c)
+                            tma_page(&v_map, vbuf + vs * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &sh.vfull[vs],
+                                     c * 128, z);
+                    } else if (lane >= 16u) {
                         const bool is_v = lane >= 24u;
                         const float* src = (is_v ? a.g.v_scales : a.g.k_scales) + (good ? z : 0u);
                         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                         s32(is_v ? &sh.vscale[st][slot] : &sh.kscale[st][slot])),
+                                         s32(is_v ? &sh.vscale[vs][slot] : &sh.kscale[vs][slot])),
                                      "l"(src), "r"(good ? 4u : 0u)
                                      : "memory");
                     }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.kfull[st])) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.scfull[vs])) : "memory");
                 }
+                if (*gave_up) break;
             }
             if (*gave_up) {  // the copies in flight land before the shared memory is given back
-                for (uint32_t i = n > NS ? n - NS : 0u; i < n; ++i) {
-                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.kfull[i % NS], (i / NS) & 1u); ++w) {}
-                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.vfull[i % NS], (i / NS) & 1u); ++w) {}
-                }
+                for (uint32_t i = n > NK ? n - NK : 0u; i < n; ++i)
+                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.kfull[i % NK], (i / NK) & 1u); ++w) {}
+                for (uint32_t i = n > NV ? n - NV : 0u; i < n; ++i)
+                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.vfull[i % NV], (i / NV) & 1u); ++w) {}
+                asm volatile("cp.async.wait_all;" ::: "memory");
             }
         } else if (warp == 1) {
-            // ---- products: the scores of tile n, then the output of tile n - 1 ----
-            const uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(R >> 3) << 17) | (8u << 24);
-            const uint32_t idesc_o = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
+            // ---- scores: hi and lo rows of the queries are one operand of 2 R rows ----
+            const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
             const uint32_t ksteps = (D + 31u) / 32u;
+            const uint64_t k_desc = desc_sw128(s32(kbuf)), q_desc = desc_sw128(s32(qbuf));
             uint32_t n = 0, np = 0;
-            bool on = true;
-            auto output = [&](uint32_t m) {
-                const uint32_t st = m % NS, b = m & 1u;
-                if (!bar_wait(&sh.vfull[st], (m / NS) & 1u, gave_up)) return false;
-                if (!bar_wait(&sh.wfull[b], (m >> 1) & 1u, gave_up)) return false;
-                if (m >= 2 && !bar_wait(&sh.oempty[b], ((m >> 1) - 1u) & 1u, gave_up)) return false;
-                tc_after();
-                if (lane == 0) {
-                    const uint32_t v = s32(stages + st * C::kStage + DC * C::kChunk), w = s32(wbuf + b * C::kW);
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) {
-                        const uint32_t d = tmem + 2u * R + (b * DC + c) * 2u * R;
-#pragma unroll
-                        for (int k = 0; k < kTile / 32; ++k)
-                            mma_f8(d, desc_sw128(v + c * C::kChunk + k * 4096u), desc_plain(w + k * 512u, 128u, 16u * kTile),
-                                   idesc_o, k > 0);
-                    }
-                    tc_commit(&sh.ofull[b]);
-                    tc_commit(&sh.empty[st]);
-                }
-                __syncwarp();
-                return true;
-            };
-            while (on && next_piece(a.shape, a.b, shift, walk, &pc)) {
+            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
                 const uint32_t qb = np & 1u;
-                if (!bar_wait(&sh.qfull[qb], (np >> 1) & 1u, gave_up)) break;
+                bar_wait(&sh.qfull[qb], (np >> 1) & 1u, gave_up);
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t st = n % NS, b = n & 1u;
-                    on = bar_wait(&sh.kfull[st], (n / NS) & 1u, gave_up) &&
-                         (n < 2 || bar_wait(&sh.sempty[b], ((n >> 1) - 1u) & 1u, gave_up));
-                    if (!on) break;
+                    const uint32_t ks = n % NK, b = n & 1u;
+                    bar_wait(&sh.kfull[ks], (n / NK) & 1u, gave_up);
+                    if (n >= 2) bar_wait(&sh.sempty[b], ((n >> 1) - 1u) & 1u, gave_up);
                     tc_after();
-                    if (lane == 0) {
-                        const uint32_t k0 = s32(stages + st * C::kStage), q0 = s32(qbuf + qb * C::kQ);
-                        for (uint32_t part = 0; part < 2; ++part)
-                            for (uint32_t k = 0; k < ksteps; ++k)
-                                mma_f8(tmem + b * R, desc_sw128(k0 + (k >> 2) * C::kChunk + (k & 3u) * 32u),
-                                       desc_sw128(q0 + (k >> 2) * (2u * R * 128u) + part * (R * 128u) + (k & 3u) * 32u), idesc_s,
-                                       part + k > 0);
-                        tc_commit(&sh.sfull[b]);
+                    if (__any_sync(kFull, *gave_up != 0u)) continue;
+                    const uint64_t kd = k_desc + ks * (C::kBuf >> 4), qd = q_desc + qb * (C::kQ >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4 * DC; ++k)
+                            if (static_cast<uint32_t>(k) < ksteps)
+                                mma_f8(tmem + b * 2u * R, kd + (((k >> 2) * C::kChunk + (k & 3) * 32u) >> 4),
+                                       qd + (((k >> 2) * (2u * R * 128u) + (k & 3) * 32u) >> 4), idesc, k > 0);
+                    }
+                    __syncwarp();
+                    if (elect_one()) {
+                        tc_commit(&sh.sfull[n % kRing]);
                         if (t + 1 == pc.t1) tc_commit(&sh.qempty[qb]);
                     }
                     __syncwarp();
-                    if (n > 0) on = output(n - 1);
-                    if (!on) break;
                 }
                 ++np;
             }
-            if (on && n > 0 && !*gave_up) output(n - 1);
-        } else if (warp < 4) {
-            // ---- queries: a warp per row, split into two e4m3 terms ----
+        } else if (warp == 2) {
+            // ---- outputs: hi and lo columns of the weights are one operand of 2 R columns ----
+            const uint32_t idesc = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
+            const uint64_t v_desc = desc_sw128(s32(vbuf)), w_desc = desc_plain(s32(wbuf), 128u, 16u * kTile);
+            uint32_t n = 0;
+            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+                for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
+                    const uint32_t vs = n % NV, b = n & 1u;
+                    bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
+                    // (the softmax has waited for the output buffer to be free)
+                    bar_wait(&sh.wfull[b], (n >> 1) & 1u, gave_up);
+                    tc_after();
+                    if (__any_sync(kFull, *gave_up != 0u)) continue;
+                    const uint64_t vd = v_desc + vs * (C::kBuf >> 4), wd = w_desc + b * (C::kW >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < DC; ++c)
+#pragma unroll
+                            for (int k = 0; k < kTile / 32; ++k)
+                                mma_f8(tmem + 4u * R + (b * DC + c) * 2u * R, vd + ((c * C::kChunk + k * 4096u) >> 4),
+                                       wd + ((k * 512u) >> 4), idesc, k > 0);
+                    }
+                    __syncwarp();
+                    if (elect_one()) tc_commit(&sh.ofull[n % kRing]);
+                    __syncwarp();
+                }
+            }
+        } else if (warp == 3) {
+            // ---- queries of the pieces after the first ----
             uint32_t np = 0;
             while (next_piece(a.shape, a.b, shift, walk, &pc)) {
-                const uint32_t qb = np & 1u, slot = np % kQSlots;
-                if (np >= 2 && !bar_wait(&sh.qempty[qb], ((np >> 1) - 1u) & 1u, gave_up)) break;
-                uint8_t* dst = qbuf + qb * C::kQ;
-                for (uint32_t r = warp - 2u; r < R; r += 2u) {
-                    const uint32_t rr = pc.row_tile * R + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
-                    const int32_t pos = pc.plan.p0 + static_cast<int32_t>(tok);
-                    const bool valid = r < pc.rows;
-                    float x[DC][4];
-                    float m = 0.0f;
-                    bool bad = false;
-#pragma unroll
-                    for (int c = 0; c < DC; ++c)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t d = c * 128u + lane * 4u + j;
-                            x[c][j] = 0.0f;
-                            if (valid && d < D) {
-                                const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) +
-                                                         (pc.plan.row0 + tok) * a.q.token_stride +
-                                                         (pc.head * a.shape.group + g) * a.q.head_stride;
-                                load_turned<__nv_bfloat16, 1>(a.rope, p, d, pos, &x[c][j]);
-                                // a turned query is rounded to its type, as a rotation of its own would
-                                x[c][j] = __bfloat162float(__float2bfloat16_rn(x[c][j]));
-                            }
-                            const float ab = fabsf(x[c][j]);
-                            if (ab < __builtin_huge_valf()) m = fmaxf(m, ab);
-                            else bad = true;
-                        }
-                    m = warp_max(m);
-                    bad = __any_sync(0xFFFFFFFFu, bad);
-                    const int e = kv_scale_exp(m);
-                    const float mul = exp2_int(-e);
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) {
-                        const float v0 = x[c][0] * mul, v1 = x[c][1] * mul, v2 = x[c][2] * mul, v3 = x[c][3] * mul;
-                        uint32_t h = e4m3x2(v0, v1) | (e4m3x2(v2, v3) << 16);
-                        const float2 h01 = e4m3x2_to_float2(h), h23 = e4m3x2_to_float2(h >> 16);
-                        uint32_t l = e4m3x2(v0 - h01.x, v1 - h01.y) | (e4m3x2(v2 - h23.x, v3 - h23.y) << 16);
-                        if (bad) h = 0x7F7F7F7Fu, l = 0u;  // a NaN or Inf makes the row NaN
-                        const uint32_t at = c * (2u * R * 128u) + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u;
-                        *reinterpret_cast<uint32_t*>(dst + at) = h;
-                        *reinterpret_cast<uint32_t*>(dst + at + R * 128u) = l;
-                    }
-                    if (lane == 0) {
-                        sh.frow[slot][r] = exp2_int(e) * (a.scale * kLog2e);
-                        sh.qpos[slot][r] = valid ? pos : (-2147483647 - 1);
-                    }
-                }
-                fence_async_smem();
+                const uint32_t qb = np & 1u, rs = np % kQSlots;
+                if (np >= 2) bar_wait(&sh.qempty[qb], ((np >> 1) - 1u) & 1u, gave_up);
+                if (np > 0) stage_queries<R, DC, 4>(args, pc, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], 0u, 1u);
                 __syncwarp();
                 if (lane == 0) {
                     bar_arrive(&sh.qfull[qb]);
-                    bar_arrive(&sh.rfull[slot]);
+                    bar_arrive(&sh.rfull[rs]);
                 }
                 ++np;
             }
         } else if (warp < 8) {
             // ---- output sums: thread d of a chunk holds element d of every row ----
             const uint32_t quad = warp & 3u, d0 = quad * 32u + lane;
-            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + 2u * R;
-            uint32_t n = 0, np = 0, meets = 0;
-            bool on = true;
-            while (on && next_piece(a.shape, a.b, shift, walk, &pc)) {
-                float acc[DC][R];
+            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + 4u * R;
+            constexpr int kPer = R > 32 ? 2 : 1;  // columns of a lane where columns are dealt to lanes
+            float* fac = sh.fac[quad];
+            float* facold = sh.facold[quad];
+            uint32_t n = 0, np = 0;
+            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+                F2 acc[DC][R / 2];
 #pragma unroll
                 for (int c = 0; c < DC; ++c)
 #pragma unroll
-                    for (int r = 0; r < R; ++r) acc[c][r] = 0.0f;
+                    for (int r = 0; r < R / 2; ++r) acc[c][r] = f2(0.0f, 0.0f);
+                float M[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) M[i] = kNegInf;
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
                     const uint32_t b = n & 1u;
-                    // (the weights' barrier, long complete, orders the factors that the softmax wrote)
-                    if (!bar_wait(&sh.ofull[b], (n >> 1) & 1u, gave_up) || !bar_wait(&sh.wfull[b], (n >> 1) & 1u, gave_up)) {
-                        on = false;
-                        break;
+                    // the weights' barrier orders the factors that the softmax wrote
+                    bar_wait(&sh.wfull[b], (n >> 1) & 1u, gave_up);
+                    bool changed = false;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) {
+                        const uint32_t col = lane + 32u * i;
+                        if (col < R) {
+                            const float mg = sh.mgrp[b][col], m1 = fmaxf(M[i], mg);
+                            fac[col] = sh.osc[b][col] * (mg == m1 ? 1.0f : ex2(mg - m1));
+                            const float al = M[i] == m1 ? 1.0f : ex2(M[i] - m1);
+                            facold[col] = al;
+                            changed |= al != 1.0f;
+                            M[i] = m1;
+                        }
                     }
+                    changed = __any_sync(kFull, changed);
+                    __syncwarp();
+                    if (changed) {
+#pragma unroll
+                        for (int r = 0; r < R / 2; ++r) {
+                            const float2 al = *reinterpret_cast<const float2*>(facold + 2 * r);
+#pragma unroll
+                            for (int c = 0; c < DC; ++c) acc[c][r] = mul2(acc[c][r], f2(al.x, al.y));
+                        }
+                    }
+                    bar_wait(&sh.ofull[n % kRing], (n / kRing) & 1u, gave_up);
                     tc_after();
-                    const bool changed = (sh.changed[b][0] | sh.changed[b][C::kGroups - 1]) != 0u;
 #pragma unroll
                     for (int r = 0; r < R; r += 8) {
-                        if (static_cast<uint32_t>(r) >= pc.rows) break;
                         float o[DC][8], o_lo[DC][8];
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
@@ -471,87 +613,98 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                             tmem_ld8(t_lane + (b * DC + c) * 2u * R + R + r, o_lo[c]);
                         }
                         tmem_wait_ld();
-                        if (changed) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float al = sh.alpha[b][r + j];
-#pragma unroll
-                                for (int c = 0; c < DC; ++c) acc[c][r + j] *= al;
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float f = sh.osc[b][r + j];
+                        for (int j = 0; j < 8; j += 2) {
+                            const float2 f = *reinterpret_cast<const float2*>(fac + r + j);
 #pragma unroll
                             for (int c = 0; c < DC; ++c)
-                                acc[c][r + j] = fmaf(fmaf(o_lo[c][j], kLoInv, o[c][j]), f, acc[c][r + j]);
+                                acc[c][(r + j) / 2] = fma2(fma2(f2(o_lo[c][j], o_lo[c][j + 1]), f2(kLoInv, kLoInv), f2(o[c][j], o[c][j + 1])),
+                                                           f2(f.x, f.y), acc[c][(r + j) / 2]);
                         }
                     }
                     tc_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh.oempty[b]);
                 }
-                if (!on || !bar_wait(&sh.lfull, np & 1u, gave_up)) {
-                    on = false;
-                    break;
+                bar_wait(&sh.lfull, np & 1u, gave_up);
+                // the rows' sums, in facold; their maxima stay with the lanes, and go to fac
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const uint32_t col = lane + 32u * i;
+                    if (col < R) {
+                        float l = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float mg = sh.mfin[g][col];
+                            l += (sh.lsum[g][0][col] + sh.lsum[g][1][col] + sh.lsum[g][2][col] + sh.lsum[g][3][col]) *
+                                 (mg == M[i] ? 1.0f : ex2(mg - M[i]));
+                        }
+                        facold[col] = l;
+                        fac[col] = M[i];
+                    }
                 }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh.lempty);
                 const bool whole = pc.t0 == pc.first && pc.t1 == pc.end;
                 const uint32_t r_base = pc.row_tile * R, group = a.shape.group;
                 const uint32_t q_heads = a.shape.n_heads * group;
                 float* part = a.part + (2ull * blockIdx.x + (pc.t0 == pc.first ? 1u : 0u)) * a.part_stride;
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if (static_cast<uint32_t>(r) >= pc.rows) break;
-                    const float l = sh.lsum[0][r] + sh.lsum[1][r] + sh.lsum[2][r] + sh.lsum[3][r];
+                for (int col = 0; col < R; ++col) {
+                    const uint32_t r = ((col % V) >> 1) * 8 + (col / V) * 2 + (col & 1);
+                    if (r >= pc.rows) continue;
+                    const float l = facold[col];
+                    float y[DC];
+#pragma unroll
+                    for (int c = 0; c < DC; ++c) {
+                        const float2 p = un2(acc[c][col / 2]);
+                        y[c] = (col & 1) ? p.y : p.x;
+                    }
                     if (whole) {
                         const uint32_t tok = (r_base + r) / group, g = (r_base + r) - tok * group;
                         __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
                                            (pc.head * group + g) * a.out.head_stride;
-                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                        const float inv = 1.0f / l;
 #pragma unroll
                         for (int c = 0; c < DC; ++c)
-                            if (c * 128u + d0 < D)
-                                p[c * 128u + d0] = __float2bfloat16_rn(l == 0.0f ? 0.0f : acc[c][r] * inv);
+                            if (c * 128u + d0 < D) p[c * 128u + d0] = __float2bfloat16_rn(l == 0.0f ? 0.0f : y[c] * inv);
                         if (a.lse && d0 == 0u)
-                            a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (sh.mfin[r] + log2f(l)) * kLn2;
+                            a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (fac[col] + log2f(l)) * kLn2;
                     } else {
 #pragma unroll
                         for (int c = 0; c < DC; ++c)
-                            if (c * 128u + d0 < D) part[r * D + c * 128u + d0] = acc[c][r];
+                            if (c * 128u + d0 < D) part[r * D + c * 128u + d0] = y[c];
                         if (d0 == 0u) {
-                            part[kPartRows * D + r] = sh.mfin[r];
+                            part[kPartRows * D + r] = fac[col];
                             part[kPartRows * (D + 1u) + r] = l;
                         }
                     }
                 }
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sh.lempty);
                 ++np;
                 if (whole) continue;
                 // pieces of one unit meet: the last CTA to arrive joins them in CTA order
                 const uint32_t c0 = place_owner(pc.start, total, ctas);
                 const uint32_t c1 = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, total, ctas);
                 __threadfence();
-                on = warps_meet(&sh.meet[2], &meets, gave_up);
-                if (!on) break;
+                group_sync(1);
                 if (warp == 4 && lane == 0) {
                     sh.last_flag = atomicAdd(a.counter + c0, 1u) == c1 - c0 ? 1u : 0u;
                     if (sh.last_flag) a.counter[c0] = 0u;
                 }
-                on = warps_meet(&sh.meet[2], &meets, gave_up);
-                if (!on) break;
+                group_sync(1);
                 if (!sh.last_flag) continue;
                 __threadfence();
                 for (uint32_t r = 0; r < pc.rows; ++r) {
-                    float M = kNegInf, l = 0.0f, o[DC];
+                    float m = kNegInf, l = 0.0f, o[DC];
 #pragma unroll
                     for (int c = 0; c < DC; ++c) o[c] = 0.0f;
                     for (uint32_t c = c0; c <= c1; ++c)
-                        M = fmaxf(M, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r));
+                        m = fmaxf(m, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r));
                     for (uint32_t c = c0; c <= c1; ++c) {
                         const float* p = a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride;
-                        const float m = __ldcg(p + kPartRows * D + r);
-                        const float f = m == M ? 1.0f : exp2f(m - M);
+                        const float mc = __ldcg(p + kPartRows * D + r);
+                        const float f = mc == m ? 1.0f : exp2f(mc - m);
                         l += __ldcg(p + kPartRows * (D + 1u) + r) * f;
 #pragma unroll
                         for (int k = 0; k < DC; ++k)
@@ -564,154 +717,205 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     for (int k = 0; k < DC; ++k)
                         if (k * 128u + d0 < D) p[k * 128u + d0] = __float2bfloat16_rn(l == 0.0f ? 0.0f : o[k] / l);
                     if (a.lse && d0 == 0u)
-                        a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (M + log2f(l)) * kLn2;
+                        a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (m + log2f(l)) * kLn2;
                 }
             }
         } else {
-            // ---- softmax: a thread per token, its warpgroup's kCols rows ----
-            constexpr int NC = C::kCols;
-            const uint32_t quad = warp & 3u, grp = (warp - 8u) >> 2, tl = quad * 32u + lane, col0 = grp * NC;
-            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + col0;
+            // ---- softmax: group g takes the tiles n with n % 2 == g ----
+            const uint32_t quad = warp & 3u, grp = (warp - 8u) >> 2, q = lane & 3u, tr = lane >> 2;
+            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + grp * 2u * R;
+            const uint32_t pg0 = (quad * 32u) >> shift, pg1 = (quad * 32u + 16u) >> shift;
+            constexpr int kOwn = V > 8 ? V / 8 : 1;  // columns that a lane ends with where they are dealt out
+            const uint32_t own = q * V + first_of<V>(lane);
             float2* my_ref = sh.ref[warp - 8u];
-            uint32_t n = 0, np = 0, meets = 0;
-            bool on = true;
-            while (on && next_piece(a.shape, a.b, shift, walk, &pc)) {
-                const uint32_t slot = np % kQSlots;
-                if (!bar_wait(&sh.rfull[slot], (np / kQSlots) & 1u, gave_up)) break;
-                const float* frow = sh.frow[slot] + col0;
-                const int32_t* qpos = sh.qpos[slot] + col0;
-                const uint32_t cols = pc.rows > col0 ? min(pc.rows - col0, static_cast<uint32_t>(NC)) : 0u;
-                // tiles in [safe0, safe1) are inside every row's positions
+            float* my_rescale = sh.rescale[warp - 8u];
+            uint8_t* w0 = wbuf + grp * C::kW + (quad * 4u) * 128u + tr * 16u + ((q * V) >> 4) * (16u * kTile) + ((q * V) & 15u);
+            const auto max_op = [](float x, float y) { return fmaxf(x, y); };
+            const auto add_op = [](float x, float y) { return x + y; };
+            uint32_t n = 0, np = 0;
+            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+                const uint32_t rs = np % kQSlots;
+                bar_wait(&sh.rfull[rs], (np / kQSlots) & 1u, gave_up);
+                const float* frow = sh.frow[rs] + q * V;
+                const int32_t* qpos = sh.qpos[rs] + q * V;
+                // tiles in [safe_from, reach) are inside every row's positions
                 const int32_t p_first = pc.plan.p0 + static_cast<int32_t>(pc.row_tile * R / a.shape.group);
                 const int32_t p_last = pc.plan.p0 + static_cast<int32_t>((pc.row_tile * R + pc.rows - 1u) / a.shape.group);
                 const int32_t reach = a.shape.all ? pc.plan.len : min(pc.plan.len, p_first + 1);
                 const int32_t safe_from = a.shape.window ? p_last - static_cast<int32_t>(a.shape.window) + 1 : 0;
-                float l[NC];
+                float l[V];
 #pragma unroll
-                for (int c = 0; c < NC; ++c) l[c] = 0.0f;
-                float M = kNegInf;  // of row `lane`
+                for (int i = 0; i < V; ++i) l[i] = 0.0f;
+                float M[kOwn], f_own[kOwn];
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    M[i] = kNegInf;
+                    f_own[i] = sh.frow[rs][own + i];
+                }
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t st = n % NS, b = n & 1u;
-                    on = bar_wait(&sh.kfull[st], (n / NS) & 1u, gave_up) && bar_wait(&sh.sfull[b], (n >> 1) & 1u, gave_up);
-                    if (!on) break;
-                    tc_after();
-                    float x[NC];
-#pragma unroll
-                    for (int c = 0; c < NC; c += 8)
-                        if (static_cast<uint32_t>(c) < cols) tmem_ld8(t_lane + b * R + c, x + c);
-                    tmem_wait_ld();
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&sh.sempty[b]);
-                    const int32_t pos = t * kTile + static_cast<int32_t>(tl);
-                    const uint32_t pg = tl >> shift;
-                    const float fk = sh.kscale[st][pg];
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        if (static_cast<uint32_t>(c & ~7) < cols) x[c] *= fk * frow[c];
-                    if (t * kTile < safe_from || (t + 1) * kTile > reach) {
-                        const int32_t w = static_cast<int32_t>(a.shape.window);
-#pragma unroll
-                        for (int c = 0; c < NC; ++c)
-                            if (static_cast<uint32_t>(c & ~7) < cols) {
-                                const int32_t qp = qpos[c];
-                                bool ok = pos < pc.plan.len && (a.shape.all || pos <= qp);
-                                if (w) ok = ok && pos > qp - w;
-                                if (!ok) x[c] = kNegInf;
-                            }
-                    }
+                    if ((n & 1u) != grp) continue;
+                    const uint32_t vs = n % NV, use = n >> 1;
+                    float(*wmax)[R] = sh.wmax[grp][use & 1u];  // (its last readers met since)
+                    bar_wait(&sh.scfull[vs], (n / NV) & 1u, gave_up);
+                    const float fk0 = sh.kscale[vs][pg0], fk1 = sh.kscale[vs][pg1];
                     // exponents of the values' scales, relative to the tile's largest: they go into the weights.
                     // Where they differ by much, the weights' factor has to come from the largest product of
                     // weight and scale: the largest weight's own value could be below others' rounding.
-                    const int ep = lane < args.pages_per_tile ? scale_exp_of(sh.vscale[st][lane & 7u]) : -127;
-                    const int er = __reduce_max_sync(0xFFFFFFFFu, ep);
-                    const bool wide = __any_sync(0xFFFFFFFFu, ep > -127 && ep < er - 4);
-                    const int ev = scale_exp_of(sh.vscale[st][pg]);
-                    const float vr = exp2_int(max(ev - er, -126));
-                    // the tile's maximum of every row: lane c ends with row c's
-                    float mine = kNegInf;
+                    const int ep = scale_exp_of(sh.vscale[vs][lane & (args.pages_per_tile - 1u)]);
+                    int er = ep;
+                    er = max(er, __shfl_xor_sync(kFull, er, 4));
+                    er = max(er, __shfl_xor_sync(kFull, er, 2));
+                    er = max(er, __shfl_xor_sync(kFull, er, 1));
+                    const bool wide = __any_sync(kFull, ep > -127 && ep < er - 4);
+                    const int ev0 = max(scale_exp_of(sh.vscale[vs][pg0]) - er, -126);
+                    const int ev1 = max(scale_exp_of(sh.vscale[vs][pg1]) - er, -126);
+                    const bool edge = t * kTile < safe_from || (t + 1) * kTile > reach;
+                    bar_wait(&sh.sfull[n % kRing], (n / kRing) & 1u, gave_up);
+                    tc_after();
+                    float x[V / 2][2][4];  // [8-column block][column][token]
 #pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        if (static_cast<uint32_t>(c & ~7) < cols) {
-                            const float m = warp_max(x[c]);
-                            if (lane == static_cast<uint32_t>(c)) mine = m;
+                    for (int j = 0; j < V / 2; ++j) {
+                        float f[8], g[8];
+                        tmem_ld_frag(t_lane + 8 * j, f);
+                        tmem_ld_frag(t_lane + (16u << 16) + 8 * j, f + 4);
+                        tmem_ld_frag(t_lane + R + 8 * j, g);
+                        tmem_ld_frag(t_lane + (16u << 16) + R + 8 * j, g + 4);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float fk = i < 2 ? fk0 : fk1;
+                            const float2 y = un2(mul2(add2(f2(f[2 * i], f[2 * i + 1]), f2(g[2 * i], g[2 * i + 1])), f2(fk, fk)));
+                            x[j][0][i] = y.x, x[j][1][i] = y.y;
                         }
-                    if (lane < NC) sh.wmax[b][grp][quad][lane] = mine;
-                    if (wide) {  // see below: the largest weight times scale, too
-                        float mine2 = kNegInf;
-#pragma unroll
-                        for (int c = 0; c < NC; ++c)
-                            if (static_cast<uint32_t>(c & ~7) < cols) {
-                                const float m = warp_max(x[c] + static_cast<float>(max(ev - er, -126)));
-                                if (lane == static_cast<uint32_t>(c)) mine2 = m;
-                            }
-                        if (lane < NC) sh.wmax2[grp][quad][lane] = mine2;
                     }
-                    on = warps_meet(&sh.meet[grp], &meets, gave_up);
-                    if (!on) break;
-                    float mt = kNegInf;
-                    if (lane < NC) {
-                        mt = fmaxf(fmaxf(sh.wmax[b][grp][0][lane], sh.wmax[b][grp][1][lane]),
-                                   fmaxf(sh.wmax[b][grp][2][lane], sh.wmax[b][grp][3][lane]));
-                    }
-                    const float m1 = fmaxf(M, mt);
-                    const float alpha = M == m1 ? 1.0f : ex2(M - m1);
-                    // weights e^(x - m1) times 2^(k + 8), k such that the tile's largest is in (128, 256]
-                    if (wide) {
-                        if (lane < NC)
-                            mt = fmaxf(fmaxf(sh.wmax2[grp][0][lane], sh.wmax2[grp][1][lane]),
-                                       fmaxf(sh.wmax2[grp][2][lane], sh.wmax2[grp][3][lane]));
-                        on = warps_meet(&sh.meet[grp], &meets, gave_up);
-                        if (!on) break;
-                    }
-                    const float gap = m1 - mt;
-                    const int k = gap < 100.0f ? static_cast<int>(gap) : (mt == kNegInf ? 0 : 100);
+                    tc_before();
                     __syncwarp();
-                    if (lane < NC) my_ref[lane] = make_float2(m1 == kNegInf ? 0.0f : m1, exp2_int(k + 8));
-                    const bool changed = __any_sync(0xFFFFFFFFu, alpha != 1.0f);
-                    if (quad == 0) {
-                        if (n >= 2 && !bar_wait(&sh.oempty[b], ((n >> 1) - 1u) & 1u, gave_up)) {
-                            on = false;
-                        } else {
-                            if (lane < NC) {
-                                sh.osc[b][col0 + lane] = exp2_int(max(er, -126)) * exp2_int(-k - 8);
-                                sh.alpha[b][col0 + lane] = alpha;
+                    if (lane == 0) bar_arrive(&sh.sempty[grp]);
+                    if (edge) {
+                        const int32_t w = static_cast<int32_t>(a.shape.window);
+#pragma unroll
+                        for (int c = 0; c < V; ++c) {
+                            const int32_t qp = qpos[c];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int32_t pos = t * kTile + static_cast<int32_t>(quad * 32u + i * 8u + tr);
+                                bool ok = pos < pc.plan.len && (a.shape.all || pos <= qp);
+                                if (w) ok = ok && pos > qp - w;
+                                if (!ok) x[c >> 1][c & 1][i] = kNegInf;
                             }
-                            if (lane == 0) sh.changed[b][grp] = changed ? 1u : 0u;
                         }
                     }
+                    // the tile's maximum of every row: within the thread, over its warp, over the group
+                    float mx[V];
+#pragma unroll
+                    for (int c = 0; c < V; ++c)
+                        mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]), fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]));
+                    fold_lanes<V>(mx, lane, max_op);
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
+                    group_sync(2 + grp);
+                    float mt[kOwn];
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i)
+                        mt[i] = fmaxf(fmaxf(wmax[0][own + i], wmax[1][own + i]),
+                                      fmaxf(wmax[2][own + i], wmax[3][own + i])) * f_own[i];
+                    float mw[kOwn];  // of weight times value scale
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) mw[i] = mt[i];
+                    if (wide) {
+#pragma unroll
+                        for (int c = 0; c < V; ++c)
+                            mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]) * frow[c] + static_cast<float>(ev0),
+                                          fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]) * frow[c] + static_cast<float>(ev1));
+                        fold_lanes<V>(mx, lane, max_op);
+                        group_sync(2 + grp);  // the first maxima have been read
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
+                        group_sync(2 + grp);
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i)
+                            mw[i] = fmaxf(fmaxf(wmax[0][own + i], wmax[1][own + i]),
+                                          fmaxf(wmax[2][own + i], wmax[3][own + i]));
+                    }
+                    // weights e^(x - m1) times 2^k, k such that the tile's largest is in (1/2, 1]
+                    bool changed = false;
+                    float alpha[kOwn];
+                    int k[kOwn];
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) {
+                        const float m1 = fmaxf(M[i], mt[i]);
+                        alpha[i] = M[i] == m1 ? 1.0f : ex2(M[i] - m1);
+                        changed |= alpha[i] != 1.0f;
+                        const float gap = m1 - mw[i];
+                        k[i] = gap < 100.0f ? static_cast<int>(gap) : (mw[i] == kNegInf ? 0 : 100);
+                        my_ref[own + i] = make_float2(m1 == kNegInf ? 0.0f : -m1, exp2_int(k[i]));
+                        M[i] = m1;
+                    }
+                    changed = __any_sync(kFull, changed);
                     if (changed) {
 #pragma unroll
-                        for (int c = 0; c < NC; ++c) l[c] *= __shfl_sync(0xFFFFFFFFu, alpha, c);
+                        for (int i = 0; i < kOwn; ++i) my_rescale[own + i] = alpha[i];
+                        __syncwarp();
+#pragma unroll
+                        for (int c = 0; c < V; ++c) l[c] *= my_rescale[q * V + c];
                     }
-                    M = m1;
                     __syncwarp();
-                    if (on && n >= 2) on = bar_wait(&sh.ofull[b], ((n >> 1) - 1u) & 1u, gave_up);  // the weights' buffer
-                    if (!on) break;
-                    uint8_t* w0 = wbuf + b * C::kW + (tl >> 3) * 128u + (tl & 7u) * 16u;
+                    if (use >= 1) bar_wait(&sh.ofull[(n - 2u) % kRing], ((n - 2u) / kRing) & 1u, gave_up);  // the weights' buffer is free
+                    const float vr0 = exp2_int(ev0), vr1 = exp2_int(ev1);
+                    uint32_t hi[4][(V + 3) / 4], lo[4][(V + 3) / 4];
 #pragma unroll
-                    for (int c = 0; c < NC; c += 8) {
-                        if (static_cast<uint32_t>(c) >= cols) break;
-                        uint32_t hi[4], lo[4];
+                    for (int j = 0; j < V / 2; ++j) {
+                        const float4 rf = *reinterpret_cast<const float4*>(my_ref + q * V + 2 * j);
+                        const float2 fr = *reinterpret_cast<const float2*>(frow + 2 * j);
+                        const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z);
+                        const F2 wf0 = mul2(f2(rf.y, rf.w), f2(vr0, vr0)), wf1 = mul2(f2(rf.y, rf.w), f2(vr1, vr1));
+                        F2 sum = f2(l[2 * j], l[2 * j + 1]);
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const float2 r0 = my_ref[c + j], r1 = my_ref[c + j + 1];
-                            const float p0 = ex2(x[c + j] - r0.x), p1 = ex2(x[c + j + 1] - r1.x);
-                            l[c + j] += p0;
-                            l[c + j + 1] += p1;
-                            split2(p0 * (r0.y * vr), p1 * (r1.y * vr), &hi[j / 2], &lo[j / 2]);
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 y = un2(fma2(f2(x[j][0][i], x[j][1][i]), scale2, minus));
+                            const F2 p = f2(ex2(y.x), ex2(y.y));
+                            sum = add2(sum, p);
+                            uint32_t h, g;
+                            split2(mul2(p, i < 2 ? wf0 : wf1), &h, &g);
+                            if (j & 1) {
+                                hi[i][j / 2] = __byte_perm(hi[i][j / 2], h, 0x6420);
+                                lo[i][j / 2] |= g << 16;
+                            } else {
+                                hi[i][j / 2] = h;
+                                lo[i][j / 2] = g;
+                            }
                         }
-                        const uint32_t col = col0 + c;
-                        uint8_t* wp = w0 + (col >> 4) * (16u * kTile) + (col & 8u);
-                        *reinterpret_cast<uint2*>(wp) = make_uint2(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16));
-                        *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+                        const float2 s2 = un2(sum);
+                        l[2 * j] = s2.x, l[2 * j + 1] = s2.y;
                     }
-                    if ((t + 1) * kTile > pc.plan.len && grp == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint8_t* wp = w0 + i * 128;
+                        if constexpr (V == 4) {
+                            *reinterpret_cast<uint32_t*>(wp) = hi[i][0];
+                            *reinterpret_cast<uint32_t*>(wp + R * kTile) = lo[i][0];
+                        } else if constexpr (V == 8) {
+                            *reinterpret_cast<uint2*>(wp) = make_uint2(hi[i][0], hi[i][1]);
+                            *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(lo[i][0], lo[i][1]);
+                        } else {
+                            *reinterpret_cast<uint4*>(wp) = make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
+                            *reinterpret_cast<uint4*>(wp + R * kTile) = make_uint4(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                        }
+                    }
+                    if (quad == 0) {
+                        if (use >= 1) bar_wait(&sh.oempty[grp], (use - 1u) & 1u, gave_up);
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i) {
+                            sh.osc[grp][own + i] = exp2_int(max(er, -126)) * exp2_int(-k[i] - 8);
+                            sh.mgrp[grp][own + i] = M[i];
+                        }
+                    }
+                    if ((t + 1) * kTile > pc.plan.len) {
                         // what lies behind the sequence's end may hold NaN bytes, and 0 * NaN is NaN
-                        on = bar_wait(&sh.vfull[st], (n / NS) & 1u, gave_up);
-                        if (!on) break;
-                        if (pos >= pc.plan.len) {
-                            uint8_t* v = stages + st * C::kStage + DC * C::kChunk + tl * 128u;
+                        bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
+                        const uint32_t tok = quad * 32u + lane;
+                        if (t * kTile + static_cast<int32_t>(tok) >= pc.plan.len) {
+                            uint8_t* v = vbuf + vs * C::kBuf + tok * 128u;
 #pragma unroll
                             for (int c = 0; c < DC; ++c)
 #pragma unroll
@@ -721,23 +925,15 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     }
                     fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(&sh.wfull[b]);
+                    if (lane == 0) bar_arrive(&sh.wfull[grp]);
                 }
-                if (!on) break;
-                // the rows' sums over the warp's tokens: lane c ends with row c's
-                float mine = 0.0f;
+                // the rows' sums over the warp's tokens
+                fold_lanes<V>(l, lane, add_op);
+                if (np >= 1) bar_wait(&sh.lempty, (np - 1u) & 1u, gave_up);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    if (static_cast<uint32_t>(c & ~7) >= cols) continue;
-                    float s = l[c];
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-                    if (lane == static_cast<uint32_t>(c)) mine = s;
-                }
-                if (np >= 1 && !bar_wait(&sh.lempty, (np - 1u) & 1u, gave_up)) break;
-                if (lane < NC) {
-                    sh.lsum[quad][col0 + lane] = mine;
-                    if (quad == 0) sh.mfin[col0 + lane] = M;
+                for (int i = 0; i < kOwn; ++i) {
+                    sh.lsum[grp][quad][own + i] = l[i];
+                    if (quad == 0) sh.mfin[grp][own + i] = M[i];
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lfull);
@@ -745,23 +941,22 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
             }
         }
     }
-    if (warp == 2 || warp == 3) {
-        // statuses: a sequence per warp, over the grid
-        for (uint32_t s = blockIdx.x * 2u + (warp - 2u); s < a.b.n_seqs; s += gridDim.x * 2u) {
+    if (warp == 3) {
+        // statuses, over the grid
+        for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
             const bool ok = seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
-            const bool bad = __any_sync(0xFFFFFFFFu, !ok);
+            const bool bad = __any_sync(kFull, !ok);
             if (lane == 0) a.status[s] = bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK;
             __syncwarp();
         }
     }
-
     tc_before();
     __syncthreads();
     tc_after();
     if (sh.gave_up) {
         // never expected: the products in flight end (bounded) before their memory is given back
-        if (warp == 1) {
-            if (lane == 0) {
+        if (warp == 1 || warp == 2) {
+            if (elect_one()) {
                 tc_commit(&sh.done);
                 for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.done, 0u); ++w) {}
             }
@@ -828,6 +1023,10 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
     MmaArgs m;
     m.a = a;
     m.pages_per_tile = kTile / a.g.page_size;
+    m.q_vec = ((reinterpret_cast<uintptr_t>(a.q.data) | 2u * a.q.token_stride | 2u * a.q.head_stride) & 15u) == 0 &&
+                      rope_by_8(a.rope)
+                  ? 1u
+                  : 0u;
     const uint64_t rows = static_cast<uint64_t>(max_new ? max_new : 1u) * a.shape.group;
     if (a.g.head_dim <= 128) {
         if (rows <= 16) return launch<16, 1>(m, k_map, v_map, n_sms, stream);
