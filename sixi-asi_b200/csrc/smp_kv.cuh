@@ -205,6 +205,12 @@ struct AttnShape {
     uint32_t group, rt, tile_shift, window, all, n_heads;
 };
 
+// 64-bit quotient; the 32-bit one, which is much shorter, where it is enough
+__device__ __forceinline__ uint64_t quot(uint64_t a, uint64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 struct SeqPlan {
     int32_t n, len;       // new tokens, length
     int64_t row0;
@@ -252,7 +258,7 @@ __device__ __forceinline__ SeqPlan plan_seq(const AttnShape& a, const KvBatchVie
     unit_tiles(a, p, 0, &f0, &e0);
     // bound of a pair: floor(x / T) + floor(y / T) <= floor((x + y) / T) for the two last positions
     const uint64_t reach = 2ull * static_cast<uint64_t>(max(p.p0, 0)) +
-                           (static_cast<uint64_t>(p.nr + 1) * a.rt) / a.group;
+                           quot(static_cast<uint64_t>(p.nr + 1) * a.rt, a.group);
     const uint32_t two = min(static_cast<uint32_t>((reach >> a.tile_shift) + 2u), 2u * one);
     const uint64_t flat = static_cast<uint64_t>(p.nr) * one;
     const uint64_t pair = static_cast<uint64_t>((p.nr + 1) / 2) * two;
@@ -299,8 +305,8 @@ __device__ __forceinline__ bool next_piece(const AttnShape& a, const KvBatchView
             continue;
         }
         const uint64_t in_seq = w.at - w.seq_at;
-        const uint64_t lane = in_seq / w.plan.weight;
-        const uint32_t head = static_cast<uint32_t>(lane / w.plan.lanes);
+        const uint64_t lane = quot(in_seq, w.plan.weight);
+        const uint32_t head = static_cast<uint32_t>(quot(lane, w.plan.lanes));
         const uint32_t slot = static_cast<uint32_t>(lane - static_cast<uint64_t>(head) * w.plan.lanes);
         uint32_t off = static_cast<uint32_t>(in_seq - lane * w.plan.weight);
         uint64_t start = w.seq_at + lane * w.plan.weight;
@@ -376,7 +382,7 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
             if (pass == 1 || one_chunk) {
                 const uint32_t n = total < gridDim.x ? static_cast<uint32_t>(total) : gridDim.x;
                 if (blockIdx.x < n) {
-                    const uint64_t at = total * blockIdx.x / n;
+                    const uint64_t at = quot(total * blockIdx.x, n);
                     const uint64_t lo = before + prev + incl - mine;
                     if (at >= lo && at < lo + mine) {
                         scratch[NT / 32] = s;
@@ -393,8 +399,8 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
     *total_out = total;
     *ctas = n;
     if (blockIdx.x >= n) return false;
-    w->at = total * blockIdx.x / n;
-    w->stop = total * (blockIdx.x + 1) / n;
+    w->at = quot(total * blockIdx.x, n);
+    w->stop = quot(total * (blockIdx.x + 1), n);
     w->seq = static_cast<uint32_t>(scratch[NT / 32]);
     w->seq_at = scratch[NT / 32 + 1];
     w->loaded = false;
@@ -419,7 +425,7 @@ __device__ __forceinline__ bool seq_pages_ok(const AttnShape& a, const KvBatchVi
 
 // CTA that owns place x when n CTAs share `total` places (n <= total)
 __device__ __forceinline__ uint32_t place_owner(uint64_t x, uint64_t total, uint32_t n) {
-    return static_cast<uint32_t>(((x + 1) * n - 1) / total);
+    return static_cast<uint32_t>(quot((x + 1) * n - 1, total));
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -27,10 +27,11 @@
 // A product of up to 128 columns takes about as long as one of 16 (40 to 66 cycles measured), so hi and lo are
 // side by side in one operand of twice the rows, not two products.
 //
-// Roles, one CTA per SM: warp 0 copies pages, warps 1 and 2 issue the two products, warp 3 stages queries
-// (turned, split) and checks page tables, warps 4-7 keep the output's sums (one head element a thread), warps 8-11
-// and 12-15 are two softmax groups that take every other tile, each with its own running maximum. A tile's
-// softmax is a chain of waits; two at a time, with the scores of the next ready before it ends, hide it.
+// Roles, one CTA per SM: warps 0 and 3 copy the pages of keys and of values, warps 1 and 2 issue the two
+// products, warps 4-7 keep the output's sums (one head element a thread), the next 8 or 12 are two or three
+// softmax groups that take the tiles in turn, each with its own running maximum, and of the last 4 three stage
+// queries (turned, split) and one walks the work and checks page tables. A tile's softmax is a chain of waits; two or three
+// at a time, with the scores of the next ready before one ends, hide it.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -48,24 +49,31 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait (never expected to run out)
 constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
+constexpr uint32_t kPieces = 16; // piece records kept; the walk stays 12 ahead of the output at most
 constexpr int kQSlots = 8;  // pieces whose row records are kept: softmax lags the staging by fewer than 5
 
-// R rows of a row tile, DC 128-element chunks of a head
-template <int R, int DC>
+// R columns for the rows of a row tile, of which the first 8 * NB are used, DC 128-element chunks of a head, G softmax
+// groups
+template <int R, int DC, int NB, int G>
 struct Cfg {
-    static constexpr int kThreads = 512;
+    static constexpr int kThreads = 384 + 128 * G;
+    // Registers of a thread by role: copies and products need few, output sums and softmax many. The shares of the
+    // warpgroups add up to what the block is launched with (96 a thread for 5 warpgroups, 80 for 6).
+    static constexpr int kRegsLaunch = G == 2 ? 96 : 80, kRegsIssue = 48, kRegsHelp = 56;
+    static constexpr int kRegsOut = G == 2 ? 136 : 88, kRegsSoft = G == 2 ? 120 : 96;
+    static_assert(kRegsIssue + kRegsHelp + kRegsOut + G * kRegsSoft <= (3 + G) * kRegsLaunch, "registers");
     static constexpr int V = R / 4;                       // rows of a softmax thread
     static constexpr uint32_t kChunk = kTile * 128u;      // bytes of a tile's chunk of keys or values
     static constexpr uint32_t kBuf = DC * kChunk;
     static constexpr uint32_t kQ = DC * 2u * R * 128u;    // hi rows, lo rows, chunk by chunk
     static constexpr uint32_t kW = 2u * R * kTile;        // hi, lo
-    static constexpr uint32_t kFixed = 2u * kQ + 2u * kW;
-    static constexpr uint32_t kSmall = 2048u + 320u * R;  // bound of the small arrays
+    static constexpr uint32_t kFixed = 2u * kQ + G * kW;
+    static constexpr uint32_t kSmall = 4096u + (132u + 108u * G) * R;  // bound of the small arrays
     static constexpr int kBufs = static_cast<int>((227u * 1024u - 1024u - kSmall - kFixed) / kBuf);
     static constexpr int kNK = kBufs / 2 > 6 ? 6 : kBufs / 2;            // tiles of keys in flight
     static constexpr int kNV = kBufs - kNK > 6 ? 6 : kBufs - kNK;        // and of values
     static constexpr uint32_t kDyn = kFixed + (kNK + kNV) * kBuf + 1024u;
-    static constexpr uint32_t kColsUsed = 4u * R + 4u * DC * R;  // scores and outputs, hi and lo, two of each
+    static constexpr uint32_t kColsUsed = G * 2u * R * (1u + DC);  // scores and outputs, hi and lo, one of each a group
     static constexpr uint32_t kTmem = kColsUsed <= 64 ? 64u : (kColsUsed <= 128 ? 128u : (kColsUsed <= 256 ? 256u : 512u));
     static_assert(kNK >= 2 && kNV >= 2 && kColsUsed <= 512, "does not fit");
 };
@@ -105,6 +113,12 @@ __device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, volatile 
     }
     __syncwarp();
 }
+// this warpgroup's registers a thread from `from` to `to`
+template <int to, int from>
+__device__ __forceinline__ void set_regs() {
+    if constexpr (to > from) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(to));
+    if constexpr (to < from) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(to));
+}
 // one lane of the (converged) warp: with it the compiler keeps the operands of a product uniform, which halves
 // the cost of issuing one (40 cycles against 63 for a lane picked by its number)
 __device__ __forceinline__ bool elect_one() {
@@ -116,7 +130,13 @@ __device__ __forceinline__ bool elect_one() {
         : "=r"(p));
     return p != 0u;
 }
-__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// a bounded barrier of four warps; *times counts the caller's
+__device__ __forceinline__ void warps_meet(uint64_t* b, uint32_t* times, volatile uint32_t* gave_up) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0) bar_arrive(b);
+    bar_wait(b, *times & 1u, gave_up);
+    ++*times;
+}
 
 __device__ __forceinline__ void tma_page(const CUtensorMap* map, void* dst, uint64_t* bar, int32_t x, int32_t z) {
     asm volatile(
@@ -241,6 +261,7 @@ __device__ __forceinline__ void fold_lanes(float* x, uint32_t lane, Op op) {
 }
 template <int N>
 __device__ __forceinline__ uint32_t first_of(uint32_t lane) {
+    if constexpr (N == 2) return lane >> 4;
     if constexpr (N == 4) return (lane >> 3) & 3u;
     if constexpr (N == 8) return lane >> 2;
     return (lane >> 2) * (N / 8);
@@ -248,24 +269,45 @@ __device__ __forceinline__ uint32_t first_of(uint32_t lane) {
 
 // ---------------------------------------------------------------------------------------------
 
-template <int R, int DC>
+// A piece as the roles read it from shared memory: one warp walks this CTA's range and publishes them
+struct PieceRec {
+    uint64_t start;
+    int64_t row0;
+    uint32_t seq, head, row_tile, rows;  // rows = 0: no more pieces
+    int32_t t0, t1, first, end;
+    int32_t p0, len;
+};
+__device__ __forceinline__ PieceRec rec_of(bool any, const Piece& pc) {
+    PieceRec r;
+    r.start = pc.start, r.row0 = pc.plan.row0;
+    r.seq = pc.seq, r.head = pc.head, r.row_tile = pc.row_tile, r.rows = any ? pc.rows : 0u;
+    r.t0 = pc.t0, r.t1 = pc.t1, r.first = pc.first, r.end = pc.end;
+    r.p0 = pc.plan.p0, r.len = pc.plan.len;
+    return r;
+}
+
+template <int R, int DC, int NB, int G>
 struct Shared {
-    static constexpr int kNK = Cfg<R, DC>::kNK, kNV = Cfg<R, DC>::kNV;
+    static constexpr int kNK = Cfg<R, DC, NB, G>::kNK, kNV = Cfg<R, DC, NB, G>::kNV;
     uint64_t kfull[kNK], vfull[kNV], scfull[kNV];
     uint64_t sfull[kRing], ofull[kRing];  // of tile n at n % kRing: its scores, its output are done
-    uint64_t sempty[2], wfull[2], oempty[2], qfull[2], qempty[2], rfull[kQSlots], lfull, lempty, done;
-    unsigned long long scratch[Cfg<R, DC>::kThreads / 32 + 2];
-    uint32_t tmem, gave_up, last_flag, pad;
+    uint64_t sempty[G], wfull[G], oempty[G], qfull[2], qempty[2], rfull[kQSlots], pfull[kPieces], meet[G], lfull, lempty,
+        done;
+    unsigned long long scratch[Cfg<R, DC, NB, G>::kThreads / 32 + 2];
+    PieceRec piece[kPieces], split[2];
+    uint64_t total;
+    uint32_t tmem, gave_up, ctas, pieces_done, split_mask, join_mask;
     float kscale[kNV][8], vscale[kNV][8];   // by page of the tile
     // by column of the weights:
     alignas(16) float frow[kQSlots][R];                 // a row's factor from the product to the score, base 2; positive
     int32_t qpos[kQSlots][R];               // a row's position
-    float wmax[2][2][4][R];                 // [group][its tiles' parity][warp] a tile's maxima
-    alignas(16) float2 ref[8][R];                       // [softmax warp] running maximum, weight factor
-    float rescale[8][R];                    // [softmax warp] factor of the older sums
-    float osc[2][R], mgrp[2][R];            // a tile's factor, and the running maximum that its weights are under
+    float wmax[G][2][4][R];                 // [group][its tiles' parity][warp] a tile's maxima
+    alignas(16) float2 ref[4 * G][R];                       // [softmax warp] running maximum, weight factor
+    float rescale[4 * G][R];                    // [softmax warp] factor of the older sums
+    float osc[G][R], mgrp[G][R];            // a tile's factor, and the running maximum that its weights are under
+    uint64_t row_at[4][R];                  // [output warp] where a row goes
     alignas(16) float fac[4][R], facold[4][R];  // [output warp] a tile's factor, the older sums' factor
-    float lsum[2][4][R], mfin[2][R];        // [group][warp] a piece's sums; [group] maxima
+    float lsum[G][4][R], mfin[G][R];        // [group][warp] a piece's sums; [group] maxima
 };
 
 struct MmaArgs {
@@ -274,12 +316,18 @@ struct MmaArgs {
     uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
 };
 
+// row of a column of the weights, and of the output
+template <uint32_t V>
+__device__ __forceinline__ constexpr uint32_t row_of(uint32_t col) {
+    return ((col % V) >> 1) * 8u + (col / V) * 2u + (col & 1u);
+}
+
 // A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle), 8 elements a lane, DC * 16 lanes a row;
 // this warp takes rows `at`, `at` + `step`, ... in units of the rows that it handles at once, U units at a time.
-template <int R, int DC, int U>
-__device__ __forceinline__ void stage_queries(const MmaArgs& args, const Piece& pc, uint8_t* dst, float* frow, int32_t* qpos,
+template <int R, int DC, int NB, int G, int U>
+__device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRec& pc, uint8_t* dst, float* frow, int32_t* qpos,
                                               uint32_t at, uint32_t step) {
-    constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC>::V;
+    constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC, NB, G>::V;
     const AttnArgs& a = args.a;
     const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
     const uint32_t sub = lane / kRowLanes, d0 = (lane % kRowLanes) * 8u;
@@ -292,10 +340,10 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const Piece& 
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
             if (r < pc.rows && d0 < D) {
-                const uint32_t rr = pc.row_tile * R + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
-                const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                const uint32_t rr = pc.row_tile * a.shape.rt + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
+                const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.row0 + tok) * a.q.token_stride +
                                          (pc.head * a.shape.group + g) * a.q.head_stride;
-                const int32_t pos = pc.plan.p0 + static_cast<int32_t>(tok);
+                const int32_t pos = pc.p0 + static_cast<int32_t>(tok);
                 if (args.q_vec) {
                     load_turned<__nv_bfloat16, 8>(a.rope, p, d0, pos, x[u]);
                 } else {
@@ -343,23 +391,144 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const Piece& 
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
                 // (positive, so that a masked score stays -inf; at 1e-30 scores are zero all the same)
                 frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
-                qpos[col] = pc.plan.p0 + static_cast<int32_t>((pc.row_tile * R + r) / a.shape.group);
+                qpos[col] = pc.p0 + static_cast<int32_t>((pc.row_tile * a.shape.rt + r) / a.shape.group);
             }
         }
     }
     fence_async_smem();
 }
 
-template <int R, int DC>
-__global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
+__device__ __forceinline__ void join_add(const float* p, float f, float4* o) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+    o->x = fmaf(v.x, f, o->x), o->y = fmaf(v.y, f, o->y), o->z = fmaf(v.z, f, o->z), o->w = fmaf(v.w, f, o->w);
+}
+
+// Units that were cut: the last of their CTAs to arrive joins the pieces, in CTA order. The output's four warps and
+// four of the softmax's do it (w: 0 to 7) after all of this CTA's own tiles, so that nothing of it waits for the
+// joining; `tmp` is shared memory that the tiles no longer need.
+template <int DC, typename Sh>
+__device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, float* tmp, uint32_t w) {
+    constexpr uint32_t kTable = 8192;  // factors of (piece, row) kept at a time
+    const uint32_t lane = threadIdx.x & 31u, t = w * 32u + lane, D = a.g.head_dim;
+    __threadfence();
+    asm volatile("bar.sync 14, 256;" ::: "memory");
+    if (w == 0) {
+        uint32_t joins = 0u;
+        if (lane < 2u && (sh.split_mask & (1u << lane))) {
+            const PieceRec& pc = sh.split[lane];
+            const uint32_t c0 = place_owner(pc.start, sh.total, sh.ctas);
+            const uint32_t c1 = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, sh.total, sh.ctas);
+            if (atomicAdd(a.counter + c0, 1u) == c1 - c0) {
+                a.counter[c0] = 0u;
+                joins = 1u << lane;
+            }
+        }
+        joins = __reduce_or_sync(0xFFFFFFFFu, joins);
+        if (lane == 0) sh.join_mask = joins;
+    }
+    asm volatile("bar.sync 14, 256;" ::: "memory");
+    if (sh.join_mask == 0u) return;
+    __threadfence();
+    for (uint32_t mine = 0; mine < 2u; ++mine) {
+        if (!(sh.join_mask & (1u << mine))) continue;
+        const PieceRec& pc = sh.split[mine];
+        const uint32_t c0 = place_owner(pc.start, sh.total, sh.ctas);
+        const uint32_t n = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, sh.total, sh.ctas) - c0 + 1u;
+        const uint32_t rows = pc.rows;
+        const float* first = a.part + (2ull * c0 + 1u) * a.part_stride;       // the piece of c0 is its CTA's last
+        const float* rest = a.part + (2ull * c0) * a.part_stride;             // the others' are their CTA's first
+        const auto piece_of = [&](uint32_t c) { return c == 0 ? first : rest + 2ull * c * a.part_stride; };
+        float* fm = tmp;              // [n][rows] maxima, then factors
+        float* fl = tmp + kTable;     // [n][rows] sums
+        float* norm = fl + kTable;    // [rows]
+        // (n * rows is at most the CTAs times 64: beyond the table, rows are taken in groups)
+        const uint32_t group = min(rows, kTable / n);
+        for (uint32_t g0 = 0; g0 < rows; g0 += group) {
+            const uint32_t gr = min(group, rows - g0);
+            for (uint32_t i = t; i < n * gr; i += 256u) {
+                const uint32_t c = i / gr, r = i - c * gr;
+                const float* p = piece_of(c) + kPartRows * D + g0 + r;
+                fm[i] = __ldcg(p);
+                fl[i] = __ldcg(p + kPartRows);
+            }
+            asm volatile("bar.sync 14, 256;" ::: "memory");
+            if (t < gr) {
+                float m = kNegInf, l = 0.0f;
+                for (uint32_t c = 0; c < n; ++c) m = fmaxf(m, fm[c * gr + t]);
+                for (uint32_t c = 0; c < n; ++c) {
+                    const float mc = fm[c * gr + t], f = mc == m ? 1.0f : ex2(mc - m);
+                    l += fl[c * gr + t] * f;
+                    fm[c * gr + t] = f;
+                }
+                norm[t] = l == 0.0f ? 0.0f : 1.0f / l;
+                if (a.lse) {
+                    const uint32_t rr = pc.row_tile * a.shape.rt + g0 + t, tok = rr / a.shape.group;
+                    a.lse[(pc.row0 + tok) * (a.shape.n_heads * a.shape.group) + pc.head * a.shape.group + rr - tok * a.shape.group] =
+                        (m + log2f(l)) * kLn2;
+                }
+            }
+            asm volatile("bar.sync 14, 256;" ::: "memory");
+            // a warp a row, four elements a lane; up to four rows at a time, so that loads are in flight
+            constexpr uint32_t kRows = 4;
+            for (uint32_t r0 = w; r0 < gr; r0 += 8u * kRows) {
+                float4 o[kRows][DC];
+                uint32_t row[kRows];
+#pragma unroll
+                for (uint32_t u = 0; u < kRows; ++u) {
+                    row[u] = min(r0 + 8u * u, gr - 1u);
+#pragma unroll
+                    for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+                const uint32_t live = (gr - r0 + 7u) / 8u;  // rows of this warp from here on
+                if (live == 1u) {
+#pragma unroll 8
+                    for (uint32_t c = 0; c < n; ++c)
+#pragma unroll
+                        for (int k = 0; k < DC; ++k)
+                            if (k * 128u + lane * 4u < D)
+                                join_add(piece_of(c) + (g0 + row[0]) * D + k * 128u + lane * 4u, fm[c * gr + row[0]], &o[0][k]);
+                } else {
+#pragma unroll 2
+                    for (uint32_t c = 0; c < n; ++c)
+#pragma unroll
+                        for (uint32_t u = 0; u < kRows; ++u)
+#pragma unroll
+                            for (int k = 0; k < DC; ++k)
+                                if (k * 128u + lane * 4u < D)
+                                    join_add(piece_of(c) + (g0 + row[u]) * D + k * 128u + lane * 4u, fm[c * gr + row[u]], &o[u][k]);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kRows; ++u) {
+                    if (u >= live) continue;
+                    const uint32_t rr = pc.row_tile * a.shape.rt + g0 + row[u], tok = rr / a.shape.group;
+                    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.row0 + tok) * a.out.token_stride +
+                                       (pc.head * a.shape.group + rr - tok * a.shape.group) * a.out.head_stride;
+                    const float f = norm[row[u]];
+#pragma unroll
+                    for (int k = 0; k < DC; ++k)
+                        if (k * 128u + lane * 4u < D) {
+                            __nv_bfloat16* d = p + k * 128u + lane * 4u;
+                            d[0] = __float2bfloat16_rn(o[u][k].x * f), d[1] = __float2bfloat16_rn(o[u][k].y * f);
+                            d[2] = __float2bfloat16_rn(o[u][k].z * f), d[3] = __float2bfloat16_rn(o[u][k].w * f);
+                        }
+                }
+            }
+            asm volatile("bar.sync 14, 256;" ::: "memory");
+        }
+    }
+}
+
+template <int R, int DC, int NB, int G>
+__global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     attend_mma_kernel(const __grid_constant__ MmaArgs args, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
-    using C = Cfg<R, DC>;
-    constexpr int NK = C::kNK, NV = C::kNV, V = C::V;
+    using C = Cfg<R, DC, NB, G>;
+    constexpr int NK = C::kNK, NV = C::kNV;
+    constexpr uint32_t V = C::V, kStagers = C::kThreads / 32 - 2;
     constexpr uint32_t kFull = 0xFFFFFFFFu;
     extern __shared__ uint8_t raw[];
-    __shared__ Shared<R, DC> sh;
-    static_assert(sizeof(Shared<R, DC>) <= C::kSmall, "small arrays");
+    __shared__ Shared<R, DC, NB, G> sh;
+    static_assert(sizeof(Shared<R, DC, NB, G>) <= C::kSmall, "small arrays");
     const AttnArgs& a = args.a;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t shift = a.g.page_shift, D = a.g.head_dim;
@@ -374,18 +543,19 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
         for (int i = 0; i < NK; ++i) bar_init(&sh.kfull[i], 1);
         for (int i = 0; i < NV; ++i) bar_init(&sh.vfull[i], 1), bar_init(&sh.scfull[i], 32);
         for (int i = 0; i < kRing; ++i) bar_init(&sh.sfull[i], 1), bar_init(&sh.ofull[i], 1);
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < G; ++i) {
             bar_init(&sh.sempty[i], 4);
             bar_init(&sh.wfull[i], 4);
             bar_init(&sh.oempty[i], 4);
-            bar_init(&sh.qfull[i], 1);
-            bar_init(&sh.qempty[i], 1);
         }
-        for (int i = 0; i < kQSlots; ++i) bar_init(&sh.rfull[i], 1);
-        bar_init(&sh.lfull, 8);
+        for (int i = 0; i < 2; ++i) bar_init(&sh.qfull[i], 3), bar_init(&sh.qempty[i], 1);
+        for (int i = 0; i < kQSlots; ++i) bar_init(&sh.rfull[i], 3);
+        for (uint32_t i = 0; i < kPieces; ++i) bar_init(&sh.pfull[i], 1);
+        for (int i = 0; i < G; ++i) bar_init(&sh.meet[i], 4);
+        bar_init(&sh.lfull, 4 * G);
         bar_init(&sh.lempty, 4);
         bar_init(&sh.done, 2);
-        sh.gave_up = 0u;
+        sh.gave_up = sh.pieces_done = sh.split_mask = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -399,42 +569,68 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
         asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
     PieceWalk walk;
-    uint64_t total;
-    uint32_t ctas;
-    tc_before();
-    const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &walk, &total, &ctas);
-    tc_after();  // (walk_init's barriers have ordered the allocation and the barriers' set-up)
+    {
+        uint64_t total;
+        uint32_t ctas;
+        tc_before();
+        const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &walk, &total, &ctas);
+        if (warp == C::kThreads / 32 - 1) {
+            Piece pc;
+            const bool any = busy && next_piece(a.shape, a.b, shift, walk, &pc);
+            if (lane == 0) {
+                sh.piece[0] = rec_of(any, pc);
+                sh.total = total;
+                sh.ctas = ctas;
+                bar_arrive(&sh.pfull[0]);
+            }
+        }
+        __syncthreads();
+        tc_after();
+    }
     const uint32_t tmem = sh.tmem;
 
-    if (busy) {
-        Piece pc;
-        if (warp != 0) {
-            // the first piece's queries: by every warp but the copying one, which starts at once
-            PieceWalk w = walk;
-            if (next_piece(a.shape, a.b, shift, w, &pc))
-                stage_queries<R, DC, (R * DC / 2 + 14) / 15>(args, pc, qbuf, sh.frow[0], sh.qpos[0], warp - 1u, 15u);
-            asm volatile("bar.sync 4, 480;" ::: "memory");
+    if (sh.piece[0].rows != 0u) {
+        if (warp != 0 && warp != 3) {
+            // the first piece's queries: by every warp but the copying ones, which start at once
+            stage_queries<R, DC, NB, G, (8 * NB * DC / 2 + kStagers - 1) / kStagers>(args, sh.piece[0], qbuf, sh.frow[0],
+                                                                                   sh.qpos[0], warp - (warp > 3 ? 2u : 1u), kStagers);
+            asm volatile("bar.sync 15, %0;" ::"n"(C::kThreads - 64) : "memory");
         }
-        if (warp == 0) {
-            // ---- pages: lanes 0-7 copy a tile's pages of keys, 8-15 of values, the others their scales ----
-            const uint32_t ppt = args.pages_per_tile, per_window = 32u / ppt;
+        // the next piece, or false after the last one
+        const auto piece = [&](uint32_t np) -> const PieceRec* {
+            bar_wait(&sh.pfull[np % kPieces], (np / kPieces) & 1u, gave_up);
+            if (__any_sync(kFull, *gave_up != 0u) || sh.piece[np % kPieces].rows == 0u) return nullptr;
+            return &sh.piece[np % kPieces];
+        };
+        if (warp < 4) {
+        set_regs<C::kRegsIssue, C::kRegsLaunch>();
+        if (warp == 0 || warp == 3) {
+            // ---- pages: warp 0 copies the keys', warp 3 the values' and both's scales; a lane a page ----
+            const bool is_v = warp == 3;
+            const uint32_t ppt = args.pages_per_tile, n_buf = is_v ? NV : NK;
             const uint32_t none = a.g.n_pages * a.g.n_heads;  // a coordinate past the end: zeros
-            const uint32_t slot = lane & 7u;
-            uint32_t n = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+            const uint32_t slot = lane & 7u, window_mask = 32u / ppt - 1u;
+            const CUtensorMap* map = is_v ? &v_map : &k_map;
+            uint8_t* buf = is_v ? vbuf : kbuf;
+            uint64_t* full = is_v ? sh.vfull : sh.kfull;
+            uint64_t* done = is_v ? sh.ofull : sh.sfull;  // of tile n - n_buf: its buffer is free
+            uint32_t n = 0, st = 0;
+            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                const PieceRec& pc = *rec;
                 const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
-                const uint32_t n_pg = (static_cast<uint32_t>(pc.plan.len) + a.g.page_size - 1u) >> shift;
+                const uint32_t n_pg = (static_cast<uint32_t>(pc.len) + a.g.page_size - 1u) >> shift, head = pc.head;
                 uint32_t lo_pg = 0;  // pages wholly before the window of the unit's first row are not read
                 if (a.shape.window) {
-                    const int32_t lo = pc.plan.p0 + static_cast<int32_t>(pc.row_tile * R / a.shape.group) -
+                    const int32_t lo = pc.p0 + static_cast<int32_t>(pc.row_tile * a.shape.rt / a.shape.group) -
                                        static_cast<int32_t>(a.shape.window) + 1;
                     lo_pg = lo > 0 ? static_cast<uint32_t>(lo) >> shift : 0u;
                 }
                 // 32 page ids at a time, the next 32 asked for before they are needed
+                const uint32_t tiles = static_cast<uint32_t>(pc.t1 - pc.t0);
                 uint32_t idx = static_cast<uint32_t>(pc.t0) * ppt + lane;
                 int32_t ids = -1, ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
-                for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t in = static_cast<uint32_t>(t - pc.t0) % per_window;
+                for (uint32_t i = 0; i < tiles; ++i, ++n) {
+                    const uint32_t in = i & window_mask;
                     if (in == 0) {
                         ids = ids_next;
                         idx += 32u;
@@ -442,47 +638,32 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     }
                     const int32_t id = __shfl_sync(kFull, ids, in * ppt + (slot & (ppt - 1u)));
                     const bool good = static_cast<uint32_t>(id) < a.g.n_pages;
-                    const uint32_t z = good ? static_cast<uint32_t>(id) * a.g.n_heads + pc.head : none;
-                    const uint32_t ks = n % NK, vs = n % NV;
-                    if (n >= NK) bar_wait(&sh.sfull[(n - NK) % kRing], ((n - NK) / kRing) & 1u, gave_up);
-                    if (*gave_up) break;
-                    if (lane == 0) bar_expect(&sh.kfull[ks], C::kBuf);
+                    const uint32_t z = good ? static_cast<uint32_t>(id) * a.g.n_heads + head : none;
+                    if (n >= n_buf) bar_wait(&done[(n - n_buf) % kRing], ((n - n_buf) / kRing) & 1u, gave_up);
+                    if (__any_sync(kFull, *gave_up != 0u)) break;
+                    if (lane == 0) bar_expect(&full[st], C::kBuf);
                     __syncwarp();
                     if (lane < ppt) {
 #pragma unroll
                         for (int c = 0; c < DC; ++c)
-                            tma_page(&k_map, kbuf + ks * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &sh.kfull[ks],
-                                     c * 128, z);
+                            tma_page(map, buf + st * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &full[st], c * 128, z);
                     }
-                    if (n >= NV) bar_wait(&sh.ofull[(n - NV) % kRing], ((n - NV) / kRing) & 1u, gave_up);
-                    if (*gave_up) {
-                        ++n;  // the keys' copy is in flight
-                        break;
+                    if (is_v) {
+                        if (lane >= 16u) {
+                            const float* src = (lane >= 24u ? a.g.v_scales : a.g.k_scales) + (good ? z : 0u);
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                                             s32(lane >= 24u ? &sh.vscale[st][slot] : &sh.kscale[st][slot])),
+                                         "l"(src), "r"(good ? 4u : 0u)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.scfull[st])) : "memory");
                     }
-                    if (lane == 0) bar_expect(&sh.vfull[vs], C::kBuf);
-                    __syncwarp();
-                    if (lane >= 8u && lane < 8u + ppt) {
-#pragma unroll
-                        for (int c = 0; c < DC; ++c)
-                            tma_page(&v_map, vbuf + vs * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &sh.vfull[vs],
-                                     c * 128, z);
-                    } else if (lane >= 16u) {
-                        const bool is_v = lane >= 24u;
-                        const float* src = (is_v ? a.g.v_scales : a.g.k_scales) + (good ? z : 0u);
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                         s32(is_v ? &sh.vscale[vs][slot] : &sh.kscale[vs][slot])),
-                                     "l"(src), "r"(good ? 4u : 0u)
-                                     : "memory");
-                    }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.scfull[vs])) : "memory");
+                    if (++st == n_buf) st = 0;
                 }
-                if (*gave_up) break;
             }
             if (*gave_up) {  // the copies in flight land before the shared memory is given back
-                for (uint32_t i = n > NK ? n - NK : 0u; i < n; ++i)
-                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.kfull[i % NK], (i / NK) & 1u); ++w) {}
-                for (uint32_t i = n > NV ? n - NV : 0u; i < n; ++i)
-                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&sh.vfull[i % NV], (i / NV) & 1u); ++w) {}
+                for (uint32_t i = n > n_buf ? n - n_buf : 0u; i < n; ++i)
+                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&full[i % n_buf], (i / n_buf) & 1u); ++w) {}
                 asm volatile("cp.async.wait_all;" ::: "memory");
             }
         } else if (warp == 1) {
@@ -490,14 +671,15 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
             const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
             const uint32_t ksteps = (D + 31u) / 32u;
             const uint64_t k_desc = desc_sw128(s32(kbuf)), q_desc = desc_sw128(s32(qbuf));
-            uint32_t n = 0, np = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+            uint32_t n = 0;
+            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                const PieceRec& pc = *rec;
                 const uint32_t qb = np & 1u;
                 bar_wait(&sh.qfull[qb], (np >> 1) & 1u, gave_up);
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t ks = n % NK, b = n & 1u;
+                    const uint32_t ks = n % NK, b = n % G;
                     bar_wait(&sh.kfull[ks], (n / NK) & 1u, gave_up);
-                    if (n >= 2) bar_wait(&sh.sempty[b], ((n >> 1) - 1u) & 1u, gave_up);
+                    if (n >= G) bar_wait(&sh.sempty[b], (n / G - 1u) & 1u, gave_up);
                     tc_after();
                     if (__any_sync(kFull, *gave_up != 0u)) continue;
                     const uint64_t kd = k_desc + ks * (C::kBuf >> 4), qd = q_desc + qb * (C::kQ >> 4);
@@ -515,19 +697,19 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     }
                     __syncwarp();
                 }
-                ++np;
             }
-        } else if (warp == 2) {
+        } else {
             // ---- outputs: hi and lo columns of the weights are one operand of 2 R columns ----
             const uint32_t idesc = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
             const uint64_t v_desc = desc_sw128(s32(vbuf)), w_desc = desc_plain(s32(wbuf), 128u, 16u * kTile);
             uint32_t n = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                const PieceRec& pc = *rec;
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t vs = n % NV, b = n & 1u;
+                    const uint32_t vs = n % NV, b = n % G;
                     bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
                     // (the softmax has waited for the output buffer to be free)
-                    bar_wait(&sh.wfull[b], (n >> 1) & 1u, gave_up);
+                    bar_wait(&sh.wfull[b], (n / G) & 1u, gave_up);
                     tc_after();
                     if (__any_sync(kFull, *gave_up != 0u)) continue;
                     const uint64_t vd = v_desc + vs * (C::kBuf >> 4), wd = w_desc + b * (C::kW >> 4);
@@ -536,7 +718,7 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                         for (int c = 0; c < DC; ++c)
 #pragma unroll
                             for (int k = 0; k < kTile / 32; ++k)
-                                mma_f8(tmem + 4u * R + (b * DC + c) * 2u * R, vd + ((c * C::kChunk + k * 4096u) >> 4),
+                                mma_f8(tmem + G * 2u * R + (b * DC + c) * 2u * R, vd + ((c * C::kChunk + k * 4096u) >> 4),
                                        wd + ((k * 512u) >> 4), idesc, k > 0);
                     }
                     __syncwarp();
@@ -544,29 +726,18 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     __syncwarp();
                 }
             }
-        } else if (warp == 3) {
-            // ---- queries of the pieces after the first ----
-            uint32_t np = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
-                const uint32_t qb = np & 1u, rs = np % kQSlots;
-                if (np >= 2) bar_wait(&sh.qempty[qb], ((np >> 1) - 1u) & 1u, gave_up);
-                if (np > 0) stage_queries<R, DC, 4>(args, pc, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], 0u, 1u);
-                __syncwarp();
-                if (lane == 0) {
-                    bar_arrive(&sh.qfull[qb]);
-                    bar_arrive(&sh.rfull[rs]);
-                }
-                ++np;
-            }
+        }
         } else if (warp < 8) {
+            set_regs<C::kRegsOut, C::kRegsLaunch>();
             // ---- output sums: thread d of a chunk holds element d of every row ----
             const uint32_t quad = warp & 3u, d0 = quad * 32u + lane;
-            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + 4u * R;
+            const uint32_t t_lane = tmem + ((quad * 32u) << 16) + G * 2u * R;
             constexpr int kPer = R > 32 ? 2 : 1;  // columns of a lane where columns are dealt to lanes
             float* fac = sh.fac[quad];
             float* facold = sh.facold[quad];
             uint32_t n = 0, np = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+            for (; const PieceRec* rec = piece(np); ++np) {
+                const PieceRec& pc = *rec;
                 F2 acc[DC][R / 2];
 #pragma unroll
                 for (int c = 0; c < DC; ++c)
@@ -576,14 +747,14 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) M[i] = kNegInf;
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t b = n & 1u;
+                    const uint32_t b = n % G;
                     // the weights' barrier orders the factors that the softmax wrote
-                    bar_wait(&sh.wfull[b], (n >> 1) & 1u, gave_up);
+                    bar_wait(&sh.wfull[b], (n / G) & 1u, gave_up);
                     bool changed = false;
 #pragma unroll
                     for (int i = 0; i < kPer; ++i) {
                         const uint32_t col = lane + 32u * i;
-                        if (col < R) {
+                        if (col < R && row_of<V>(col) < 8u * NB) {
                             const float mg = sh.mgrp[b][col], m1 = fmaxf(M[i], mg);
                             fac[col] = sh.osc[b][col] * (mg == m1 ? 1.0f : ex2(mg - m1));
                             const float al = M[i] == m1 ? 1.0f : ex2(M[i] - m1);
@@ -606,6 +777,7 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     tc_after();
 #pragma unroll
                     for (int r = 0; r < R; r += 8) {
+                        if (row_of<V>(r) >= 8u * NB) continue;  // (the lowest row of the eight)
                         float o[DC][8], o_lo[DC][8];
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
@@ -631,10 +803,10 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const uint32_t col = lane + 32u * i;
-                    if (col < R) {
+                    if (col < R && row_of<V>(col) < 8u * NB) {
                         float l = 0.0f;
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
+                        for (int g = 0; g < G; ++g) {
                             const float mg = sh.mfin[g][col];
                             l += (sh.lsum[g][0][col] + sh.lsum[g][1][col] + sh.lsum[g][2][col] + sh.lsum[g][3][col]) *
                                  (mg == M[i] ? 1.0f : ex2(mg - M[i]));
@@ -646,106 +818,97 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lempty);
                 const bool whole = pc.t0 == pc.first && pc.t1 == pc.end;
-                const uint32_t r_base = pc.row_tile * R, group = a.shape.group;
-                const uint32_t q_heads = a.shape.n_heads * group;
-                float* part = a.part + (2ull * blockIdx.x + (pc.t0 == pc.first ? 1u : 0u)) * a.part_stride;
+                const uint32_t mine = (pc.t0 == pc.first ? 1u : 0u);
+                if (whole) {
+                    // where each row goes: worked out by the lanes, a column each
+                    __syncwarp();
 #pragma unroll
-                for (int col = 0; col < R; ++col) {
-                    const uint32_t r = ((col % V) >> 1) * 8 + (col / V) * 2 + (col & 1);
-                    if (r >= pc.rows) continue;
-                    const float l = facold[col];
-                    float y[DC];
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) {
-                        const float2 p = un2(acc[c][col / 2]);
-                        y[c] = (col & 1) ? p.y : p.x;
-                    }
-                    if (whole) {
-                        const uint32_t tok = (r_base + r) / group, g = (r_base + r) - tok * group;
-                        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
-                                           (pc.head * group + g) * a.out.head_stride;
-                        const float inv = 1.0f / l;
-#pragma unroll
-                        for (int c = 0; c < DC; ++c)
-                            if (c * 128u + d0 < D) p[c * 128u + d0] = __float2bfloat16_rn(l == 0.0f ? 0.0f : y[c] * inv);
-                        if (a.lse && d0 == 0u)
-                            a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (fac[col] + log2f(l)) * kLn2;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < DC; ++c)
-                            if (c * 128u + d0 < D) part[r * D + c * 128u + d0] = y[c];
-                        if (d0 == 0u) {
-                            part[kPartRows * D + r] = fac[col];
-                            part[kPartRows * (D + 1u) + r] = l;
+                    for (int i = 0; i < kPer; ++i) {
+                        const uint32_t col = lane + 32u * i, r = row_of<V>(col);
+                        if (col < R && r < pc.rows) {
+                            const uint32_t tok = (pc.row_tile * a.shape.rt + r) / a.shape.group;
+                            const uint32_t hq = pc.head * a.shape.group + (pc.row_tile * a.shape.rt + r) - tok * a.shape.group;
+                            sh.row_at[quad][col] = (pc.row0 + tok) * a.out.token_stride + hq * a.out.head_stride;
+                            if (a.lse && quad == 0)
+                                a.lse[(pc.row0 + tok) * (a.shape.n_heads * a.shape.group) + hq] =
+                                    (fac[col] + log2f(facold[col])) * kLn2;
+                            facold[col] = facold[col] == 0.0f ? 0.0f : 1.0f / facold[col];  // (a row without positions: 0)
                         }
+                    }
+                    __syncwarp();
+                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.data);
+#pragma unroll
+                    for (int col = 0; col < R; ++col) {
+                        if (row_of<V>(col) >= pc.rows) continue;
+                        const float inv = facold[col];
+                        __nv_bfloat16* p = out + sh.row_at[quad][col];
+#pragma unroll
+                        for (int c = 0; c < DC; ++c) {
+                            const float2 y = un2(acc[c][col / 2]);
+                            if (c * 128u + d0 < D) p[c * 128u + d0] = __float2bfloat16_rn(((col & 1) ? y.y : y.x) * inv);
+                        }
+                    }
+                } else {
+                    float* part = a.part + (2ull * blockIdx.x + mine) * a.part_stride;
+#pragma unroll
+                    for (int col = 0; col < R; ++col) {
+                        const uint32_t r = row_of<V>(col);
+                        if (r >= pc.rows) continue;
+#pragma unroll
+                        for (int c = 0; c < DC; ++c) {
+                            const float2 y = un2(acc[c][col / 2]);
+                            if (c * 128u + d0 < D) part[r * D + c * 128u + d0] = (col & 1) ? y.y : y.x;
+                        }
+                    }
+                    if (quad == 0) {
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) {
+                            const uint32_t col = lane + 32u * i, r = row_of<V>(col);
+                            if (col < R && r < pc.rows) {
+                                part[kPartRows * D + r] = fac[col];
+                                part[kPartRows * (D + 1u) + r] = facold[col];
+                            }
+                        }
+                    }
+                    // at most two pieces of a CTA are parts of a unit: its first and its last
+                    if (warp == 4 && lane == 0) {
+                        sh.split[mine] = pc;
+                        sh.split_mask |= 1u << mine;
                     }
                 }
                 __syncwarp();
-                ++np;
-                if (whole) continue;
-                // pieces of one unit meet: the last CTA to arrive joins them in CTA order
-                const uint32_t c0 = place_owner(pc.start, total, ctas);
-                const uint32_t c1 = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, total, ctas);
-                __threadfence();
-                group_sync(1);
-                if (warp == 4 && lane == 0) {
-                    sh.last_flag = atomicAdd(a.counter + c0, 1u) == c1 - c0 ? 1u : 0u;
-                    if (sh.last_flag) a.counter[c0] = 0u;
-                }
-                group_sync(1);
-                if (!sh.last_flag) continue;
-                __threadfence();
-                for (uint32_t r = 0; r < pc.rows; ++r) {
-                    float m = kNegInf, l = 0.0f, o[DC];
-#pragma unroll
-                    for (int c = 0; c < DC; ++c) o[c] = 0.0f;
-                    for (uint32_t c = c0; c <= c1; ++c)
-                        m = fmaxf(m, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r));
-                    for (uint32_t c = c0; c <= c1; ++c) {
-                        const float* p = a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride;
-                        const float mc = __ldcg(p + kPartRows * D + r);
-                        const float f = mc == m ? 1.0f : exp2f(mc - m);
-                        l += __ldcg(p + kPartRows * (D + 1u) + r) * f;
-#pragma unroll
-                        for (int k = 0; k < DC; ++k)
-                            if (k * 128u + d0 < D) o[k] += __ldcg(p + r * D + k * 128u + d0) * f;
-                    }
-                    const uint32_t tok = (r_base + r) / group, g = (r_base + r) - tok * group;
-                    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
-                                       (pc.head * group + g) * a.out.head_stride;
-#pragma unroll
-                    for (int k = 0; k < DC; ++k)
-                        if (k * 128u + d0 < D) p[k * 128u + d0] = __float2bfloat16_rn(l == 0.0f ? 0.0f : o[k] / l);
-                    if (a.lse && d0 == 0u)
-                        a.lse[(pc.plan.row0 + tok) * q_heads + pc.head * group + g] = (m + log2f(l)) * kLn2;
-                }
+                if (warp == 4 && lane == 0) *const_cast<volatile uint32_t*>(&sh.pieces_done) = np + 1u;
             }
-        } else {
-            // ---- softmax: group g takes the tiles n with n % 2 == g ----
+            join_pieces<DC>(a, sh, reinterpret_cast<float*>(dyn), warp - 4u);
+        } else if (warp < 8 + 4 * G) {
+            set_regs<C::kRegsSoft, C::kRegsLaunch>();
+            // ---- softmax: group g takes the tiles n with n % G == g ----
             const uint32_t quad = warp & 3u, grp = (warp - 8u) >> 2, q = lane & 3u, tr = lane >> 2;
             const uint32_t t_lane = tmem + ((quad * 32u) << 16) + grp * 2u * R;
             const uint32_t pg0 = (quad * 32u) >> shift, pg1 = (quad * 32u + 16u) >> shift;
-            constexpr int kOwn = V > 8 ? V / 8 : 1;  // columns that a lane ends with where they are dealt out
-            const uint32_t own = q * V + first_of<V>(lane);
+            constexpr int kFold = NB > 4 ? 16 : (NB > 2 ? 8 : 2 * NB);  // a thread's columns, to a power of two
+            constexpr int kOwn = kFold > 8 ? kFold / 8 : 1;             // those that a lane ends with where they are dealt out
+            const uint32_t own = q * V + first_of<kFold>(lane);
             float2* my_ref = sh.ref[warp - 8u];
             float* my_rescale = sh.rescale[warp - 8u];
             uint8_t* w0 = wbuf + grp * C::kW + (quad * 4u) * 128u + tr * 16u + ((q * V) >> 4) * (16u * kTile) + ((q * V) & 15u);
             const auto max_op = [](float x, float y) { return fmaxf(x, y); };
             const auto add_op = [](float x, float y) { return x + y; };
-            uint32_t n = 0, np = 0;
-            while (next_piece(a.shape, a.b, shift, walk, &pc)) {
+            uint32_t n = 0, np = 0, meets = 0;
+            for (; const PieceRec* rec = piece(np); ++np) {
+                const PieceRec& pc = *rec;
                 const uint32_t rs = np % kQSlots;
                 bar_wait(&sh.rfull[rs], (np / kQSlots) & 1u, gave_up);
                 const float* frow = sh.frow[rs] + q * V;
                 const int32_t* qpos = sh.qpos[rs] + q * V;
                 // tiles in [safe_from, reach) are inside every row's positions
-                const int32_t p_first = pc.plan.p0 + static_cast<int32_t>(pc.row_tile * R / a.shape.group);
-                const int32_t p_last = pc.plan.p0 + static_cast<int32_t>((pc.row_tile * R + pc.rows - 1u) / a.shape.group);
-                const int32_t reach = a.shape.all ? pc.plan.len : min(pc.plan.len, p_first + 1);
+                const int32_t p_first = pc.p0 + static_cast<int32_t>(pc.row_tile * a.shape.rt / a.shape.group);
+                const int32_t p_last = pc.p0 + static_cast<int32_t>((pc.row_tile * a.shape.rt + pc.rows - 1u) / a.shape.group);
+                const int32_t reach = a.shape.all ? pc.len : min(pc.len, p_first + 1);
                 const int32_t safe_from = a.shape.window ? p_last - static_cast<int32_t>(a.shape.window) + 1 : 0;
                 float l[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) l[i] = 0.0f;
+                for (uint32_t i = 0; i < V; ++i) l[i] = 0.0f;
                 float M[kOwn], f_own[kOwn];
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
@@ -753,8 +916,8 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     f_own[i] = sh.frow[rs][own + i];
                 }
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    if ((n & 1u) != grp) continue;
-                    const uint32_t vs = n % NV, use = n >> 1;
+                    if (n % G != grp) continue;
+                    const uint32_t vs = n % NV, use = n / G;
                     float(*wmax)[R] = sh.wmax[grp][use & 1u];  // (its last readers met since)
                     bar_wait(&sh.scfull[vs], (n / NV) & 1u, gave_up);
                     const float fk0 = sh.kscale[vs][pg0], fk1 = sh.kscale[vs][pg1];
@@ -774,7 +937,12 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     tc_after();
                     float x[V / 2][2][4];  // [8-column block][column][token]
 #pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {
+                    for (int j = 0; j < static_cast<int>(V / 2); ++j) {
+                        if (j >= NB) {  // columns without rows
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[j][0][i] = x[j][1][i] = kNegInf;
+                            continue;
+                        }
                         float f[8], g[8];
                         tmem_ld_frag(t_lane + 8 * j, f);
                         tmem_ld_frag(t_lane + (16u << 16) + 8 * j, f + 4);
@@ -794,26 +962,26 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     if (edge) {
                         const int32_t w = static_cast<int32_t>(a.shape.window);
 #pragma unroll
-                        for (int c = 0; c < V; ++c) {
+                        for (int c = 0; c < static_cast<int>(V); ++c) {
                             const int32_t qp = qpos[c];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int32_t pos = t * kTile + static_cast<int32_t>(quad * 32u + i * 8u + tr);
-                                bool ok = pos < pc.plan.len && (a.shape.all || pos <= qp);
+                                bool ok = pos < pc.len && (a.shape.all || pos <= qp);
                                 if (w) ok = ok && pos > qp - w;
                                 if (!ok) x[c >> 1][c & 1][i] = kNegInf;
                             }
                         }
                     }
                     // the tile's maximum of every row: within the thread, over its warp, over the group
-                    float mx[V];
+                    float mx[kFold];
 #pragma unroll
-                    for (int c = 0; c < V; ++c)
+                    for (int c = 0; c < kFold; ++c)
                         mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]), fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]));
-                    fold_lanes<V>(mx, lane, max_op);
+                    fold_lanes<kFold>(mx, lane, max_op);
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
-                    group_sync(2 + grp);
+                    warps_meet(&sh.meet[grp], &meets, gave_up);
                     float mt[kOwn];
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i)
@@ -824,14 +992,14 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     for (int i = 0; i < kOwn; ++i) mw[i] = mt[i];
                     if (wide) {
 #pragma unroll
-                        for (int c = 0; c < V; ++c)
+                        for (int c = 0; c < kFold; ++c)
                             mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]) * frow[c] + static_cast<float>(ev0),
                                           fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]) * frow[c] + static_cast<float>(ev1));
-                        fold_lanes<V>(mx, lane, max_op);
-                        group_sync(2 + grp);  // the first maxima have been read
+                        fold_lanes<kFold>(mx, lane, max_op);
+                        warps_meet(&sh.meet[grp], &meets, gave_up);  // the first maxima have been read
 #pragma unroll
                         for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
-                        group_sync(2 + grp);
+                        warps_meet(&sh.meet[grp], &meets, gave_up);
 #pragma unroll
                         for (int i = 0; i < kOwn; ++i)
                             mw[i] = fmaxf(fmaxf(wmax[0][own + i], wmax[1][own + i]),
@@ -857,49 +1025,63 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                         for (int i = 0; i < kOwn; ++i) my_rescale[own + i] = alpha[i];
                         __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < V; ++c) l[c] *= my_rescale[q * V + c];
+                        for (int c = 0; c < static_cast<int>(V); ++c) l[c] *= my_rescale[q * V + c];
                     }
                     __syncwarp();
-                    if (use >= 1) bar_wait(&sh.ofull[(n - 2u) % kRing], ((n - 2u) / kRing) & 1u, gave_up);  // the weights' buffer is free
-                    const float vr0 = exp2_int(ev0), vr1 = exp2_int(ev1);
-                    uint32_t hi[4][(V + 3) / 4], lo[4][(V + 3) / 4];
+                    if (use >= 1) bar_wait(&sh.ofull[(n - G) % kRing], ((n - G) / kRing) & 1u, gave_up);  // the weights' buffer is free
+                    // two tokens at a time (they share a page), so that their bytes take few registers
 #pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {
-                        const float4 rf = *reinterpret_cast<const float4*>(my_ref + q * V + 2 * j);
-                        const float2 fr = *reinterpret_cast<const float2*>(frow + 2 * j);
-                        const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z);
-                        const F2 wf0 = mul2(f2(rf.y, rf.w), f2(vr0, vr0)), wf1 = mul2(f2(rf.y, rf.w), f2(vr1, vr1));
-                        F2 sum = f2(l[2 * j], l[2 * j + 1]);
+                    for (int half = 0; half < 2; ++half) {
+                        const float vr = exp2_int(half == 0 ? ev0 : ev1);
+                        uint32_t hi[2][(V + 3) / 4], lo[2][(V + 3) / 4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 y = un2(fma2(f2(x[j][0][i], x[j][1][i]), scale2, minus));
-                            const F2 p = f2(ex2(y.x), ex2(y.y));
-                            sum = add2(sum, p);
-                            uint32_t h, g;
-                            split2(mul2(p, i < 2 ? wf0 : wf1), &h, &g);
-                            if (j & 1) {
-                                hi[i][j / 2] = __byte_perm(hi[i][j / 2], h, 0x6420);
-                                lo[i][j / 2] |= g << 16;
-                            } else {
-                                hi[i][j / 2] = h;
-                                lo[i][j / 2] = g;
+                        for (int j = 0; j < static_cast<int>(V / 2); ++j) {
+                            if (j >= NB) {
+                                if (j & 1) continue;
+                                hi[0][j / 2] = hi[1][j / 2] = lo[0][j / 2] = lo[1][j / 2] = 0u;
+                                continue;
                             }
-                        }
-                        const float2 s2 = un2(sum);
-                        l[2 * j] = s2.x, l[2 * j + 1] = s2.y;
-                    }
+                            const float4 rf = *reinterpret_cast<const float4*>(my_ref + q * V + 2 * j);
+                            const float2 fr = *reinterpret_cast<const float2*>(frow + 2 * j);
+                            const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z), wf = mul2(f2(rf.y, rf.w), f2(vr, vr));
+                            F2 sum = f2(l[2 * j], l[2 * j + 1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint8_t* wp = w0 + i * 128;
-                        if constexpr (V == 4) {
-                            *reinterpret_cast<uint32_t*>(wp) = hi[i][0];
-                            *reinterpret_cast<uint32_t*>(wp + R * kTile) = lo[i][0];
-                        } else if constexpr (V == 8) {
-                            *reinterpret_cast<uint2*>(wp) = make_uint2(hi[i][0], hi[i][1]);
-                            *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(lo[i][0], lo[i][1]);
-                        } else {
-                            *reinterpret_cast<uint4*>(wp) = make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
-                            *reinterpret_cast<uint4*>(wp + R * kTile) = make_uint4(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                            for (int i = 0; i < 2; ++i) {
+                                const float2 y = un2(fma2(f2(x[j][0][2 * half + i], x[j][1][2 * half + i]), scale2, minus));
+                                const F2 p = f2(ex2(y.x), ex2(y.y));
+                                sum = add2(sum, p);
+                                uint32_t h, g;
+                                split2(mul2(p, wf), &h, &g);
+                                if (j & 1) {
+                                    hi[i][j / 2] = __byte_perm(hi[i][j / 2], h, 0x6420);
+                                    lo[i][j / 2] = __byte_perm(lo[i][j / 2], g, 0x5410);
+                                } else {
+                                    hi[i][j / 2] = h;
+                                    lo[i][j / 2] = g;
+                                }
+                            }
+                            const float2 s2 = un2(sum);
+                            l[2 * j] = s2.x, l[2 * j + 1] = s2.y;
+                        }
+                        // an odd block without a partner: its bytes still lie apart
+#pragma unroll
+                        for (int j = 0; j < static_cast<int>(V / 2); j += 2)
+                            if (j + 1 >= NB)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) hi[i][j / 2] = __byte_perm(hi[i][j / 2], 0u, 0x6420);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint8_t* wp = w0 + (2 * half + i) * 128;
+                            if constexpr (V == 4) {
+                                *reinterpret_cast<uint32_t*>(wp) = hi[i][0];
+                                *reinterpret_cast<uint32_t*>(wp + R * kTile) = lo[i][0];
+                            } else if constexpr (V == 8) {
+                                *reinterpret_cast<uint2*>(wp) = make_uint2(hi[i][0], hi[i][1]);
+                                *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(lo[i][0], lo[i][1]);
+                            } else {
+                                *reinterpret_cast<uint4*>(wp) = make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
+                                *reinterpret_cast<uint4*>(wp + R * kTile) = make_uint4(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                            }
                         }
                     }
                     if (quad == 0) {
@@ -910,11 +1092,11 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                             sh.mgrp[grp][own + i] = M[i];
                         }
                     }
-                    if ((t + 1) * kTile > pc.plan.len) {
+                    if ((t + 1) * kTile > pc.len) {
                         // what lies behind the sequence's end may hold NaN bytes, and 0 * NaN is NaN
                         bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
                         const uint32_t tok = quad * 32u + lane;
-                        if (t * kTile + static_cast<int32_t>(tok) >= pc.plan.len) {
+                        if (t * kTile + static_cast<int32_t>(tok) >= pc.len) {
                             uint8_t* v = vbuf + vs * C::kBuf + tok * 128u;
 #pragma unroll
                             for (int c = 0; c < DC; ++c)
@@ -928,7 +1110,7 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                     if (lane == 0) bar_arrive(&sh.wfull[grp]);
                 }
                 // the rows' sums over the warp's tokens
-                fold_lanes<V>(l, lane, add_op);
+                fold_lanes<kFold>(l, lane, add_op);
                 if (np >= 1) bar_wait(&sh.lempty, (np - 1u) & 1u, gave_up);
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
@@ -937,11 +1119,42 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lfull);
-                ++np;
+            }
+            if (grp == 0) join_pieces<DC>(a, sh, reinterpret_cast<float*>(dyn), warp - 4u);
+        } else {
+        set_regs<C::kRegsHelp, C::kRegsLaunch>();
+        if (warp == C::kThreads / 32 - 1) {
+            // ---- the walk: pieces are published ahead of the roles ----
+            for (uint32_t np = 1; sh.piece[(np - 1u) % kPieces].rows != 0u; ++np) {
+                Piece pc;
+                const bool any = next_piece(a.shape, a.b, shift, walk, &pc);
+                volatile uint32_t* done = &sh.pieces_done;
+                for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i) __nanosleep(64);
+                __syncwarp();
+                if (__any_sync(kFull, np - *done > 12u)) break;  // (given up)
+                if (lane == 0) {
+                    sh.piece[np % kPieces] = rec_of(any, pc);
+                    bar_arrive(&sh.pfull[np % kPieces]);
+                }
+                __syncwarp();
+            }
+        } else {
+            // ---- queries: of the pieces after the first ----
+            const uint32_t h = warp - (8u + 4u * G);
+            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                const uint32_t qb = np & 1u, rs = np % kQSlots;
+                if (np >= 2) bar_wait(&sh.qempty[qb], ((np >> 1) - 1u) & 1u, gave_up);
+                if (np > 0) stage_queries<R, DC, NB, G, 2>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], h, 3u);
+                __syncwarp();
+                if (lane == 0) {
+                    bar_arrive(&sh.qfull[qb]);
+                    bar_arrive(&sh.rfull[rs]);
+                }
             }
         }
+        }
     }
-    if (warp == 3) {
+    if (warp == C::kThreads / 32 - 1) {
         // statuses, over the grid
         for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
             const bool ok = seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
@@ -969,25 +1182,26 @@ __global__ void __launch_bounds__(Cfg<R, DC>::kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
 }
 
-template <int R, int DC>
-cudaError_t launch(const MmaArgs& m, const CUtensorMap& k, const CUtensorMap& v, uint32_t n_sms, cudaStream_t stream) {
-    using C = Cfg<R, DC>;
+template <int R, int DC, int NB, int G>
+cudaError_t launch(const MmaArgs& m, const CUtensorMap& k, const CUtensorMap& v, uint32_t rt, uint32_t n_sms,
+                   cudaStream_t stream) {
+    using C = Cfg<R, DC, NB, G>;
     static std::atomic<uint64_t> ready{0};  // the shared-memory opt-in is set once per device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(ready.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(attend_mma_kernel<R, DC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(attend_mma_kernel<R, DC, NB, G>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(C::kDyn));
         if (e != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_acq_rel);
     }
     const uint32_t ctas = n_sms < kAttnMaxCtas ? n_sms : kAttnMaxCtas;
     MmaArgs args = m;
-    args.a.shape.rt = R;
+    args.a.shape.rt = rt;
     args.a.shape.tile_shift = kTileShift;
-    attend_mma_kernel<R, DC><<<ctas, C::kThreads, C::kDyn, stream>>>(args, k, v);
+    attend_mma_kernel<R, DC, NB, G><<<ctas, C::kThreads, C::kDyn, stream>>>(args, k, v);
     return cudaGetLastError();
 }
 
@@ -1028,13 +1242,20 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
                   ? 1u
                   : 0u;
     const uint64_t rows = static_cast<uint64_t>(max_new ? max_new : 1u) * a.shape.group;
+    // rows of a row tile: what deals `rows` out evenly, in the blocks of 8 rows that the softmax works in (72 rows
+    // are 40 and 32, not 64 and 8)
+    const uint64_t most = a.g.head_dim <= 128 ? 64 : 32, tiles = (rows + most - 1) / most;
+    const uint32_t rt = static_cast<uint32_t>((((rows + tiles - 1) / tiles) + 7u) & ~7ull);
     if (a.g.head_dim <= 128) {
-        if (rows <= 16) return launch<16, 1>(m, k_map, v_map, n_sms, stream);
-        if (rows <= 32) return launch<32, 1>(m, k_map, v_map, n_sms, stream);
-        return launch<64, 1>(m, k_map, v_map, n_sms, stream);
+        if (rt <= 8) return launch<16, 1, 1, 3>(m, k_map, v_map, rt, n_sms, stream);
+        if (rt <= 16) return launch<16, 1, 2, 3>(m, k_map, v_map, rt, n_sms, stream);
+        if (rt <= 32) return launch<32, 1, 4, 2>(m, k_map, v_map, rt, n_sms, stream);
+        if (rt <= 40) return launch<64, 1, 5, 2>(m, k_map, v_map, rt, n_sms, stream);
+        return launch<64, 1, 8, 2>(m, k_map, v_map, rt, n_sms, stream);
     }
-    if (rows <= 16) return launch<16, 2>(m, k_map, v_map, n_sms, stream);
-    return launch<32, 2>(m, k_map, v_map, n_sms, stream);
+    if (rt <= 8) return launch<16, 2, 1, 3>(m, k_map, v_map, rt, n_sms, stream);
+    if (rt <= 16) return launch<16, 2, 2, 3>(m, k_map, v_map, rt, n_sms, stream);
+    return launch<32, 2, 4, 2>(m, k_map, v_map, rt, n_sms, stream);
 }
 
 }  // namespace sixi_b200
