@@ -475,7 +475,6 @@ struct sixi_kv {
     uint32_t* seq_state;  // [2 * max_seqs], zero between calls
     uint32_t* counter;    // [kAttnMaxCtas], zero between calls
     float* part;          // attention's partial results
-    uint64_t part_stride;
     CUtensorMap k_map, v_map;  // pages as attention copies them
 };
 
@@ -598,11 +597,12 @@ int32_t sixi_kv_create(int32_t device, const sixi_kv_config* c, void* k_pages, v
     while ((1u << shift) < P) ++shift;
     h->g = KvGeom{static_cast<uint8_t*>(k_pages), static_cast<uint8_t*>(v_pages), k_scales, v_scales, c->n_pages, P, shift,
                   c->n_kv_heads, c->head_dim};
-    h->part_stride = static_cast<uint64_t>(kPartRows) * (c->head_dim + 2u);
+    // 64 rows a CTA for one CTA per SM, or 16 for two
+    const uint64_t part = 2ull * h->n_sms * part_floats(64, c->head_dim);
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&h->seq_state), sizeof(uint32_t) * 2u * c->max_seqs);
     if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&h->counter), sizeof(uint32_t) * kAttnMaxCtas);
     if (e == cudaSuccess)
-        e = cudaMalloc(reinterpret_cast<void**>(&h->part), sizeof(float) * 2u * kAttnMaxCtas * h->part_stride);
+        e = cudaMalloc(reinterpret_cast<void**>(&h->part), sizeof(float) * part);
     if (e == cudaSuccess) e = cudaMemset(h->seq_state, 0, sizeof(uint32_t) * 2u * c->max_seqs);
     if (e == cudaSuccess) e = cudaMemset(h->counter, 0, sizeof(uint32_t) * kAttnMaxCtas);
     if (e == cudaSuccess) e = make_page_map(k_pages, h->g, &h->k_map);
@@ -743,7 +743,6 @@ int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch*
     a.status = out_status;
     a.part = h->part;
     a.counter = h->counter;
-    a.part_stride = h->part_stride;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return kv_from_cuda(q->dtype == SIXI_SMP_BF16
                             ? launch_attend_bf16(a, h->k_map, h->v_map, b->max_new, h->n_sms, s)

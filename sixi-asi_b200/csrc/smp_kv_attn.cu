@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
                         (sm.m[tid] + log2f(sm.l[tid])) * kLn2;
                 }
             } else {
-                part[kPartRows * D + tid] = sm.m[tid];
-                part[kPartRows * (D + 1u) + tid] = sm.l[tid];
+                part[kRt * D + tid] = sm.m[tid];
+                part[kRt * (D + 1u) + tid] = sm.l[tid];
             }
         }
         if (whole) continue;
@@ -292,12 +292,12 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
             const uint32_t r = i / D, d = i - r * D;
             float M = kNegInf, l = 0.0f, o = 0.0f;
             for (uint32_t c = c0; c <= c1; ++c)
-                M = fmaxf(M, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kPartRows * D + r));
+                M = fmaxf(M, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kRt * D + r));
             for (uint32_t c = c0; c <= c1; ++c) {
                 const float* p = a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride;
-                const float m = __ldcg(p + kPartRows * D + r);
+                const float m = __ldcg(p + kRt * D + r);
                 const float f = m == M ? 1.0f : exp2f(m - M);
-                l += __ldcg(p + kPartRows * (D + 1u) + r) * f;
+                l += __ldcg(p + kRt * (D + 1u) + r) * f;
                 o += __ldcg(p + r * D + d) * f;
             }
             const uint32_t rr = r_base + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
@@ -317,6 +317,7 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
 cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, cudaStream_t stream) {
     a.shape.rt = kRt;
     a.shape.tile_shift = kTileShift;
+    a.part_stride = part_floats(kRt, a.g.head_dim);
     const uint32_t D = a.g.head_dim;
     const size_t smem = sizeof(float) * (static_cast<size_t>(kRt) * D + 4u * kT * (D + 16u) / 4u + 4u * kT + 2u * kRt * kT +
                                          4096u + 3u * kRt);

@@ -305,7 +305,7 @@ struct Shared {
     alignas(16) float2 ref[4 * G][R];                       // [softmax warp] running maximum, weight factor
     float rescale[4 * G][R];                    // [softmax warp] factor of the older sums
     float osc[G][R], mgrp[G][R];            // a tile's factor, and the running maximum that its weights are under
-    uint64_t row_at[4][R];                  // [output warp] where a row goes
+    alignas(16) uint64_t row_at[4][R];      // [output warp] where a row goes
     alignas(16) float fac[4][R], facold[4][R];  // [output warp] a tile's factor, the older sums' factor
     float lsum[G][4][R], mfin[G][R];        // [group][warp] a piece's sums; [group] maxima
 };
@@ -447,9 +447,9 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, float* tm
             const uint32_t gr = min(group, rows - g0);
             for (uint32_t i = t; i < n * gr; i += 256u) {
                 const uint32_t c = i / gr, r = i - c * gr;
-                const float* p = piece_of(c) + kPartRows * D + g0 + r;
+                const float* p = piece_of(c) + a.shape.rt * D + g0 + r;
                 fm[i] = __ldcg(p);
-                fl[i] = __ldcg(p + kPartRows);
+                fl[i] = __ldcg(p + a.shape.rt);
             }
             asm volatile("bar.sync 14, 256;" ::: "memory");
             if (t < gr) {
@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lempty);
                 const bool whole = pc.t0 == pc.first && pc.t1 == pc.end;
-                const uint32_t mine = (pc.t0 == pc.first ? 1u : 0u);
+                const uint32_t mine = (pc.t0 == pc.first ? 1u : 0u), rows = pc.rows;
                 if (whole) {
                     // where each row goes: worked out by the lanes, a column each
                     __syncwarp();
@@ -836,37 +836,45 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                         }
                     }
                     __syncwarp();
-                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.data);
+                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.data) + d0;
+                    // (four columns at a time: their places and factors are read together, the stores are predicated)
 #pragma unroll
-                    for (int col = 0; col < R; ++col) {
-                        if (row_of<V>(col) >= pc.rows) continue;
-                        const float inv = facold[col];
-                        __nv_bfloat16* p = out + sh.row_at[quad][col];
+                    for (int col = 0; col < R; col += 4) {
+                        if (row_of<V>(col) >= 8u * NB) continue;
+                        const float4 inv = *reinterpret_cast<const float4*>(facold + col);
+                        const float f[4] = {inv.x, inv.y, inv.z, inv.w};
+                        const ulonglong2 at0 = *reinterpret_cast<const ulonglong2*>(&sh.row_at[quad][col]);
+                        const ulonglong2 at1 = *reinterpret_cast<const ulonglong2*>(&sh.row_at[quad][col + 2]);
+                        const uint64_t at[4] = {at0.x, at0.y, at1.x, at1.y};
 #pragma unroll
-                        for (int c = 0; c < DC; ++c) {
-                            const float2 y = un2(acc[c][col / 2]);
-                            if (c * 128u + d0 < D) p[c * 128u + d0] = __float2bfloat16_rn(((col & 1) ? y.y : y.x) * inv);
-                        }
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int c = 0; c < DC; ++c) {
+                                const float2 y = un2(acc[c][(col + i) / 2]);
+                                const __nv_bfloat16 v = __float2bfloat16_rn(((i & 1) ? y.y : y.x) * f[i]);
+                                if (row_of<V>(col + i) < rows && c * 128u + d0 < D) out[at[i] + c * 128u] = v;
+                            }
                     }
                 } else {
-                    float* part = a.part + (2ull * blockIdx.x + mine) * a.part_stride;
+                    float* part = a.part + (2ull * blockIdx.x + mine) * a.part_stride + d0;
 #pragma unroll
                     for (int col = 0; col < R; ++col) {
-                        const uint32_t r = row_of<V>(col);
-                        if (r >= pc.rows) continue;
+                        if (row_of<V>(col) >= 8u * NB) continue;
 #pragma unroll
                         for (int c = 0; c < DC; ++c) {
                             const float2 y = un2(acc[c][col / 2]);
-                            if (c * 128u + d0 < D) part[r * D + c * 128u + d0] = (col & 1) ? y.y : y.x;
+                            if (row_of<V>(col) < rows && c * 128u + d0 < D)
+                                part[row_of<V>(col) * D + c * 128u] = (col & 1) ? y.y : y.x;
                         }
                     }
+                    part -= d0;
                     if (quad == 0) {
 #pragma unroll
                         for (int i = 0; i < kPer; ++i) {
                             const uint32_t col = lane + 32u * i, r = row_of<V>(col);
                             if (col < R && r < pc.rows) {
-                                part[kPartRows * D + r] = fac[col];
-                                part[kPartRows * (D + 1u) + r] = facold[col];
+                                part[a.shape.rt * D + r] = fac[col];
+                                part[a.shape.rt * (D + 1u) + r] = facold[col];
                             }
                         }
                     }
@@ -1200,6 +1208,7 @@ cudaError_t launch(const MmaArgs& m, const CUtensorMap& k, const CUtensorMap& v,
     const uint32_t ctas = n_sms < kAttnMaxCtas ? n_sms : kAttnMaxCtas;
     MmaArgs args = m;
     args.a.shape.rt = rt;
+    args.a.part_stride = part_floats(rt, m.a.g.head_dim);
     args.a.shape.tile_shift = kTileShift;
     attend_mma_kernel<R, DC, NB, G><<<ctas, C::kThreads, C::kDyn, stream>>>(args, k, v);
     return cudaGetLastError();

@@ -55,23 +55,41 @@ def _dev_index(device) -> int:
     return d.index if d.index is not None else torch.cuda.current_device()
 
 
-def _stream(stream) -> int:
-    import torch
+class _Caller:
+    """What the calls of one handle share: a step makes one or two of them a layer, so the records that they pass
+    are made once and filled in place (a handle serves one thread at a time), and the stream is asked for
+    without making a torch object of it."""
 
-    return int((stream if stream is not None else torch.cuda.current_stream()).cuda_stream)
+    def __init__(self, device: int):
+        import torch
 
+        self.torch, self.device, self.dev = torch, device, torch.device("cuda", device)
+        self.dtypes = {torch.float32: F32, torch.bfloat16: BF16}
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.views = (KvTensor(), KvTensor())
+        self.at = tuple(ctypes.addressof(v) for v in self.views)
 
-def _view(t, device: int, dim: int, what: str) -> KvTensor:
-    """[tokens, heads, dim] rows of a torch tensor with unit stride along dim."""
-    import torch
+    def stream(self, stream) -> int:
+        if stream is not None:
+            return int(stream.cuda_stream)
+        if self.raw_stream is not None:
+            return self.raw_stream(self.device)
+        return int(self.torch.cuda.current_stream(self.device).cuda_stream)
 
-    if t.dtype not in (torch.float32, torch.bfloat16) or t.dim() != 3 or t.shape[2] != dim:
-        raise ValueError(f"{what}: fp32 or bf16 [tokens, heads, {dim}] expected, got {t.dtype} {tuple(t.shape)}")
-    if t.device.type != "cuda" or t.device.index != device:
-        raise ValueError(f"{what}: on {t.device}, not cuda:{device}")
-    if t.stride(2) != 1:
-        raise ValueError(f"{what}: the last dimension must have unit stride")
-    return KvTensor(t.data_ptr(), F32 if t.dtype == torch.float32 else BF16, t.shape[1], t.stride(0), t.stride(1))
+    def view(self, i: int, t, tokens: int, dim: int, what: str) -> int:
+        """Record i filled with t [tokens, heads, dim] (unit stride along dim); its address."""
+        dt = self.dtypes.get(t.dtype)
+        shape = t.shape
+        if dt is None or len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+            raise ValueError(f"{what}: fp32 or bf16 [{tokens}, heads, {dim}] expected, got {t.dtype} {tuple(shape)}")
+        if not t.is_cuda or t.get_device() != self.device:
+            raise ValueError(f"{what}: on {t.device}, not cuda:{self.device}")
+        stride = t.stride()
+        if stride[2] != 1:
+            raise ValueError(f"{what}: the last dimension must have unit stride")
+        v = self.views[i]
+        v.data, v.dtype, v.n_heads, v.token_stride, v.head_stride = t.data_ptr(), dt, shape[1], stride[0], stride[1]
+        return self.at[i]
 
 
 class Rope:
@@ -85,6 +103,7 @@ class Rope:
             raise ValueError(f"unknown rotary layout {layout!r} or scaling {scaling!r}")
         self.h = None
         self.device = _dev_index(device)
+        self.call = _Caller(self.device)
         self.rot_dim = rot_dim
         c = RopeConfig(rot_dim, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], original_max_position, base, factor,
                        beta_fast, beta_slow)
@@ -106,17 +125,15 @@ class Rope:
     def apply(self, x, positions, inverse: bool = False, out=None, stream=None):
         """x [tokens, heads, dim] turned by positions [tokens] (int32); inverse turns back (the gradient).
         out may be x."""
-        import torch
-
-        if positions.dtype != torch.int32 or positions.shape != (x.shape[0],) or not positions.is_contiguous():
+        c, n, dim = self.call, x.shape[0], x.shape[-1]
+        if positions.dtype != c.torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
             raise ValueError("positions: contiguous int32 [tokens] expected")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = c.torch.empty_like(x)
         elif out.shape != x.shape:
             raise ValueError(f"out: {tuple(x.shape)} expected, got {tuple(out.shape)}")
-        xv, ov = _view(x, self.device, x.shape[2], "x"), _view(out, self.device, x.shape[2], "out")
-        st = _lib().sixi_kv_rope_apply(self.h, ctypes.byref(xv), _ptr(positions), x.shape[0], x.shape[2],
-                                       1 if inverse else 0, ctypes.byref(ov), _stream(stream))
+        st = _lib().sixi_kv_rope_apply(self.h, c.view(0, x, n, dim, "x"), positions.data_ptr(), n, dim, 1 if inverse else 0,
+                                       c.view(1, out, n, dim, "out"), c.stream(stream))
         _check("sixi_kv_rope_apply", st)
         return out
 
@@ -140,6 +157,7 @@ class KvBatch:
         self.n_seqs, self.n_tokens, self.max_new = n, int(n_tokens), int(max_new)
         self.struct = KvBatchStruct(page_table.data_ptr(), page_table.stride(0), offsets.data_ptr(), lens.data_ptr(), n,
                                     page_table.shape[1], self.n_tokens, self.max_new)
+        self.at = ctypes.addressof(self.struct)
 
 
 class KvCache:
@@ -154,7 +172,8 @@ class KvCache:
         self.h = None
         given = next((t for t in (k_pages, v_pages, k_scales, v_scales) if t is not None), None)
         self.device = _dev_index(given.device if device is None and given is not None else device)
-        dev = torch.device("cuda", self.device)
+        self.call = _Caller(self.device)
+        dev = self.call.dev
         shape = (n_pages, n_kv_heads, page_size, head_dim)
 
         def buffer(t, shape, dtypes, what):
@@ -188,43 +207,34 @@ class KvCache:
         except Exception:
             pass
 
-    def _tensor(self, t, batch: KvBatch, what: str) -> KvTensor:
-        if t.dim() != 3 or t.shape[0] != batch.n_tokens:
-            raise ValueError(f"{what}: [{batch.n_tokens}, heads, {self.head_dim}] expected, got {tuple(t.shape)}")
-        return _view(t, self.device, self.head_dim, what)
-
     def _status(self, status, batch: KvBatch):
-        import torch
-
+        t = self.call.torch
         if status is None:
-            return torch.empty(batch.n_seqs, dtype=torch.int32, device=torch.device("cuda", self.device))
-        if status.dtype != torch.int32 or status.shape != (batch.n_seqs,) or not status.is_contiguous():
+            return t.empty(batch.n_seqs, dtype=t.int32, device=self.call.dev)
+        if status.dtype != t.int32 or status.shape != (batch.n_seqs,) or not status.is_contiguous():
             raise ValueError(f"status: contiguous int32 [{batch.n_seqs}] expected")
         return status
 
     def append(self, k, v, batch: KvBatch, rope: Rope | None = None, status=None, stream=None):
         """Writes k, v [tokens, n_kv_heads, head_dim] at the batch's positions, the keys turned by rope.
         Returns the status of each sequence (int32, device)."""
-        kv, vv = self._tensor(k, batch, "k"), self._tensor(v, batch, "v")
+        c, n, dim = self.call, batch.n_tokens, self.head_dim
         status = self._status(status, batch)
-        st = _lib().sixi_kv_append(self.h, ctypes.byref(kv), ctypes.byref(vv), ctypes.byref(batch.struct),
-                                   rope.h if rope is not None else None, _ptr(status), _stream(stream))
+        st = _lib().sixi_kv_append(self.h, c.view(0, k, n, dim, "k"), c.view(1, v, n, dim, "v"), batch.at,
+                                   rope.h if rope is not None else None, status.data_ptr(), c.stream(stream))
         _check("sixi_kv_append", st)
         return status
 
     def read(self, batch: KvBatch, dtype=None, k=None, v=None, status=None, stream=None):
         """The batch's positions as values: k, v [tokens, n_kv_heads, head_dim] (dtype bf16 or fp32)."""
-        import torch
-
+        c, n, dim = self.call, batch.n_tokens, self.head_dim
         if k is None or v is None:
-            dt = dtype or torch.bfloat16
-            shape, dev = (batch.n_tokens, self.n_kv_heads, self.head_dim), torch.device("cuda", self.device)
-            k = torch.empty(shape, dtype=dt, device=dev) if k is None else k
-            v = torch.empty(shape, dtype=dt, device=dev) if v is None else v
-        kv, vv = self._tensor(k, batch, "k"), self._tensor(v, batch, "v")
+            dt = dtype or c.torch.bfloat16
+            k = c.torch.empty((n, self.n_kv_heads, dim), dtype=dt, device=c.dev) if k is None else k
+            v = c.torch.empty((n, self.n_kv_heads, dim), dtype=dt, device=c.dev) if v is None else v
         status = self._status(status, batch)
-        st = _lib().sixi_kv_read(self.h, ctypes.byref(batch.struct), ctypes.byref(kv), ctypes.byref(vv), _ptr(status),
-                                 _stream(stream))
+        st = _lib().sixi_kv_read(self.h, batch.at, c.view(0, k, n, dim, "k"), c.view(1, v, n, dim, "v"), status.data_ptr(),
+                                 c.stream(stream))
         _check("sixi_kv_read", st)
         return k, v
 
@@ -232,21 +242,19 @@ class KvCache:
                rope: Rope | None = None, out=None, lse=None, status=None, stream=None):
         """Attention of q [tokens, n_q_heads, head_dim] over the cache: (out like q, lse fp32 [tokens,
         n_q_heads], status int32 [seqs]). scale defaults to head_dim ** -0.5; window 0 is none."""
-        import torch
-
+        c, n, dim = self.call, batch.n_tokens, self.head_dim
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = c.torch.empty_like(q)
         elif out.shape != q.shape:
             raise ValueError(f"out: {tuple(q.shape)} expected, got {tuple(out.shape)}")
         if lse is None:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        elif lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
+            lse = c.torch.empty(q.shape[:2], dtype=c.torch.float32, device=c.dev)
+        elif lse.dtype != c.torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous fp32 {tuple(q.shape[:2])} expected")
-        qv, ov = self._tensor(q, batch, "q"), self._tensor(out, batch, "out")
         status = self._status(status, batch)
-        st = _lib().sixi_kv_attend(self.h, ctypes.byref(qv), ctypes.byref(batch.struct),
-                                   self.head_dim ** -0.5 if scale is None else scale, window,
-                                   0 if causal else ATTEND_ALL, rope.h if rope is not None else None, ctypes.byref(ov),
-                                   _ptr(lse), _ptr(status), _stream(stream))
+        st = _lib().sixi_kv_attend(self.h, c.view(0, q, n, dim, "q"), batch.at,
+                                   dim ** -0.5 if scale is None else scale, window, 0 if causal else ATTEND_ALL,
+                                   rope.h if rope is not None else None, c.view(1, out, n, dim, "out"), lse.data_ptr(),
+                                   status.data_ptr(), c.stream(stream))
         _check("sixi_kv_attend", st)
         return out, lse, status
