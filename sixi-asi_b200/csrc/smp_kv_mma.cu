@@ -50,7 +50,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait (never expected to run out)
 constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
 constexpr uint32_t kPieces = 16; // piece records kept; the walk stays 12 ahead of the output at most
-constexpr int kQSlots = 8;  // pieces whose row records are kept: softmax lags the staging by fewer than 5
+constexpr int kQSlots = 16;  // pieces whose row records are kept: softmax lags the staging by fewer than 10
 
 // R columns for the rows of a row tile, of which the first 8 * NB are used, DC 128-element chunks of a head, G softmax
 // groups
@@ -59,16 +59,17 @@ struct Cfg {
     static constexpr int kThreads = 384 + 128 * G;
     // Registers of a thread by role: copies and products need few, output sums and softmax many. The shares of the
     // warpgroups add up to what the block is launched with (96 a thread for 5 warpgroups, 80 for 6).
-    static constexpr int kRegsLaunch = G == 2 ? 96 : 80, kRegsIssue = 48, kRegsHelp = 56;
-    static constexpr int kRegsOut = G == 2 ? 136 : 88, kRegsSoft = G == 2 ? 120 : 96;
+    static constexpr int kRegsLaunch = G == 2 ? 96 : 80, kRegsIssue = 48, kRegsHelp = G == 2 ? 72 : 80;
+    static constexpr int kRegsOut = G == 2 ? 136 : 88, kRegsSoft = G == 2 ? 112 : 88;
     static_assert(kRegsIssue + kRegsHelp + kRegsOut + G * kRegsSoft <= (3 + G) * kRegsLaunch, "registers");
     static constexpr int V = R / 4;                       // rows of a softmax thread
     static constexpr uint32_t kChunk = kTile * 128u;      // bytes of a tile's chunk of keys or values
     static constexpr uint32_t kBuf = DC * kChunk;
     static constexpr uint32_t kQ = DC * 2u * R * 128u;    // hi rows, lo rows, chunk by chunk
     static constexpr uint32_t kW = 2u * R * kTile;        // hi, lo
-    static constexpr uint32_t kFixed = 2u * kQ + G * kW;
-    static constexpr uint32_t kSmall = 4096u + (132u + 108u * G) * R;  // bound of the small arrays
+    static constexpr int kNQ = R == 16 ? 4 : 2;           // pieces whose queries are staged
+    static constexpr uint32_t kFixed = kNQ * kQ + G * kW;
+    static constexpr uint32_t kSmall = 7168u + (196u + 108u * G) * R;  // bound of the small arrays
     static constexpr int kBufs = static_cast<int>((227u * 1024u - 1024u - kSmall - kFixed) / kBuf);
     static constexpr int kNK = kBufs / 2 > 6 ? 6 : kBufs / 2;            // tiles of keys in flight
     static constexpr int kNV = kBufs - kNK > 6 ? 6 : kBufs - kNK;        // and of values
@@ -138,11 +139,12 @@ __device__ __forceinline__ void warps_meet(uint64_t* b, uint32_t* times, volatil
     ++*times;
 }
 
-__device__ __forceinline__ void tma_page(const CUtensorMap* map, void* dst, uint64_t* bar, int32_t x, int32_t z) {
+__device__ __forceinline__ void tma_page(const CUtensorMap* map, void* dst, uint64_t* bar, int32_t x, int32_t z,
+                                         uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-            s32(dst)),
-        "l"(map), "r"(s32(bar)), "r"(x), "r"(0), "r"(z)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, "
+        "%5}], [%2], %6;" ::"r"(s32(dst)),
+        "l"(map), "r"(s32(bar)), "r"(x), "r"(0), "r"(z), "l"(policy)
         : "memory");
 }
 
@@ -288,10 +290,10 @@ __device__ __forceinline__ PieceRec rec_of(bool any, const Piece& pc) {
 
 template <int R, int DC, int NB, int G>
 struct Shared {
-    static constexpr int kNK = Cfg<R, DC, NB, G>::kNK, kNV = Cfg<R, DC, NB, G>::kNV;
+    static constexpr int kNK = Cfg<R, DC, NB, G>::kNK, kNV = Cfg<R, DC, NB, G>::kNV, kNQ = Cfg<R, DC, NB, G>::kNQ;
     uint64_t kfull[kNK], vfull[kNV], scfull[kNV];
     uint64_t sfull[kRing], ofull[kRing];  // of tile n at n % kRing: its scores, its output are done
-    uint64_t sempty[G], wfull[G], oempty[G], qfull[2], qempty[2], rfull[kQSlots], pfull[kPieces], meet[G], lfull, lempty,
+    uint64_t sempty[G], wfull[G], oempty[G], qfull[kNQ], qempty[kNQ], rfull[kQSlots], pfull[kPieces], meet[G], lfull, lempty,
         done;
     unsigned long long scratch[Cfg<R, DC, NB, G>::kThreads / 32 + 2];
     PieceRec piece[kPieces], split[2];
@@ -305,6 +307,7 @@ struct Shared {
     alignas(16) float2 ref[4 * G][R];                       // [softmax warp] running maximum, weight factor
     float rescale[4 * G][R];                    // [softmax warp] factor of the older sums
     float osc[G][R], mgrp[G][R];            // a tile's factor, and the running maximum that its weights are under
+    float2 sines[3][128];                   // [staging warp] of a token's pairs
     alignas(16) uint64_t row_at[4][R];      // [output warp] where a row goes
     alignas(16) float fac[4][R], facold[4][R];  // [output warp] a tile's factor, the older sums' factor
     float lsum[G][4][R], mfin[G][R];        // [group][warp] a piece's sums; [group] maxima
@@ -313,6 +316,7 @@ struct Shared {
 struct MmaArgs {
     AttnArgs a;
     uint32_t pages_per_tile;
+    uint32_t read_once;  // no page is read by more than one row tile
     uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
 };
 
@@ -323,32 +327,78 @@ __device__ __forceinline__ constexpr uint32_t row_of(uint32_t col) {
 }
 
 // A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle), 8 elements a lane, DC * 16 lanes a row;
-// this warp takes rows `at`, `at` + `step`, ... in units of the rows that it handles at once, U units at a time.
+// this warp takes rows `at`, `at` + `step`, ... in units of the rows that it handles at once, U units at a time. Sines
+// cost more than all else here, and the rows of one token share them: where a warp's rows at a time belong to one
+// token, its lanes work the token's pairs out between them, in tab (128 places of shared memory; NULL: none).
 template <int R, int DC, int NB, int G, int U>
 __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRec& pc, uint8_t* dst, float* frow, int32_t* qpos,
-                                              uint32_t at, uint32_t step) {
+                                              uint32_t at, uint32_t step, float2* tab) {
     constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC, NB, G>::V;
     const AttnArgs& a = args.a;
     const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
     const uint32_t sub = lane / kRowLanes, d0 = (lane % kRowLanes) * 8u;
     const float sign = a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : 0.0f);
+    const bool vec = args.q_vec != 0u, turn = a.rope.turns != nullptr, mine = d0 < D;
+    const uint32_t half = a.rope.rot_dim >> 1, base = pc.row_tile * a.shape.rt, group = a.shape.group;
+    uint32_t turned = 0xFFFFFFFFu;  // the token that tab holds
     for (uint32_t rb = at * kAtOnce; rb < pc.rows; rb += step * kAtOnce * U) {
         float x[U][8], m[U];
+        uint32_t tok[U];
+        const uint32_t tok0 = (base + rb) / group;
+        const bool one = turn && tab != nullptr && vec &&
+                         (base + min(rb + (U - 1u) * step * kAtOnce + kAtOnce - 1u, pc.rows - 1u)) / group == tok0;
+        if (one && tok0 != turned) {
+            __syncwarp();
+            for (uint32_t i = lane; i < half; i += 32u) {
+                float sn, cs;
+                rope_sincos(a.rope, pc.p0 + static_cast<int32_t>(tok0), i, &sn, &cs);
+                tab[i] = make_float2(cs, sn);
+            }
+            __syncwarp();
+            turned = tok0;
+        }
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t r = rb + u * step * kAtOnce + sub;
+            const uint32_t rr = base + min(rb + u * step * kAtOnce + sub, pc.rows - 1u);
+            tok[u] = rr / group;
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.row0 + tok[u]) * a.q.token_stride +
+                                     (pc.head * group + rr - tok[u] * group) * a.q.head_stride;
+            const int32_t pos = pc.p0 + static_cast<int32_t>(tok[u]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
-            if (r < pc.rows && d0 < D) {
-                const uint32_t rr = pc.row_tile * a.shape.rt + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
-                const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.row0 + tok) * a.q.token_stride +
-                                         (pc.head * a.shape.group + g) * a.q.head_stride;
-                const int32_t pos = pc.p0 + static_cast<int32_t>(tok);
-                if (args.q_vec) {
-                    load_turned<__nv_bfloat16, 8>(a.rope, p, d0, pos, x[u]);
-                } else {
+            if (!mine) continue;
+            if (!vec) {
+#pragma unroll 1
+                for (uint32_t j = 0; j < 8; ++j) {
+                    float y;
+                    load_turned<__nv_bfloat16, 1>(a.rope, p, d0 + j, pos, &y);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) load_turned<__nv_bfloat16, 1>(a.rope, p, d0 + j, pos, &x[u][j]);
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (i == j) x[u][i] = y;
+                }
+            } else if (turn && !one) {
+                load_turned<__nv_bfloat16, 8>(a.rope, p, d0, pos, x[u]);
+            } else {
+                load_vec<__nv_bfloat16, 8>(p + d0, x[u]);
+                if (turn && d0 < a.rope.rot_dim) {
+                    if (a.rope.interleaved) {
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const float2 t = tab[(d0 + j) >> 1];
+                            const float y = x[u][j] * t.x - x[u][j + 1] * t.y;
+                            x[u][j + 1] = x[u][j + 1] * t.x + x[u][j] * t.y;
+                            x[u][j] = y;
+                        }
+                    } else {
+                        const bool upper = d0 >= half;
+                        float o[8];
+                        load_vec<__nv_bfloat16, 8>(p + (upper ? d0 - half : d0 + half), o);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 t = tab[(upper ? d0 - half : d0) + j];
+                            x[u][j] = upper ? x[u][j] * t.x + o[j] * t.y : x[u][j] * t.x - o[j] * t.y;
+                        }
+                    }
                 }
             }
         }
@@ -358,7 +408,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // a turned query is rounded to its type, as a rotation of its own would be
-                x[u][j] = __bfloat162float(__float2bfloat16_rn(x[u][j]));
+                if (turn) x[u][j] = __bfloat162float(__float2bfloat16_rn(x[u][j]));
                 const float ab = fabsf(x[u][j]);
                 m[u] = ab < __builtin_huge_valf() ? fmaxf(m[u], ab) : __builtin_huge_valf();
             }
@@ -391,25 +441,19 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
                 // (positive, so that a masked score stays -inf; at 1e-30 scores are zero all the same)
                 frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
-                qpos[col] = pc.p0 + static_cast<int32_t>((pc.row_tile * a.shape.rt + r) / a.shape.group);
+                qpos[col] = pc.p0 + static_cast<int32_t>(tok[u]);
             }
         }
     }
     fence_async_smem();
 }
 
-__device__ __forceinline__ void join_add(const float* p, float f, float4* o) {
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
-    o->x = fmaf(v.x, f, o->x), o->y = fmaf(v.y, f, o->y), o->z = fmaf(v.z, f, o->z), o->w = fmaf(v.w, f, o->w);
-}
-
 // Units that were cut: the last of their CTAs to arrive joins the pieces, in CTA order. The output's four warps and
 // four of the softmax's do it (w: 0 to 7) after all of this CTA's own tiles, so that nothing of it waits for the
-// joining; `tmp` is shared memory that the tiles no longer need.
+// joining.
 template <int DC, typename Sh>
-__device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, float* tmp, uint32_t w) {
-    constexpr uint32_t kTable = 8192;  // factors of (piece, row) kept at a time
-    const uint32_t lane = threadIdx.x & 31u, t = w * 32u + lane, D = a.g.head_dim;
+__device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, uint32_t w) {
+    const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
     __threadfence();
     asm volatile("bar.sync 14, 256;" ::: "memory");
     if (w == 0) {
@@ -438,82 +482,86 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, float* tm
         const float* first = a.part + (2ull * c0 + 1u) * a.part_stride;       // the piece of c0 is its CTA's last
         const float* rest = a.part + (2ull * c0) * a.part_stride;             // the others' are their CTA's first
         const auto piece_of = [&](uint32_t c) { return c == 0 ? first : rest + 2ull * c * a.part_stride; };
-        float* fm = tmp;              // [n][rows] maxima, then factors
-        float* fl = tmp + kTable;     // [n][rows] sums
-        float* norm = fl + kTable;    // [rows]
-        // (n * rows is at most the CTAs times 64: beyond the table, rows are taken in groups)
-        const uint32_t group = min(rows, kTable / n);
-        for (uint32_t g0 = 0; g0 < rows; g0 += group) {
-            const uint32_t gr = min(group, rows - g0);
-            for (uint32_t i = t; i < n * gr; i += 256u) {
-                const uint32_t c = i / gr, r = i - c * gr;
-                const float* p = piece_of(c) + a.shape.rt * D + g0 + r;
-                fm[i] = __ldcg(p);
-                fl[i] = __ldcg(p + a.shape.rt);
+        // a warp a row, four elements a lane, two rows at a time; a lane holds the factor of a piece (of every 32nd)
+        for (uint32_t r0 = w; r0 < rows; r0 += 16u) {
+            const uint32_t row[2] = {r0, min(r0 + 8u, rows - 1u)};
+            float m[2], l[2], f[2], norm[2];
+            float4 o[2][DC], v[2][DC][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                m[u] = kNegInf, l[u] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
-            asm volatile("bar.sync 14, 256;" ::: "memory");
-            if (t < gr) {
-                float m = kNegInf, l = 0.0f;
-                for (uint32_t c = 0; c < n; ++c) m = fmaxf(m, fm[c * gr + t]);
-                for (uint32_t c = 0; c < n; ++c) {
-                    const float mc = fm[c * gr + t], f = mc == m ? 1.0f : ex2(mc - m);
-                    l += fl[c * gr + t] * f;
-                    fm[c * gr + t] = f;
-                }
-                norm[t] = l == 0.0f ? 0.0f : 1.0f / l;
-                if (a.lse) {
-                    const uint32_t rr = pc.row_tile * a.shape.rt + g0 + t, tok = rr / a.shape.group;
-                    a.lse[(pc.row0 + tok) * (a.shape.n_heads * a.shape.group) + pc.head * a.shape.group + rr - tok * a.shape.group] =
-                        (m + log2f(l)) * kLn2;
-                }
-            }
-            asm volatile("bar.sync 14, 256;" ::: "memory");
-            // a warp a row, four elements a lane; up to four rows at a time, so that loads are in flight
-            constexpr uint32_t kRows = 4;
-            for (uint32_t r0 = w; r0 < gr; r0 += 8u * kRows) {
-                float4 o[kRows][DC];
-                uint32_t row[kRows];
+            // (the first pieces' sums are on their way before the factors are known)
+            const auto fetch = [&](uint32_t c) {
 #pragma unroll
-                for (uint32_t u = 0; u < kRows; ++u) {
-                    row[u] = min(r0 + 8u * u, gr - 1u);
-#pragma unroll
-                    for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-                const uint32_t live = (gr - r0 + 7u) / 8u;  // rows of this warp from here on
-                if (live == 1u) {
-#pragma unroll 8
-                    for (uint32_t c = 0; c < n; ++c)
-#pragma unroll
-                        for (int k = 0; k < DC; ++k)
-                            if (k * 128u + lane * 4u < D)
-                                join_add(piece_of(c) + (g0 + row[0]) * D + k * 128u + lane * 4u, fm[c * gr + row[0]], &o[0][k]);
-                } else {
-#pragma unroll 2
-                    for (uint32_t c = 0; c < n; ++c)
-#pragma unroll
-                        for (uint32_t u = 0; u < kRows; ++u)
-#pragma unroll
-                            for (int k = 0; k < DC; ++k)
-                                if (k * 128u + lane * 4u < D)
-                                    join_add(piece_of(c) + (g0 + row[u]) * D + k * 128u + lane * 4u, fm[c * gr + row[u]], &o[u][k]);
-                }
-#pragma unroll
-                for (uint32_t u = 0; u < kRows; ++u) {
-                    if (u >= live) continue;
-                    const uint32_t rr = pc.row_tile * a.shape.rt + g0 + row[u], tok = rr / a.shape.group;
-                    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.row0 + tok) * a.out.token_stride +
-                                       (pc.head * a.shape.group + rr - tok * a.shape.group) * a.out.head_stride;
-                    const float f = norm[row[u]];
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int k = 0; k < DC; ++k)
-                        if (k * 128u + lane * 4u < D) {
-                            __nv_bfloat16* d = p + k * 128u + lane * 4u;
-                            d[0] = __float2bfloat16_rn(o[u][k].x * f), d[1] = __float2bfloat16_rn(o[u][k].y * f);
-                            d[2] = __float2bfloat16_rn(o[u][k].z * f), d[3] = __float2bfloat16_rn(o[u][k].w * f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (k * 128u + lane * 4u < D)
+                                v[u][k][i] = __ldcg(reinterpret_cast<const float4*>(piece_of(min(c + i, n - 1u)) + row[u] * D +
+                                                                                    k * 128u + lane * 4u));
+            };
+            fetch(0);
+            for (uint32_t c = lane; c < n; c += 32u)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __ldcg(piece_of(c) + a.shape.rt * D + row[u]));
+#pragma unroll
+            for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o2));
+            for (uint32_t c0l = 0; c0l < n; c0l += 32u) {
+                const uint32_t c = c0l + lane;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f[u] = 0.0f;
+                    if (c < n) {
+                        const float* p = piece_of(c) + a.shape.rt * D + row[u];
+                        const float mc = __ldcg(p);
+                        f[u] = mc == m[u] ? 1.0f : ex2(mc - m[u]);
+                        l[u] += __ldcg(p + a.shape.rt) * f[u];
+                    }
+                }
+                for (uint32_t i0 = 0; i0 < 32u && c0l + i0 < n; i0 += 4u) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const float g = __shfl_sync(0xFFFFFFFFu, f[u], i0 + i);  // (0 past the last piece)
+#pragma unroll
+                            for (int k = 0; k < DC; ++k) {
+                                if (g == 0.0f) continue;
+                                o[u][k].x = fmaf(v[u][k][i].x, g, o[u][k].x), o[u][k].y = fmaf(v[u][k][i].y, g, o[u][k].y);
+                                o[u][k].z = fmaf(v[u][k][i].z, g, o[u][k].z), o[u][k].w = fmaf(v[u][k][i].w, g, o[u][k].w);
+                            }
                         }
+                    if (c0l + i0 + 4u < n) fetch(c0l + i0 + 4u);
                 }
             }
-            asm volatile("bar.sync 14, 256;" ::: "memory");
+#pragma unroll
+            for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], o2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u == 1 && r0 + 8u >= rows) continue;
+                norm[u] = l[u] == 0.0f ? 0.0f : 1.0f / l[u];
+                const uint32_t rr = pc.row_tile * a.shape.rt + row[u], tok = rr / a.shape.group;
+                const uint32_t hq = pc.head * a.shape.group + rr - tok * a.shape.group;
+                if (a.lse && lane == 0)
+                    a.lse[(pc.row0 + tok) * (a.shape.n_heads * a.shape.group) + hq] = (m[u] + log2f(l[u])) * kLn2;
+                __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.row0 + tok) * a.out.token_stride + hq * a.out.head_stride;
+#pragma unroll
+                for (int k = 0; k < DC; ++k)
+                    if (k * 128u + lane * 4u < D) {
+                        __nv_bfloat16* d = p + k * 128u + lane * 4u;
+                        d[0] = __float2bfloat16_rn(o[u][k].x * norm[u]), d[1] = __float2bfloat16_rn(o[u][k].y * norm[u]);
+                        d[2] = __float2bfloat16_rn(o[u][k].z * norm[u]), d[3] = __float2bfloat16_rn(o[u][k].w * norm[u]);
+                    }
+            }
         }
     }
 }
@@ -523,8 +571,10 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     attend_mma_kernel(const __grid_constant__ MmaArgs args, const __grid_constant__ CUtensorMap k_map,
                       const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<R, DC, NB, G>;
-    constexpr int NK = C::kNK, NV = C::kNV;
+    constexpr int NK = C::kNK, NV = C::kNV, NQ = C::kNQ;
     constexpr uint32_t V = C::V, kStagers = C::kThreads / 32 - 2;
+    // small row tiles are staged by one warp each, three at a time; large ones by three warps
+    constexpr uint32_t kHelp = R == 16 ? 1 : 3;
     constexpr uint32_t kFull = 0xFFFFFFFFu;
     extern __shared__ uint8_t raw[];
     __shared__ Shared<R, DC, NB, G> sh;
@@ -536,28 +586,26 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     uint8_t* kbuf = dyn;
     uint8_t* vbuf = kbuf + NK * C::kBuf;
     uint8_t* qbuf = vbuf + NV * C::kBuf;
-    uint8_t* wbuf = qbuf + 2u * C::kQ;
+    uint8_t* wbuf = qbuf + NQ * C::kQ;
     volatile uint32_t* gave_up = &sh.gave_up;
 
-    if (tid == 0) {
-        for (int i = 0; i < NK; ++i) bar_init(&sh.kfull[i], 1);
-        for (int i = 0; i < NV; ++i) bar_init(&sh.vfull[i], 1), bar_init(&sh.scfull[i], 32);
-        for (int i = 0; i < kRing; ++i) bar_init(&sh.sfull[i], 1), bar_init(&sh.ofull[i], 1);
-        for (int i = 0; i < G; ++i) {
-            bar_init(&sh.sempty[i], 4);
-            bar_init(&sh.wfull[i], 4);
-            bar_init(&sh.oempty[i], 4);
+    if (warp == 0) {
+        if (lane < NK) bar_init(&sh.kfull[lane], 1);
+        if (lane < NV) bar_init(&sh.vfull[lane], 1), bar_init(&sh.scfull[lane], 32);
+        if (lane < kRing) bar_init(&sh.sfull[lane], 1), bar_init(&sh.ofull[lane], 1);
+        if (lane < G) bar_init(&sh.sempty[lane], 4), bar_init(&sh.wfull[lane], 4), bar_init(&sh.oempty[lane], 4), bar_init(&sh.meet[lane], 4);
+        if (lane < NQ) bar_init(&sh.qfull[lane], kHelp), bar_init(&sh.qempty[lane], 1);
+        if (lane < kQSlots) bar_init(&sh.rfull[lane], kHelp);
+        if (lane < kPieces) bar_init(&sh.pfull[lane], 1);
+        if (lane == 0) {
+            bar_init(&sh.lfull, 4 * G);
+            bar_init(&sh.lempty, 4);
+            bar_init(&sh.done, 2);
+            sh.gave_up = sh.pieces_done = sh.split_mask = 0u;
         }
-        for (int i = 0; i < 2; ++i) bar_init(&sh.qfull[i], 3), bar_init(&sh.qempty[i], 1);
-        for (int i = 0; i < kQSlots; ++i) bar_init(&sh.rfull[i], 3);
-        for (uint32_t i = 0; i < kPieces; ++i) bar_init(&sh.pfull[i], 1);
-        for (int i = 0; i < G; ++i) bar_init(&sh.meet[i], 4);
-        bar_init(&sh.lfull, 4 * G);
-        bar_init(&sh.lempty, 4);
-        bar_init(&sh.done, 2);
-        sh.gave_up = sh.pieces_done = sh.split_mask = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&sh.tmem)), "r"(C::kTmem)
@@ -593,7 +641,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
         if (warp != 0 && warp != 3) {
             // the first piece's queries: by every warp but the copying ones, which start at once
             stage_queries<R, DC, NB, G, (8 * NB * DC / 2 + kStagers - 1) / kStagers>(args, sh.piece[0], qbuf, sh.frow[0],
-                                                                                   sh.qpos[0], warp - (warp > 3 ? 2u : 1u), kStagers);
+                                                                                   sh.qpos[0], warp - (warp > 3 ? 2u : 1u), kStagers, nullptr);
             asm volatile("bar.sync 15, %0;" ::"n"(C::kThreads - 64) : "memory");
         }
         // the next piece, or false after the last one
@@ -614,6 +662,10 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             uint8_t* buf = is_v ? vbuf : kbuf;
             uint64_t* full = is_v ? sh.vfull : sh.kfull;
             uint64_t* done = is_v ? sh.ofull : sh.sfull;  // of tile n - n_buf: its buffer is free
+            // pages that one row tile reads once leave L2 first: partial results and queries stay
+            uint64_t policy;
+            if (args.read_once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+            else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
             uint32_t n = 0, st = 0;
             for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
                 const PieceRec& pc = *rec;
@@ -646,7 +698,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     if (lane < ppt) {
 #pragma unroll
                         for (int c = 0; c < DC; ++c)
-                            tma_page(map, buf + st * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &full[st], c * 128, z);
+                            tma_page(map, buf + st * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &full[st], c * 128, z, policy);
                     }
                     if (is_v) {
                         if (lane >= 16u) {
@@ -674,8 +726,8 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             uint32_t n = 0;
             for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
                 const PieceRec& pc = *rec;
-                const uint32_t qb = np & 1u;
-                bar_wait(&sh.qfull[qb], (np >> 1) & 1u, gave_up);
+                const uint32_t qb = np % NQ;
+                bar_wait(&sh.qfull[qb], (np / NQ) & 1u, gave_up);
                 for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
                     const uint32_t ks = n % NK, b = n % G;
                     bar_wait(&sh.kfull[ks], (n / NK) & 1u, gave_up);
@@ -887,7 +939,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 __syncwarp();
                 if (warp == 4 && lane == 0) *const_cast<volatile uint32_t*>(&sh.pieces_done) = np + 1u;
             }
-            join_pieces<DC>(a, sh, reinterpret_cast<float*>(dyn), warp - 4u);
+            join_pieces<DC>(a, sh, warp - 4u);
         } else if (warp < 8 + 4 * G) {
             set_regs<C::kRegsSoft, C::kRegsLaunch>();
             // ---- softmax: group g takes the tiles n with n % G == g ----
@@ -1128,7 +1180,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lfull);
             }
-            if (grp == 0) join_pieces<DC>(a, sh, reinterpret_cast<float*>(dyn), warp - 4u);
+            if (grp == 0) join_pieces<DC>(a, sh, warp - 4u);
         } else {
         set_regs<C::kRegsHelp, C::kRegsLaunch>();
         if (warp == C::kThreads / 32 - 1) {
@@ -1144,15 +1196,27 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     sh.piece[np % kPieces] = rec_of(any, pc);
                     bar_arrive(&sh.pfull[np % kPieces]);
                 }
+                // the piece's queries into L2: while the pages stream in, a load from memory takes some 5 us
+                if (any)
+                    for (uint32_t i = lane; i < pc.rows * 4u; i += 32u) {
+                        const uint32_t rr = pc.row_tile * a.shape.rt + (i >> 2), tok = rr / a.shape.group;
+                        const uint32_t d = min((i & 3u) * 64u, D - 1u);
+                        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                                                 (pc.head * a.shape.group + rr - tok * a.shape.group) * a.q.head_stride + d;
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+                    }
                 __syncwarp();
             }
         } else {
             // ---- queries: of the pieces after the first ----
             const uint32_t h = warp - (8u + 4u * G);
             for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
-                const uint32_t qb = np & 1u, rs = np % kQSlots;
-                if (np >= 2) bar_wait(&sh.qempty[qb], ((np >> 1) - 1u) & 1u, gave_up);
-                if (np > 0) stage_queries<R, DC, NB, G, 2>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], h, 3u);
+                if (kHelp == 1 && np % 3u != h) continue;
+                const uint32_t qb = np % NQ, rs = np % kQSlots;
+                if (np >= NQ) bar_wait(&sh.qempty[qb], (np / NQ - 1u) & 1u, gave_up);
+                if (np > 0)
+                    stage_queries<R, DC, NB, G, (R == 16 ? 4 : 2)>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], kHelp == 1 ? 0u : h,
+                                                   kHelp, sh.sines[h]);
                 __syncwarp();
                 if (lane == 0) {
                     bar_arrive(&sh.qfull[qb]);
@@ -1255,6 +1319,7 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
     // are 40 and 32, not 64 and 8)
     const uint64_t most = a.g.head_dim <= 128 ? 64 : 32, tiles = (rows + most - 1) / most;
     const uint32_t rt = static_cast<uint32_t>((((rows + tiles - 1) / tiles) + 7u) & ~7ull);
+    m.read_once = rows <= rt ? 1u : 0u;
     if (a.g.head_dim <= 128) {
         if (rt <= 8) return launch<16, 1, 1, 3>(m, k_map, v_map, rt, n_sms, stream);
         if (rt <= 16) return launch<16, 1, 2, 3>(m, k_map, v_map, rt, n_sms, stream);
