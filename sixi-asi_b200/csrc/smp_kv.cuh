@@ -190,6 +190,15 @@ __device__ __forceinline__ void load_turned(const RopeView& r, const T* p, uint3
     }
 }
 
+__device__ __forceinline__ void unpack8(uint4 v, float* x) {  // 8 bf16
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = __uint_as_float(w[j] << 16);
+        x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // attention: how a call's work is cut
 

@@ -326,13 +326,36 @@ __device__ __forceinline__ constexpr uint32_t row_of(uint32_t col) {
     return ((col % V) >> 1) * 8u + (col / V) * 2u + (col & 1u);
 }
 
-// A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle), 8 elements a lane, DC * 16 lanes a row;
-// this warp takes rows `at`, `at` + `step`, ... in units of the rows that it handles at once, U units at a time. Sines
-// cost more than all else here, and the rows of one token share them: where a warp's rows at a time belong to one
-// token, its lanes work the token's pairs out between them, in tab (128 places of shared memory; NULL: none).
+// Queries are staged 8 elements a lane, DC * 16 lanes a row; a warp takes rows `at`, `at` + `step`, ... in units of the
+// rows that it handles at once, U units at a time.
+template <int DC>
+__device__ __forceinline__ const __nv_bfloat16* query_row(const AttnArgs& a, const PieceRec& pc, uint32_t r, uint32_t* tok) {
+    const uint32_t rr = pc.row_tile * a.shape.rt + r;
+    *tok = rr / a.shape.group;
+    return static_cast<const __nv_bfloat16*>(a.q.data) + (pc.row0 + *tok) * a.q.token_stride +
+           (pc.head * a.shape.group + rr - *tok * a.shape.group) * a.q.head_stride;
+}
+template <int DC, int U>
+__device__ __forceinline__ void fetch_queries(const MmaArgs& args, const PieceRec& pc, uint32_t rb, uint32_t step, uint4* raw) {
+    constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes;
+    const uint32_t lane = threadIdx.x & 31u, d0 = (lane % kRowLanes) * 8u;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+        uint32_t tok;
+        const __nv_bfloat16* p =
+            query_row<DC>(args.a, pc, min(rb + u * step * kAtOnce + lane / kRowLanes, pc.rows - 1u), &tok);
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (args.q_vec && d0 < args.a.g.head_dim) raw[u] = *reinterpret_cast<const uint4*>(p + d0);
+    }
+}
+
+// A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle). raw: the first rows' elements, already asked for
+// (fetch_queries); further ones are asked for a round ahead, as a load may take microseconds while the pages stream in.
+// Sines cost most, and the rows of one token share them: where a warp's rows at a time belong to one token, its lanes
+// work the token's pairs out between them, in tab (128 places of shared memory; NULL: none).
 template <int R, int DC, int NB, int G, int U>
 __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRec& pc, uint8_t* dst, float* frow, int32_t* qpos,
-                                              uint32_t at, uint32_t step, float2* tab) {
+                                              uint32_t at, uint32_t step, float2* tab, uint4* raw) {
     constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC, NB, G>::V;
     const AttnArgs& a = args.a;
     const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
@@ -343,7 +366,6 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
     uint32_t turned = 0xFFFFFFFFu;  // the token that tab holds
     for (uint32_t rb = at * kAtOnce; rb < pc.rows; rb += step * kAtOnce * U) {
         float x[U][8], m[U];
-        uint32_t tok[U];
         const uint32_t tok0 = (base + rb) / group;
         const bool one = turn && tab != nullptr && vec &&
                          (base + min(rb + (U - 1u) * step * kAtOnce + kAtOnce - 1u, pc.rows - 1u)) / group == tok0;
@@ -358,50 +380,62 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             turned = tok0;
         }
 #pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t rr = base + min(rb + u * step * kAtOnce + sub, pc.rows - 1u);
-            tok[u] = rr / group;
-            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.row0 + tok[u]) * a.q.token_stride +
-                                     (pc.head * group + rr - tok[u] * group) * a.q.head_stride;
-            const int32_t pos = pc.p0 + static_cast<int32_t>(tok[u]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
-            if (!mine) continue;
-            if (!vec) {
+        for (uint32_t u = 0; u < U; ++u) unpack8(raw[u], x[u]);
+        if (!vec || (turn && !one)) {
 #pragma unroll 1
-                for (uint32_t j = 0; j < 8; ++j) {
-                    float y;
-                    load_turned<__nv_bfloat16, 1>(a.rope, p, d0 + j, pos, &y);
+            for (uint32_t u = 0; u < U; ++u) {
+                uint32_t tok;
+                const __nv_bfloat16* p = query_row<DC>(a, pc, min(rb + u * step * kAtOnce + sub, pc.rows - 1u), &tok);
+                float y[8];
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        if (i == j) x[u][i] = y;
+                for (uint32_t j = 0; j < 8; ++j) y[j] = 0.0f;
+                if (mine) {
+#pragma unroll 1
+                    for (uint32_t j = 0; j < 8; ++j) {
+                        float z;
+                        load_turned<__nv_bfloat16, 1>(a.rope, p, d0 + j, pc.p0 + static_cast<int32_t>(tok), &z);
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i)
+                            if (i == j) y[i] = z;
+                    }
                 }
-            } else if (turn && !one) {
-                load_turned<__nv_bfloat16, 8>(a.rope, p, d0, pos, x[u]);
-            } else {
-                load_vec<__nv_bfloat16, 8>(p + d0, x[u]);
-                if (turn && d0 < a.rope.rot_dim) {
-                    if (a.rope.interleaved) {
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const float2 t = tab[(d0 + j) >> 1];
-                            const float y = x[u][j] * t.x - x[u][j + 1] * t.y;
-                            x[u][j + 1] = x[u][j + 1] * t.x + x[u][j] * t.y;
-                            x[u][j] = y;
-                        }
-                    } else {
-                        const bool upper = d0 >= half;
-                        float o[8];
-                        load_vec<__nv_bfloat16, 8>(p + (upper ? d0 - half : d0 + half), o);
+                for (uint32_t v = 0; v < U; ++v)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 t = tab[(upper ? d0 - half : d0) + j];
-                            x[u][j] = upper ? x[u][j] * t.x + o[j] * t.y : x[u][j] * t.x - o[j] * t.y;
-                        }
+                    for (uint32_t j = 0; j < 8; ++j)
+                        if (v == u) x[v][j] = y[j];
+            }
+        } else if (turn) {
+            const bool upper = d0 >= half, turns = d0 < a.rope.rot_dim;
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                float o[8];
+                if (!a.rope.interleaved) {  // (the other halves are lanes of the same row)
+                    const int from = static_cast<int>(lane) + (turns ? (upper ? -1 : 1) * static_cast<int>(half >> 3) : 0);
+                    uint4 w;
+                    w.x = __shfl_sync(0xFFFFFFFFu, raw[u].x, from), w.y = __shfl_sync(0xFFFFFFFFu, raw[u].y, from);
+                    w.z = __shfl_sync(0xFFFFFFFFu, raw[u].z, from), w.w = __shfl_sync(0xFFFFFFFFu, raw[u].w, from);
+                    unpack8(w, o);
+                }
+                if (!turns) continue;
+                if (a.rope.interleaved) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const float2 t = tab[(d0 + j) >> 1];
+                        const float y = x[u][j] * t.x - x[u][j + 1] * t.y;
+                        x[u][j + 1] = x[u][j + 1] * t.x + x[u][j] * t.y;
+                        x[u][j] = y;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 t = tab[(upper ? d0 - half : d0) + j];
+                        x[u][j] = upper ? x[u][j] * t.x + o[j] * t.y : x[u][j] * t.x - o[j] * t.y;
                     }
                 }
             }
         }
+        if (rb + step * kAtOnce * U < pc.rows) fetch_queries<DC, U>(args, pc, rb + step * kAtOnce * U, step, raw);
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             m[u] = 0.0f;
@@ -441,7 +475,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
                 // (positive, so that a masked score stays -inf; at 1e-30 scores are zero all the same)
                 frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
-                qpos[col] = pc.p0 + static_cast<int32_t>(tok[u]);
+                qpos[col] = pc.p0 + static_cast<int32_t>((base + r) / group);
             }
         }
     }
@@ -640,8 +674,11 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     if (sh.piece[0].rows != 0u) {
         if (warp != 0 && warp != 3) {
             // the first piece's queries: by every warp but the copying ones, which start at once
-            stage_queries<R, DC, NB, G, (8 * NB * DC / 2 + kStagers - 1) / kStagers>(args, sh.piece[0], qbuf, sh.frow[0],
-                                                                                   sh.qpos[0], warp - (warp > 3 ? 2u : 1u), kStagers, nullptr);
+            constexpr int kU = (8 * NB * DC / 2 + kStagers - 1) / kStagers;
+            uint4 raw[kU];
+            fetch_queries<DC, kU>(args, sh.piece[0], (warp - (warp > 3 ? 2u : 1u)) * (2u / DC), kStagers, raw);
+            stage_queries<R, DC, NB, G, kU>(args, sh.piece[0], qbuf, sh.frow[0], sh.qpos[0], warp - (warp > 3 ? 2u : 1u), kStagers,
+                                            nullptr, raw);
             asm volatile("bar.sync 15, %0;" ::"n"(C::kThreads - 64) : "memory");
         }
         // the next piece, or false after the last one
@@ -1213,10 +1250,14 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
                 if (kHelp == 1 && np % 3u != h) continue;
                 const uint32_t qb = np % NQ, rs = np % kQSlots;
+                constexpr int kU = R == 16 ? 4 : 3;
+                const uint32_t at = kHelp == 1 ? 0u : h;
+                uint4 raw[kU];
+                if (np > 0) fetch_queries<DC, kU>(args, *rec, at * (2u / DC), kHelp, raw);
                 if (np >= NQ) bar_wait(&sh.qempty[qb], (np / NQ - 1u) & 1u, gave_up);
                 if (np > 0)
-                    stage_queries<R, DC, NB, G, (R == 16 ? 4 : 2)>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], kHelp == 1 ? 0u : h,
-                                                   kHelp, sh.sines[h]);
+                    stage_queries<R, DC, NB, G, kU>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], at, kHelp,
+                                                    sh.sines[h], raw);
                 __syncwarp();
                 if (lane == 0) {
                     bar_arrive(&sh.qfull[qb]);
