@@ -157,21 +157,66 @@ struct AppendArgs {
     uint32_t* seq_state;  // [2 * max_seqs]: arrivals, flags; zero between calls
     uint32_t row_lanes;   // lanes of a row: the power of two at or above D / 8
     uint32_t team;        // threads of a team: row_lanes or kNT
+    uint32_t key_heads;   // heads of keys that a CTA takes one after the other, sharing their tokens' sines (a team of kNT)
 };
 
 constexpr int kRowsHeld = 4;
+constexpr size_t kSinesMax = 64u * 1024u;
 constexpr uint32_t kFlagNan = 1u, kFlagBounds = 2u;
 
 __device__ __forceinline__ uint32_t item_base(const KvBatchView& b, uint32_t page_shift, uint32_t s) {
     return static_cast<uint32_t>(static_cast<uint64_t>(b.offsets[s]) >> page_shift) + 2u * s;
 }
 
-// 8 elements of a row as they are rounded: turned, NaN as 0; *m the largest finite magnitude
+// 8 elements of a row, turned
 template <typename T, int VEC>
-__device__ __forceinline__ void load_row8(const RopeView& r, const T* p, uint32_t i0, int32_t pos, float* x, float* m,
-                                          bool* bad) {
+__device__ __forceinline__ void load_row8(const RopeView& r, const T* p, uint32_t i0, int32_t pos, float* x) {
 #pragma unroll
     for (int j = 0; j < 8; j += VEC) load_turned<T, VEC>(r, p, i0 + j, pos, x + j);
+}
+// the same with the row's sines at hand
+template <typename T, int VEC>
+__device__ __forceinline__ void load_turned8(const RopeView& r, const T* p, uint32_t i0, const float2* sines, float* x) {
+    const uint32_t half = r.rot_dim >> 1;
+#pragma unroll
+    for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(p + i0 + j, x + j);
+    if (r.interleaved || VEC == 1) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j += 2) {  // (VEC = 1: a pair may cross the end of the turned part only whole)
+            const uint32_t i = i0 + j;
+            if (r.interleaved) {
+                if (i >= r.rot_dim) continue;
+                const float2 t = sines[i >> 1];
+                const float y = x[j] * t.x - x[j + 1] * t.y;
+                x[j + 1] = x[j + 1] * t.x + x[j] * t.y;
+                x[j] = y;
+            } else {
+#pragma unroll
+                for (uint32_t k = j; k < j + 2; ++k) {
+                    if (i0 + k >= r.rot_dim) continue;
+                    const bool upper = i0 + k >= half;
+                    const float2 t = sines[upper ? i0 + k - half : i0 + k];
+                    float o;
+                    load_vec<T, 1>(p + (upper ? i0 + k - half : i0 + k + half), &o);
+                    x[k] = upper ? x[k] * t.x + o * t.y : x[k] * t.x - o * t.y;
+                }
+            }
+        }
+    } else if (i0 < r.rot_dim) {
+        const bool upper = i0 >= half;
+        const uint32_t p0 = upper ? i0 - half : i0;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(p + (upper ? p0 : i0 + half) + j, o + j);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 t = sines[p0 + j];
+            x[j] = upper ? x[j] * t.x + o[j] * t.y : x[j] * t.x - o[j] * t.y;
+        }
+    }
+}
+// NaN as 0; *m the largest finite magnitude
+__device__ __forceinline__ void clean8(float* x, float* m, bool* bad) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float a = fabsf(x[j]);
@@ -192,8 +237,9 @@ __device__ __forceinline__ uint2 round8(const float* x, float mul) {
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kNT, VEC == 1 ? 2 : 3) append_kernel(AppendArgs a) {
     __shared__ float red[kNT / 32];
+    extern __shared__ float2 sines[];  // [new rows of the page][rot_dim / 2], with shared sines
     const uint32_t tid = threadIdx.x;
     // the sequences whose status needs no pages (no new tokens, or numbers that do not fit)
     if (blockIdx.y == 0 && blockIdx.x < a.b.n_seqs && tid == 0) {
@@ -222,41 +268,61 @@ __global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
     const bool id_ok = static_cast<uint32_t>(id) < a.g.n_pages;
 
     const uint32_t teams = kNT / a.team;
-    const uint32_t unit = blockIdx.y * teams + tid / a.team;
     const uint32_t D = a.g.head_dim;
-    const bool live = id_ok && unit < 2u * a.g.n_heads;
-    const bool is_v = unit >= a.g.n_heads;
-    const uint32_t head = is_v ? unit - a.g.n_heads : unit;
     const uint32_t in_team = tid % a.team;
     const uint32_t i0 = (in_team % a.row_lanes) * 8u;
     const uint32_t row_in = in_team / a.row_lanes, rows_at_once = a.team / a.row_lanes;
+    // units of this CTA: one a team, or the keys of key_heads heads one after the other
+    const uint32_t key_ctas = a.key_heads ? (a.g.n_heads + a.key_heads - 1u) / a.key_heads : 0u;
+    const bool shared_sines = blockIdx.y < key_ctas;
+    const uint32_t half = a.rope.rot_dim >> 1;
+    if (shared_sines && id_ok) {
+        for (uint32_t i = tid; i < (slot1 - slot0) * half; i += kNT) {
+            const uint32_t r = i / half, p = i - r * half;
+            float sn, cs;
+            rope_sincos(a.rope, page0 + static_cast<int32_t>(slot0 + r), p, &sn, &cs);
+            sines[i] = make_float2(cs, sn);
+        }
+        __syncthreads();
+    }
+    const uint32_t unit0 = shared_sines ? blockIdx.y * a.key_heads
+                                        : (a.key_heads ? a.g.n_heads + (blockIdx.y - key_ctas) : blockIdx.y * teams + tid / a.team);
+    const uint32_t unit_end = shared_sines ? min(unit0 + a.key_heads, a.g.n_heads) : unit0 + 1u;
+    bool bad = false;
+    for (uint32_t unit = unit0; unit < unit_end; ++unit) {
+    const bool live = id_ok && unit < 2u * a.g.n_heads;
+    const bool is_v = unit >= a.g.n_heads;
+    const uint32_t head = is_v ? unit - a.g.n_heads : unit;
     const KvView& src = is_v ? a.v : a.k;
-    const RopeView rope = is_v ? RopeView{nullptr, 1.0f, 1.0f, 0u, 0u} : a.rope;
+    const RopeView rope = is_v || shared_sines ? RopeView{nullptr, 1.0f, 1.0f, 0u, 0u} : a.rope;
     const T* base = static_cast<const T*>(src.data) + head * src.head_stride;
     const bool lane_on = live && i0 < D;
+    const auto load = [&](uint32_t slot, float* y, float* m) {
+        const int32_t pos = page0 + static_cast<int32_t>(slot);
+        const T* p = base + (q.row0 + (pos - start)) * src.token_stride;
+        if (shared_sines) load_turned8<T, VEC>(a.rope, p, i0, sines + (slot - slot0) * half, y);
+        else load_row8<T, VEC>(rope, p, i0, pos, y);
+        clean8(y, m, &bad);
+    };
 
     float x[kRowsHeld][8];
     float m = 0.0f;
-    bool bad = false;
     if (lane_on) {
 #pragma unroll
         for (int p = 0; p < kRowsHeld; ++p) {
             const uint32_t slot = slot0 + p * rows_at_once + row_in;
-            if (slot < slot1) {
-                const int32_t pos = page0 + static_cast<int32_t>(slot);
-                load_row8<T, VEC>(rope, base + (q.row0 + (pos - start)) * src.token_stride, i0, pos, x[p], &m, &bad);
-            }
+            if (slot < slot1) load(slot, x[p], &m);
         }
         for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
-            const int32_t pos = page0 + static_cast<int32_t>(slot);
             float y[8];
-            load_row8<T, VEC>(rope, base + (q.row0 + (pos - start)) * src.token_stride, i0, pos, y, &m, &bad);
+            load(slot, y, &m);
         }
     }
     // the unit's maximum: over the lanes of a row by shuffles, over the CTA's warps through shared memory
     const uint32_t width = a.team < 32u ? a.team : 32u;
     for (uint32_t o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (a.team > 32u) {
+        __syncthreads();  // (the last unit's have been read)
         if ((tid & 31u) == 0) red[tid >> 5] = m;
         __syncthreads();
 #pragma unroll
@@ -301,9 +367,8 @@ __global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
                 if (slot < slot1) *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(x[p], mul);
             }
             for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
-                const int32_t pos = page0 + static_cast<int32_t>(slot);
-                float y[8];
-                load_row8<T, VEC>(rope, base + (q.row0 + (pos - start)) * src.token_stride, i0, pos, y, &m, &bad);
+                float y[8], again = 0.0f;
+                load(slot, y, &again);
                 *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(y, mul);
             }
         }
@@ -312,6 +377,7 @@ __global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
     // lanes without a unit must not miss the barrier)
     __syncthreads();
     if (in_team == 0 && write_scale) *sp = exp2_int(e);
+    }
     // the sequence's status: the last of its CTAs to arrive writes it
     const bool any_bad = __syncthreads_or(bad ? 1 : 0) != 0;
     if (tid == 0) {
@@ -321,8 +387,11 @@ __global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
         bool last = true;
         if (ctas > 1u) {
             uint32_t* st = a.seq_state + 2u * seq;
-            if (flag) atomicOr(st + 1, flag);
-            __threadfence();
+            // (only a raised flag has to be seen before the arrival; the pages themselves need no order here)
+            if (flag) {
+                atomicOr(st + 1, flag);
+                __threadfence();
+            }
             last = atomicAdd(st, 1u) == ctas - 1u;
             if (last) {
                 __threadfence();
@@ -337,19 +406,20 @@ __global__ void __launch_bounds__(kNT) append_kernel(AppendArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// sixi_kv_read: bytes times scale, 8 elements a thread; a CTA takes `per` consecutive tokens.
+// sixi_kv_read: bytes times scale, 8 elements a lane at a time; a warp takes a token, so that its page is looked up once,
+// and keeps four loads in flight. Bound by memory.
 
 struct ReadArgs {
     KvGeom g;
     KvBatchView b;
     KvView k, v;
     int32_t* status;
-    uint32_t per;
+    uint32_t per;  // tokens of a CTA
 };
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
     if (blockIdx.y == 0) {  // statuses, spread over the CTAs
         for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
             const KvSeq q = kv_seq(a.b, a.g.page_shift, s);
@@ -365,6 +435,7 @@ __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
         }
     }
     const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * a.per;
+    const uint64_t t1 = t0 + a.per < a.b.n_tokens ? t0 + a.per : a.b.n_tokens;
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += kNT) {
         const uint32_t s = s0 + tid;
@@ -378,10 +449,7 @@ __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
     const uint32_t D = a.g.head_dim, row_chunks = D / 8u, chunks = a.g.n_heads * row_chunks;
     uint32_t seq = before - 1;
     KvSeq q = kv_seq(a.b, a.g.page_shift, seq);
-    const uint64_t t1 = t0 + a.per < a.b.n_tokens ? t0 + a.per : a.b.n_tokens;
-    for (uint64_t i = tid; i < (t1 - t0) * chunks; i += kNT) {
-        const uint64_t tok = t0 + i / chunks;
-        const uint32_t c = static_cast<uint32_t>(i % chunks);
+    for (uint64_t tok = t0 + (tid >> 5); tok < t1; tok += kNT / 32) {
         while (seq + 1 < a.b.n_seqs && a.b.offsets[seq + 1] <= static_cast<int64_t>(tok)) {
             ++seq;
             q = kv_seq(a.b, a.g.page_shift, seq);
@@ -390,22 +458,41 @@ __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
         if (!q.ok || q.len < q.n || in < 0 || in >= q.n) continue;
         const uint32_t pos = static_cast<uint32_t>(q.len - q.n + static_cast<int32_t>(in));
         const int32_t id = a.b.page_table[seq * a.b.table_stride + (pos >> a.g.page_shift)];
-        const uint32_t head = c / row_chunks, i0 = (c - head * row_chunks) * 8u;
-        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (static_cast<uint32_t>(id) < a.g.n_pages) {
-            const uint64_t ph = static_cast<uint64_t>(id) * a.g.n_heads + head;
-            const float s = scales[ph];
-            const uint2 o = *reinterpret_cast<const uint2*>(
-                pages + (ph * a.g.page_size + (pos & (a.g.page_size - 1u))) * D + i0);
-            float2 f;
-            f = e4m3x2_to_float2(o.x), y[0] = f.x * s, y[1] = f.y * s;
-            f = e4m3x2_to_float2(o.x >> 16), y[2] = f.x * s, y[3] = f.y * s;
-            f = e4m3x2_to_float2(o.y), y[4] = f.x * s, y[5] = f.y * s;
-            f = e4m3x2_to_float2(o.y >> 16), y[6] = f.x * s, y[7] = f.y * s;
-        }
-        T* p = static_cast<T*>(dst.data) + tok * dst.token_stride + head * dst.head_stride + i0;
+        const bool good = static_cast<uint32_t>(id) < a.g.n_pages;
+        const uint64_t ph0 = static_cast<uint64_t>(good ? id : 0) * a.g.n_heads;
+        const uint32_t slot = pos & (a.g.page_size - 1u);
+        T* out = static_cast<T*>(dst.data) + tok * dst.token_stride;
+        constexpr int kUnroll = 4;
+        for (uint32_t c0 = lane; c0 < chunks; c0 += 32u * kUnroll) {
+            uint2 o[kUnroll];
+            float f[kUnroll];
+            uint32_t head[kUnroll], i0[kUnroll];
 #pragma unroll
-        for (int j = 0; j < 8; j += VEC) store_vec<T, VEC>(p + j, y + j);
+            for (int u = 0; u < kUnroll; ++u) {
+                const uint32_t c = min(c0 + 32u * u, chunks - 1u);
+                head[u] = c / row_chunks;
+                i0[u] = (c - head[u] * row_chunks) * 8u;
+                o[u] = make_uint2(0u, 0u);
+                f[u] = 0.0f;
+                if (good) {
+                    o[u] = *reinterpret_cast<const uint2*>(pages + ((ph0 + head[u]) * a.g.page_size + slot) * D + i0[u]);
+                    f[u] = scales[ph0 + head[u]];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (c0 + 32u * u >= chunks) continue;
+                float y[8];
+                float2 v;
+                v = e4m3x2_to_float2(o[u].x), y[0] = v.x * f[u], y[1] = v.y * f[u];
+                v = e4m3x2_to_float2(o[u].x >> 16), y[2] = v.x * f[u], y[3] = v.y * f[u];
+                v = e4m3x2_to_float2(o[u].y), y[4] = v.x * f[u], y[5] = v.y * f[u];
+                v = e4m3x2_to_float2(o[u].y >> 16), y[6] = v.x * f[u], y[7] = v.y * f[u];
+                T* p = out + head[u] * dst.head_stride + i0[u];
+#pragma unroll
+                for (int j = 0; j < 8; j += VEC) store_vec<T, VEC>(p + j, y + j);
+            }
+        }
     }
 }
 
@@ -428,25 +515,36 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
     const uint32_t rows = max_new < g.page_size ? max_new : g.page_size;
     a.team = rows <= kRowsHeld ? a.row_lanes : kNT;
     const uint32_t teams = kNT / a.team;
-    const dim3 grid(b.n_tokens / g.page_size + 2u * b.n_seqs, (2u * g.n_heads + teams - 1) / teams);
+    // The sines of a page's tokens are the same for every head: with a team of the whole CTA, a CTA works them out once
+    // (into shared memory) for four heads. At 18,800 tokens of 8 heads of 128 the rotation then costs 8 us, against
+    // 24 with every head for itself.
+    const size_t table = rope.turns == nullptr ? 0 : static_cast<size_t>(rows) * (rope.rot_dim / 2) * sizeof(float2);
+    a.key_heads = a.team == kNT && table > 0 && rows == g.page_size && table <= kSinesMax ? 4u : 0u;
+    const uint32_t units = a.key_heads ? (g.n_heads + a.key_heads - 1) / a.key_heads + g.n_heads
+                                       : (2u * g.n_heads + teams - 1) / teams;
+    const dim3 grid(b.n_tokens / g.page_size + 2u * b.n_seqs, units);
+    const size_t smem = a.key_heads ? table : 0;
     const bool vec = view_aligned(k, g.n_heads, b.n_tokens) && view_aligned(v, g.n_heads, b.n_tokens) && rope_by_8(rope);
-    if (k->dtype == SIXI_SMP_BF16) {
-        if (vec) append_kernel<__nv_bfloat16, 8><<<grid, kNT, 0, stream>>>(a);
-        else append_kernel<__nv_bfloat16, 1><<<grid, kNT, 0, stream>>>(a);
-    } else {
-        if (vec) append_kernel<float, 8><<<grid, kNT, 0, stream>>>(a);
-        else append_kernel<float, 1><<<grid, kNT, 0, stream>>>(a);
-    }
-    return cudaGetLastError();
+    const auto go = [&](auto kernel) {
+        if (smem > 48u * 1024u) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (e != cudaSuccess) return e;
+        }
+        kernel<<<grid, kNT, smem, stream>>>(a);
+        return cudaGetLastError();
+    };
+    if (k->dtype == SIXI_SMP_BF16)
+        return vec ? go(append_kernel<__nv_bfloat16, 8>) : go(append_kernel<__nv_bfloat16, 1>);
+    return vec ? go(append_kernel<float, 8>) : go(append_kernel<float, 1>);
 }
 
 cudaError_t launch_kv_read(const KvGeom& g, const KvBatchView& b, const sixi_kv_tensor* k, const sixi_kv_tensor* v,
                            int32_t* status, cudaStream_t stream) {
     ReadArgs a;
     a.g = g, a.b = b, a.k = view_of(k), a.v = view_of(v), a.status = status;
-    // tokens per CTA: about eight 8-element chunks a thread
-    const uint32_t chunks = g.n_heads * (g.head_dim / 8);
-    a.per = chunks >= 8 * kNT ? 1 : (8 * kNT) / chunks;
+    // a token a warp while that does not fill the GPU (148 SMs of 8 such CTAs), up to four
+    a.per = kNT / 32;
+    while (a.per < 4 * (kNT / 32) && b.n_tokens / a.per > 148u * 16u) a.per *= 2;
     const uint32_t blocks = (b.n_tokens + a.per - 1) / a.per;
     const dim3 grid(blocks ? blocks : 1, 2);
     const bool vec = view_aligned(k, g.n_heads, b.n_tokens) && view_aligned(v, g.n_heads, b.n_tokens);

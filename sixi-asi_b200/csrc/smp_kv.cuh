@@ -465,6 +465,107 @@ inline bool rope_by_8(const RopeView& r) {
 constexpr uint32_t kAttnMaxCtas = 512;
 inline uint64_t part_floats(uint32_t rows, uint32_t head_dim) { return static_cast<uint64_t>(rows) * (head_dim + 2u); }
 
+// ---------------------------------------------------------------------------------------------
+// joining the pieces of a unit
+
+__device__ __forceinline__ float kv_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Eight warps (w: 0 to 7) join a unit's n pieces in CTA order: piece 0 is its CTA's last result (first), the others are
+// their CTAs' first ones (rest + 2 c results on). Rows of `rt`-row results; row r goes to query token
+// (row_base + r) / group of row0 on. DC: 128-element chunks of a head.
+template <typename T, int DC>
+__device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first, const float* rest, uint32_t n, uint32_t rows,
+                                          uint32_t row_base, int64_t row0, uint32_t head, uint32_t w) {
+    constexpr int kAhead = DC == 1 ? 4 : 2;  // pieces whose loads are in flight
+    const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
+    const auto piece_of = [&](uint32_t c) { return c == 0 ? first : rest + 2ull * c * a.part_stride; };
+    // a warp a row, four elements a lane, two rows at a time; a lane holds the factor of a piece (of every 32nd)
+    for (uint32_t r0 = w; r0 < rows; r0 += 16u) {
+        const uint32_t row[2] = {r0, min(r0 + 8u, rows - 1u)};
+        float m[2], l[2], f[2], norm[2];
+        float4 o[2][DC], v[2][DC][kAhead];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            m[u] = kNegInf, l[u] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        // (the first pieces' sums are on their way before the factors are known)
+        const auto fetch = [&](uint32_t c) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < DC; ++k)
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i)
+                        if (k * 128u + lane * 4u < D)
+                            v[u][k][i] = __ldcg(reinterpret_cast<const float4*>(piece_of(min(c + i, n - 1u)) + row[u] * D +
+                                                                                k * 128u + lane * 4u));
+        };
+        fetch(0);
+        for (uint32_t c = lane; c < n; c += 32u)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __ldcg(piece_of(c) + a.shape.rt * D + row[u]));
+#pragma unroll
+        for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o2));
+        for (uint32_t c0l = 0; c0l < n; c0l += 32u) {
+            const uint32_t c = c0l + lane;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f[u] = 0.0f;
+                if (c < n) {
+                    const float* p = piece_of(c) + a.shape.rt * D + row[u];
+                    const float mc = __ldcg(p);
+                    f[u] = mc == m[u] ? 1.0f : kv_ex2(mc - m[u]);
+                    l[u] += __ldcg(p + a.shape.rt) * f[u];
+                }
+            }
+            for (uint32_t i0 = 0; i0 < 32u && c0l + i0 < n; i0 += kAhead) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float g = __shfl_sync(0xFFFFFFFFu, f[u], i0 + i);  // (0 past the last piece)
+#pragma unroll
+                        for (int k = 0; k < DC; ++k) {
+                            if (g == 0.0f) continue;
+                            o[u][k].x = fmaf(v[u][k][i].x, g, o[u][k].x), o[u][k].y = fmaf(v[u][k][i].y, g, o[u][k].y);
+                            o[u][k].z = fmaf(v[u][k][i].z, g, o[u][k].z), o[u][k].w = fmaf(v[u][k][i].w, g, o[u][k].w);
+                        }
+                    }
+                if (c0l + i0 + kAhead < n) fetch(c0l + i0 + kAhead);
+            }
+        }
+#pragma unroll
+        for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], o2);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (u == 1 && r0 + 8u >= rows) continue;
+            norm[u] = l[u] == 0.0f ? 0.0f : 1.0f / l[u];
+            const uint32_t rr = row_base + row[u], tok = rr / a.shape.group;
+            const uint32_t hq = head * a.shape.group + rr - tok * a.shape.group;
+            if (a.lse && lane == 0)
+                a.lse[(row0 + tok) * (a.shape.n_heads * a.shape.group) + hq] = (m[u] + log2f(l[u])) * 0.6931471805599453f;
+            T* p = static_cast<T*>(a.out.data) + (row0 + tok) * a.out.token_stride + hq * a.out.head_stride;
+#pragma unroll
+            for (int k = 0; k < DC; ++k)
+                if (k * 128u + lane * 4u < D) {
+                    const float y[4] = {o[u][k].x * norm[u], o[u][k].y * norm[u], o[u][k].z * norm[u], o[u][k].w * norm[u]};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) store_vec<T, 1>(p + k * 128u + lane * 4u + i, y + i);
+                }
+        }
+    }
+}
+
 cudaError_t launch_rope_apply(const RopeView& r, const sixi_kv_tensor* x, const int32_t* positions, uint32_t n_tokens,
                               uint32_t head_dim, const sixi_kv_tensor* out, cudaStream_t stream);
 cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_kv_tensor* k, const sixi_kv_tensor* v,

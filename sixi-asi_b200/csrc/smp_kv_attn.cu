@@ -17,6 +17,7 @@ constexpr int kNT = 256;
 constexpr int kRt = 16;         // rows of a row tile
 constexpr int kTileShift = 6;   // 64 tokens
 constexpr int kT = 1 << kTileShift;
+constexpr uint32_t kWindow = 32;  // tiles whose page ids are kept
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -38,47 +39,57 @@ struct Smem {
     float* red;     // [4096] sums over token groups
 };
 
+// The page ids of tiles [tile, tile + kWindow) of a piece; -1 for pages behind the sequence or before lo's.
+__device__ __forceinline__ void load_ids(const AttnArgs& a, const Piece& pc, int32_t lo, int32_t tile, int32_t* ids) {
+    const uint32_t per = max(kT >> a.g.page_shift, 1u), shift = a.g.page_shift;
+    for (uint32_t i = threadIdx.x; i < kWindow * per; i += kNT) {
+        const int32_t pos = (tile << kTileShift) + static_cast<int32_t>(per > 1u ? i << shift : i << kTileShift);
+        const uint32_t pg = static_cast<uint32_t>(pos) >> shift;
+        const bool on = pos < pc.plan.len && (lo <= 0 || pg >= static_cast<uint32_t>(lo) >> shift);
+        ids[i] = on ? a.b.page_table[pc.seq * a.b.table_stride + pg] : -1;
+    }
+}
+
 // One tile's bytes and scales into stage st; tokens outside the sequence, before the window of the unit's
 // first row (lo) or in a bad page are zero.
 __device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, const Piece& pc, int32_t lo, int32_t tile,
-                                          uint32_t st) {
-    const uint32_t D = a.g.head_dim, row = D + 16u, per = D / 16u;
+                                          uint32_t st, const int32_t* ids) {
+    const uint32_t D = a.g.head_dim, row = D + 16u, per = D / 16u, shift = a.g.page_shift;
     uint8_t* dst = sm.kv + static_cast<uint64_t>(st) * 2u * kT * row;
-    const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
+    const uint32_t ids_per = max(kT >> shift, 1u);
+    const auto place = [&](uint32_t t, uint64_t* ph) {  // of the tile's token t: its page and head, if it is read
+        const int32_t pos = tile * kT + static_cast<int32_t>(t);
+        const int32_t id = ids[ids_per > 1u ? t >> shift : 0u];
+        *ph = static_cast<uint64_t>(static_cast<uint32_t>(id)) * a.g.n_heads + pc.head;
+        return pos < pc.plan.len && pos >= lo && static_cast<uint32_t>(id) < a.g.n_pages;
+    };
     for (uint32_t i = threadIdx.x; i < 2u * kT * per; i += kNT) {
         const uint32_t kv = i / (kT * per), j = i - kv * (kT * per);
         const uint32_t t = j / per, c = j - t * per;
-        const int32_t pos = tile * kT + static_cast<int32_t>(t);
-        bool on = pos < pc.plan.len && pos >= lo;
-        uint64_t off = 0;
-        if (on) {
-            const int32_t id = table[static_cast<uint32_t>(pos) >> a.g.page_shift];
-            on = static_cast<uint32_t>(id) < a.g.n_pages;
-            if (on)
-                off = ((static_cast<uint64_t>(id) * a.g.n_heads + pc.head) * a.g.page_size +
-                       (static_cast<uint32_t>(pos) & (a.g.page_size - 1u))) * D + c * 16u;
-        }
+        uint64_t ph;
+        const bool on = place(t, &ph);
+        const uint64_t off =
+            on ? (ph * a.g.page_size + (static_cast<uint32_t>(tile * kT + t) & (a.g.page_size - 1u))) * D + c * 16u : 0u;
         cp_async16(dst + (kv * kT + t) * row + c * 16u, (kv ? a.g.v_pages : a.g.k_pages) + off, on);
     }
     if (threadIdx.x < 2u * kT) {
         const uint32_t kv = threadIdx.x >> kTileShift, t = threadIdx.x & (kT - 1u);
-        const int32_t pos = tile * kT + static_cast<int32_t>(t);
-        float f = 0.0f;
-        if (pos < pc.plan.len && pos >= lo) {
-            const int32_t id = table[static_cast<uint32_t>(pos) >> a.g.page_shift];
-            if (static_cast<uint32_t>(id) < a.g.n_pages)
-                f = (kv ? a.g.v_scales : a.g.k_scales)[static_cast<uint64_t>(id) * a.g.n_heads + pc.head];
-        }
-        sm.tok[(st * 2u + kv) * kT + t] = f;
+        uint64_t ph;
+        const bool on = place(t, &ph);
+        const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(sm.tok + (st * 2u + kv) * kT + t)), n = on ? 4u : 0u;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"((kv ? a.g.v_scales : a.g.k_scales) + (on ? ph : 0u)),
+                     "r"(n)
+                     : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ unsigned long long scratch[kNT / 32 + 2];
     __shared__ uint32_t last_flag;
+    __shared__ int32_t ids[kWindow * 4];
     const uint32_t tid = threadIdx.x, D = a.g.head_dim, row = D + 16u;
     Smem sm;
     {
@@ -112,7 +123,10 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
         const int32_t lo = a.shape.window ? pc.plan.p0 + static_cast<int32_t>(r_base / a.shape.group) -
                                                 static_cast<int32_t>(a.shape.window) + 1
                                           : 0;
-        load_tile(a, sm, pc, lo, pc.t0, 0);
+        const uint32_t ids_per = max(kT >> a.g.page_shift, 1u);
+        load_ids(a, pc, lo, pc.t0, ids);
+        __syncthreads();
+        load_tile(a, sm, pc, lo, pc.t0, 0, ids);
         // queries, turned and rounded to their type, then scaled; a NaN or Inf makes the row NaN
         for (uint32_t i = tid; i < kRt * D; i += kNT) {
             const uint32_t r = i / D, d = i - r * D;
@@ -135,7 +149,12 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
         for (int32_t tile = pc.t0; tile < pc.t1; ++tile) {
             const uint32_t st = static_cast<uint32_t>(tile - pc.t0) & 1u;
             if (tile + 1 < pc.t1) {
-                load_tile(a, sm, pc, lo, tile + 1, st ^ 1u);
+                const uint32_t at = static_cast<uint32_t>(tile + 1 - pc.t0) % kWindow;
+                if (at == 0) {
+                    load_ids(a, pc, lo, tile + 1, ids);
+                    __syncthreads();
+                }
+                load_tile(a, sm, pc, lo, tile + 1, st ^ 1u, ids + at * ids_per);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -287,28 +306,9 @@ __global__ void __launch_bounds__(kNT) attend_f32_kernel(AttnArgs a) {
         __syncthreads();
         if (!last_flag) continue;
         __threadfence();
-        // the last CTA of the unit joins the pieces in CTA order
-        for (uint32_t i = tid; i < pc.rows * D; i += kNT) {
-            const uint32_t r = i / D, d = i - r * D;
-            float M = kNegInf, l = 0.0f, o = 0.0f;
-            for (uint32_t c = c0; c <= c1; ++c)
-                M = fmaxf(M, __ldcg(a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride + kRt * D + r));
-            for (uint32_t c = c0; c <= c1; ++c) {
-                const float* p = a.part + (2ull * c + (c == c0 ? 1u : 0u)) * a.part_stride;
-                const float m = __ldcg(p + kRt * D + r);
-                const float f = m == M ? 1.0f : exp2f(m - M);
-                l += __ldcg(p + kRt * (D + 1u) + r) * f;
-                o += __ldcg(p + r * D + d) * f;
-            }
-            const uint32_t rr = r_base + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
-            T* p = static_cast<T*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
-                   (pc.head * a.shape.group + g) * a.out.head_stride + d;
-            const float y = l == 0.0f ? 0.0f : o / l;
-            store_vec<T, 1>(p, &y);
-            if (d == 0 && a.lse)
-                a.lse[(pc.plan.row0 + tok) * (a.shape.n_heads * a.shape.group) + pc.head * a.shape.group + g] =
-                    (M + log2f(l)) * kLn2;
-        }
+        // the last CTA of the unit joins the pieces
+        join_rows<T, 2>(a, a.part + (2ull * c0 + 1u) * a.part_stride, a.part + 2ull * c0 * a.part_stride, c1 - c0 + 1u,
+                        pc.rows, r_base, pc.plan.row0, pc.head, tid >> 5);
     }
 }
 

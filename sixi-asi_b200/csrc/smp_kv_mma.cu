@@ -487,7 +487,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
 // joining.
 template <int DC, typename Sh>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, uint32_t w) {
-    const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
+    const uint32_t lane = threadIdx.x & 31u;
     __threadfence();
     asm volatile("bar.sync 14, 256;" ::: "memory");
     if (w == 0) {
@@ -512,91 +512,9 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, uint32_t 
         const PieceRec& pc = sh.split[mine];
         const uint32_t c0 = place_owner(pc.start, sh.total, sh.ctas);
         const uint32_t n = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, sh.total, sh.ctas) - c0 + 1u;
-        const uint32_t rows = pc.rows;
         const float* first = a.part + (2ull * c0 + 1u) * a.part_stride;       // the piece of c0 is its CTA's last
         const float* rest = a.part + (2ull * c0) * a.part_stride;             // the others' are their CTA's first
-        const auto piece_of = [&](uint32_t c) { return c == 0 ? first : rest + 2ull * c * a.part_stride; };
-        // a warp a row, four elements a lane, two rows at a time; a lane holds the factor of a piece (of every 32nd)
-        for (uint32_t r0 = w; r0 < rows; r0 += 16u) {
-            const uint32_t row[2] = {r0, min(r0 + 8u, rows - 1u)};
-            float m[2], l[2], f[2], norm[2];
-            float4 o[2][DC], v[2][DC][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                m[u] = kNegInf, l[u] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-            // (the first pieces' sums are on their way before the factors are known)
-            const auto fetch = [&](uint32_t c) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int k = 0; k < DC; ++k)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (k * 128u + lane * 4u < D)
-                                v[u][k][i] = __ldcg(reinterpret_cast<const float4*>(piece_of(min(c + i, n - 1u)) + row[u] * D +
-                                                                                    k * 128u + lane * 4u));
-            };
-            fetch(0);
-            for (uint32_t c = lane; c < n; c += 32u)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __ldcg(piece_of(c) + a.shape.rt * D + row[u]));
-#pragma unroll
-            for (int o2 = 16; o2 > 0; o2 >>= 1)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o2));
-            for (uint32_t c0l = 0; c0l < n; c0l += 32u) {
-                const uint32_t c = c0l + lane;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    f[u] = 0.0f;
-                    if (c < n) {
-                        const float* p = piece_of(c) + a.shape.rt * D + row[u];
-                        const float mc = __ldcg(p);
-                        f[u] = mc == m[u] ? 1.0f : ex2(mc - m[u]);
-                        l[u] += __ldcg(p + a.shape.rt) * f[u];
-                    }
-                }
-                for (uint32_t i0 = 0; i0 < 32u && c0l + i0 < n; i0 += 4u) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const float g = __shfl_sync(0xFFFFFFFFu, f[u], i0 + i);  // (0 past the last piece)
-#pragma unroll
-                            for (int k = 0; k < DC; ++k) {
-                                if (g == 0.0f) continue;
-                                o[u][k].x = fmaf(v[u][k][i].x, g, o[u][k].x), o[u][k].y = fmaf(v[u][k][i].y, g, o[u][k].y);
-                                o[u][k].z = fmaf(v[u][k][i].z, g, o[u][k].z), o[u][k].w = fmaf(v[u][k][i].w, g, o[u][k].w);
-                            }
-                        }
-                    if (c0l + i0 + 4u < n) fetch(c0l + i0 + 4u);
-                }
-            }
-#pragma unroll
-            for (int o2 = 16; o2 > 0; o2 >>= 1)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], o2);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u == 1 && r0 + 8u >= rows) continue;
-                norm[u] = l[u] == 0.0f ? 0.0f : 1.0f / l[u];
-                const uint32_t rr = pc.row_tile * a.shape.rt + row[u], tok = rr / a.shape.group;
-                const uint32_t hq = pc.head * a.shape.group + rr - tok * a.shape.group;
-                if (a.lse && lane == 0)
-                    a.lse[(pc.row0 + tok) * (a.shape.n_heads * a.shape.group) + hq] = (m[u] + log2f(l[u])) * kLn2;
-                __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out.data) + (pc.row0 + tok) * a.out.token_stride + hq * a.out.head_stride;
-#pragma unroll
-                for (int k = 0; k < DC; ++k)
-                    if (k * 128u + lane * 4u < D) {
-                        __nv_bfloat16* d = p + k * 128u + lane * 4u;
-                        d[0] = __float2bfloat16_rn(o[u][k].x * norm[u]), d[1] = __float2bfloat16_rn(o[u][k].y * norm[u]);
-                        d[2] = __float2bfloat16_rn(o[u][k].z * norm[u]), d[3] = __float2bfloat16_rn(o[u][k].w * norm[u]);
-                    }
-            }
-        }
+        join_rows<__nv_bfloat16, DC>(a, first, rest, n, pc.rows, pc.row_tile * a.shape.rt, pc.row0, pc.head, w);
     }
 }
 
