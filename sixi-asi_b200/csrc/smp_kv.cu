@@ -157,7 +157,7 @@ struct AppendArgs {
     uint32_t* seq_state;  // [2 * max_seqs]: arrivals, flags; zero between calls
     uint32_t row_lanes;   // lanes of a row: the power of two at or above D / 8
     uint32_t team;        // threads of a team: row_lanes or kNT
-    uint32_t key_heads;   // heads of keys that a CTA takes one after the other, sharing their tokens' sines (a team of kNT)
+    uint32_t heads;       // with a team of kNT: heads of keys, or of values, that a CTA takes one after the other
 };
 
 constexpr int kRowsHeld = 4;
@@ -174,33 +174,29 @@ __device__ __forceinline__ void load_row8(const RopeView& r, const T* p, uint32_
 #pragma unroll
     for (int j = 0; j < 8; j += VEC) load_turned<T, VEC>(r, p, i0 + j, pos, x + j);
 }
-// the same with the row's sines at hand
+// 8 elements of a row, as loaded to x, turned with the row's sines at hand (the other halves come from p again)
 template <typename T, int VEC>
-__device__ __forceinline__ void load_turned8(const RopeView& r, const T* p, uint32_t i0, const float2* sines, float* x) {
+__device__ __forceinline__ void turn8(const RopeView& r, const T* p, uint32_t i0, const float2* sines, float* x) {
     const uint32_t half = r.rot_dim >> 1;
+    if (r.interleaved) {
 #pragma unroll
-    for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(p + i0 + j, x + j);
-    if (r.interleaved || VEC == 1) {
+        for (uint32_t j = 0; j < 8; j += 2) {
+            if (i0 + j >= r.rot_dim) continue;
+            const float2 t = sines[(i0 + j) >> 1];
+            const float y = x[j] * t.x - x[j + 1] * t.y;
+            x[j + 1] = x[j + 1] * t.x + x[j] * t.y;
+            x[j] = y;
+        }
+    } else if constexpr (VEC == 1) {
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j += 2) {  // (VEC = 1: a pair may cross the end of the turned part only whole)
+        for (uint32_t j = 0; j < 8; ++j) {
             const uint32_t i = i0 + j;
-            if (r.interleaved) {
-                if (i >= r.rot_dim) continue;
-                const float2 t = sines[i >> 1];
-                const float y = x[j] * t.x - x[j + 1] * t.y;
-                x[j + 1] = x[j + 1] * t.x + x[j] * t.y;
-                x[j] = y;
-            } else {
-#pragma unroll
-                for (uint32_t k = j; k < j + 2; ++k) {
-                    if (i0 + k >= r.rot_dim) continue;
-                    const bool upper = i0 + k >= half;
-                    const float2 t = sines[upper ? i0 + k - half : i0 + k];
-                    float o;
-                    load_vec<T, 1>(p + (upper ? i0 + k - half : i0 + k + half), &o);
-                    x[k] = upper ? x[k] * t.x + o * t.y : x[k] * t.x - o * t.y;
-                }
-            }
+            if (i >= r.rot_dim) continue;
+            const bool upper = i >= half;
+            const float2 t = sines[upper ? i - half : i];
+            float o;
+            load_vec<T, 1>(p + (upper ? i - half : i + half), &o);
+            x[j] = upper ? x[j] * t.x + o * t.y : x[j] * t.x - o * t.y;
         }
     } else if (i0 < r.rot_dim) {
         const bool upper = i0 >= half;
@@ -236,8 +232,12 @@ __device__ __forceinline__ uint2 round8(const float* x, float mul) {
     return o;
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNT, VEC == 1 ? 2 : 3) append_kernel(AppendArgs a) {
+// MODE 0: keys as they are; 1: turned, a CTA's heads sharing their tokens' sines; 2: turned, every lane its own
+enum { kAsIs = 0, kSharedSines = 1, kOwnSines = 2 };
+
+template <typename T, int VEC, int MODE>
+__global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == kSharedSines && VEC > 1 ? 3 : 2))
+    append_kernel(AppendArgs a) {
     __shared__ float red[kNT / 32];
     extern __shared__ float2 sines[];  // [new rows of the page][rot_dim / 2], with shared sines
     const uint32_t tid = threadIdx.x;
@@ -272,11 +272,10 @@ __global__ void __launch_bounds__(kNT, VEC == 1 ? 2 : 3) append_kernel(AppendArg
     const uint32_t in_team = tid % a.team;
     const uint32_t i0 = (in_team % a.row_lanes) * 8u;
     const uint32_t row_in = in_team / a.row_lanes, rows_at_once = a.team / a.row_lanes;
-    // units of this CTA: one a team, or the keys of key_heads heads one after the other
-    const uint32_t key_ctas = a.key_heads ? (a.g.n_heads + a.key_heads - 1u) / a.key_heads : 0u;
-    const bool shared_sines = blockIdx.y < key_ctas;
+    // units of this CTA: one a team, or those of some heads one after the other
+    const uint32_t groups = a.heads ? (a.g.n_heads + a.heads - 1u) / a.heads : 0u;  // of keys, then of values
     const uint32_t half = a.rope.rot_dim >> 1;
-    if (shared_sines && id_ok) {
+    if (MODE == kSharedSines && blockIdx.y < groups && id_ok) {
         for (uint32_t i = tid; i < (slot1 - slot0) * half; i += kNT) {
             const uint32_t r = i / half, p = i - r * half;
             float sn, cs;
@@ -285,33 +284,53 @@ __global__ void __launch_bounds__(kNT, VEC == 1 ? 2 : 3) append_kernel(AppendArg
         }
         __syncthreads();
     }
-    const uint32_t unit0 = shared_sines ? blockIdx.y * a.key_heads
-                                        : (a.key_heads ? a.g.n_heads + (blockIdx.y - key_ctas) : blockIdx.y * teams + tid / a.team);
-    const uint32_t unit_end = shared_sines ? min(unit0 + a.key_heads, a.g.n_heads) : unit0 + 1u;
+    uint32_t unit0 = blockIdx.y * teams + tid / a.team, unit_end = unit0 + 1u;
+    if (a.heads) {
+        const bool values = blockIdx.y >= groups;
+        const uint32_t h0 = (blockIdx.y - (values ? groups : 0u)) * a.heads;
+        unit0 = (values ? a.g.n_heads : 0u) + h0;
+        unit_end = (values ? a.g.n_heads : 0u) + min(h0 + a.heads, a.g.n_heads);
+    }
     bool bad = false;
     for (uint32_t unit = unit0; unit < unit_end; ++unit) {
     const bool live = id_ok && unit < 2u * a.g.n_heads;
     const bool is_v = unit >= a.g.n_heads;
     const uint32_t head = is_v ? unit - a.g.n_heads : unit;
     const KvView& src = is_v ? a.v : a.k;
-    const RopeView rope = is_v || shared_sines ? RopeView{nullptr, 1.0f, 1.0f, 0u, 0u} : a.rope;
+    const bool turn = MODE != kAsIs && !is_v;
     const T* base = static_cast<const T*>(src.data) + head * src.head_stride;
     const bool lane_on = live && i0 < D;
-    const auto load = [&](uint32_t slot, float* y, float* m) {
-        const int32_t pos = page0 + static_cast<int32_t>(slot);
-        const T* p = base + (q.row0 + (pos - start)) * src.token_stride;
-        if (shared_sines) load_turned8<T, VEC>(a.rope, p, i0, sines + (slot - slot0) * half, y);
-        else load_row8<T, VEC>(rope, p, i0, pos, y);
-        clean8(y, m, &bad);
+    const auto row_of = [&](uint32_t slot) {
+        return base + (q.row0 + (page0 + static_cast<int32_t>(slot) - start)) * src.token_stride;
+    };
+    const auto turn_row = [&](uint32_t slot, float* y) {  // y: the row's elements as loaded
+        if constexpr (MODE == kSharedSines) turn8<T, VEC>(a.rope, row_of(slot), i0, sines + (slot - slot0) * half, y);
+        if constexpr (MODE == kOwnSines) load_row8<T, VEC>(a.rope, row_of(slot), i0, page0 + static_cast<int32_t>(slot), y);
+    };
+    const auto load = [&](uint32_t slot, float* y, float* mm) {
+#pragma unroll
+        for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(row_of(slot) + i0 + j, y + j);
+        if (turn) turn_row(slot, y);
+        clean8(y, mm, &bad);
     };
 
     float x[kRowsHeld][8];
     float m = 0.0f;
     if (lane_on) {
+        // the held rows' elements are asked for together, then worked on
+#pragma unroll
+        for (int p = 0; p < kRowsHeld; ++p) {
+            const uint32_t slot = min(slot0 + p * rows_at_once + row_in, slot1 - 1u);
+            const T* r = row_of(slot);
+#pragma unroll
+            for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(r + i0 + j, x[p] + j);
+        }
 #pragma unroll
         for (int p = 0; p < kRowsHeld; ++p) {
             const uint32_t slot = slot0 + p * rows_at_once + row_in;
-            if (slot < slot1) load(slot, x[p], &m);
+            if (slot >= slot1) continue;
+            if (turn) turn_row(slot, x[p]);
+            clean8(x[p], &m, &bad);
         }
         for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
             float y[8];
@@ -515,15 +534,20 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
     const uint32_t rows = max_new < g.page_size ? max_new : g.page_size;
     a.team = rows <= kRowsHeld ? a.row_lanes : kNT;
     const uint32_t teams = kNT / a.team;
-    // The sines of a page's tokens are the same for every head: with a team of the whole CTA, a CTA works them out once
-    // (into shared memory) for four heads. At 18,800 tokens of 8 heads of 128 the rotation then costs 8 us, against
-    // 24 with every head for itself.
-    const size_t table = rope.turns == nullptr ? 0 : static_cast<size_t>(rows) * (rope.rot_dim / 2) * sizeof(float2);
-    a.key_heads = a.team == kNT && table > 0 && rows == g.page_size && table <= kSinesMax ? 4u : 0u;
-    const uint32_t units = a.key_heads ? (g.n_heads + a.key_heads - 1) / a.key_heads + g.n_heads
-                                       : (2u * g.n_heads + teams - 1) / teams;
-    const dim3 grid(b.n_tokens / g.page_size + 2u * b.n_seqs, units);
-    const size_t smem = a.key_heads ? table : 0;
+    // A CTA's way to its rows is a chain of lookups (sequence, length, page: some 3 us), and the sines of a page's tokens
+    // are the same for every head. So with a team of the whole CTA it takes up to four heads one after the other, while
+    // that leaves enough CTAs for the GPU.
+    const uint32_t items = b.n_tokens / g.page_size + 2u * b.n_seqs;
+    a.heads = 0;
+    if (a.team == kNT) {
+        a.heads = 4;
+        while (a.heads > 1 && static_cast<uint64_t>(items) * 2u * ((g.n_heads + a.heads - 1) / a.heads) < 8u * 148u) a.heads /= 2;
+    }
+    const size_t table = rope.turns == nullptr ? 0 : static_cast<size_t>(g.page_size) * (rope.rot_dim / 2) * sizeof(float2);
+    const int mode = table == 0 ? kAsIs : (a.heads > 1 && table <= kSinesMax ? kSharedSines : kOwnSines);
+    const uint32_t units = a.heads ? 2u * ((g.n_heads + a.heads - 1) / a.heads) : (2u * g.n_heads + teams - 1) / teams;
+    const dim3 grid(items, units);
+    const size_t smem = mode == kSharedSines ? table : 0;
     const bool vec = view_aligned(k, g.n_heads, b.n_tokens) && view_aligned(v, g.n_heads, b.n_tokens) && rope_by_8(rope);
     const auto go = [&](auto kernel) {
         if (smem > 48u * 1024u) {
@@ -533,9 +557,16 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
         kernel<<<grid, kNT, smem, stream>>>(a);
         return cudaGetLastError();
     };
-    if (k->dtype == SIXI_SMP_BF16)
-        return vec ? go(append_kernel<__nv_bfloat16, 8>) : go(append_kernel<__nv_bfloat16, 1>);
-    return vec ? go(append_kernel<float, 8>) : go(append_kernel<float, 1>);
+    const auto pick = [&](auto type) {
+        using T = decltype(type);
+        if (vec) {
+            if (mode == kAsIs) return go(append_kernel<T, 8, kAsIs>);
+            return mode == kSharedSines ? go(append_kernel<T, 8, kSharedSines>) : go(append_kernel<T, 8, kOwnSines>);
+        }
+        if (mode == kAsIs) return go(append_kernel<T, 1, kAsIs>);
+        return mode == kSharedSines ? go(append_kernel<T, 1, kSharedSines>) : go(append_kernel<T, 1, kOwnSines>);
+    };
+    return k->dtype == SIXI_SMP_BF16 ? pick(__nv_bfloat16{}) : pick(float{});
 }
 
 cudaError_t launch_kv_read(const KvGeom& g, const KvBatchView& b, const sixi_kv_tensor* k, const sixi_kv_tensor* v,

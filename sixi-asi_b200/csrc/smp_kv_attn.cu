@@ -88,6 +88,7 @@ template <typename T>
 __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ unsigned long long scratch[kNT / 32 + 2];
+    __shared__ SeqPlan found;
     __shared__ uint32_t last_flag;
     __shared__ int32_t ids[kWindow * 4];
     const uint32_t tid = threadIdx.x, D = a.g.head_dim, row = D + 16u;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     PieceWalk walk;
     uint64_t total;
     uint32_t ctas;
-    if (!walk_init<kNT>(a.shape, a.b, a.g.page_shift, scratch, &walk, &total, &ctas)) return;
+    if (!walk_init<kNT>(a.shape, a.b, a.g.page_shift, scratch, &found, &walk, &total, &ctas)) return;
 
     const uint32_t quads = D / 4u, groups = kNT / quads;
     const uint32_t quad = tid % quads, tg = tid / quads;

@@ -296,6 +296,7 @@ struct Shared {
     uint64_t sempty[G], wfull[G], oempty[G], qfull[kNQ], qempty[kNQ], rfull[kQSlots], pfull[kPieces], meet[G], lfull, lempty,
         done;
     unsigned long long scratch[Cfg<R, DC, NB, G>::kThreads / 32 + 2];
+    SeqPlan found;
     PieceRec piece[kPieces], split[2];
     uint64_t total;
     uint32_t tmem, gave_up, ctas, pieces_done, split_mask, join_mask;
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
         uint64_t total;
         uint32_t ctas;
         tc_before();
-        const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &walk, &total, &ctas);
+        const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &sh.found, &walk, &total, &ctas);
         if (warp == C::kThreads / 32 - 1) {
             Piece pc;
             const bool any = busy && next_piece(a.shape, a.b, shift, walk, &pc);
