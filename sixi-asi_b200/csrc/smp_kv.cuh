@@ -212,6 +212,9 @@ __device__ __forceinline__ void unpack8(uint4 v, float* x) {  // 8 bf16
 // tiles. A pair (or a lone unit) takes `weight` virtual tiles; what its units leave is idle.
 struct AttnShape {
     uint32_t group, rt, tile_shift, window, all, n_heads;
+    // Beginning and ending a unit takes about as long as this many of its tiles: each unit's place on the line is so much
+    // longer than its tiles, and CTAs with many short units get fewer tiles.
+    uint32_t unit_cost;
 };
 
 // 64-bit quotient; the 32-bit one, which is much shorter, where it is enough
@@ -256,7 +259,7 @@ __device__ __forceinline__ SeqPlan plan_seq(const AttnShape& a, const KvBatchVie
     int32_t f0, e0, f1, e1;
     unit_tiles(a, p, p.nr - 1, &f1, &e1);
     if (p.nr == 1) {
-        p.weight = static_cast<uint32_t>(e1 - f1);
+        p.weight = static_cast<uint32_t>(e1 - f1) + a.unit_cost;
         return p;
     }
     // bound of one unit: the last row tile's, and under a window what the window and the tile's own
@@ -269,10 +272,10 @@ __device__ __forceinline__ SeqPlan plan_seq(const AttnShape& a, const KvBatchVie
     const uint64_t reach = 2ull * static_cast<uint64_t>(max(p.p0, 0)) +
                            quot(static_cast<uint64_t>(p.nr + 1) * a.rt, a.group);
     const uint32_t two = min(static_cast<uint32_t>((reach >> a.tile_shift) + 2u), 2u * one);
-    const uint64_t flat = static_cast<uint64_t>(p.nr) * one;
-    const uint64_t pair = static_cast<uint64_t>((p.nr + 1) / 2) * two;
+    const uint64_t flat = static_cast<uint64_t>(p.nr) * (one + a.unit_cost);
+    const uint64_t pair = static_cast<uint64_t>((p.nr + 1) / 2) * (two + 2u * a.unit_cost);
     p.paired = (pair < flat && !a.all) ? 1u : 0u;
-    p.weight = p.paired ? two : one;
+    p.weight = p.paired ? two + 2u * a.unit_cost : one + a.unit_cost;
     p.lanes = p.paired ? (p.nr + 1) / 2 : p.nr;
     return p;
 }
@@ -383,7 +386,7 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
             if (s < b.n_seqs) {
                 p = plan_seq(a, b, page_shift, s);
                 mine = plan_tiles(a, p) | (static_cast<uint64_t>(p.lanes) * a.n_heads << 40);
-                small = !p.paired && p.weight <= kWholeTiles;
+                small = !p.paired && p.weight <= kWholeTiles + a.unit_cost;
             }
             uint64_t incl = mine;
 #pragma unroll

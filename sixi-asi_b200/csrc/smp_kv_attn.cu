@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
 cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, cudaStream_t stream) {
     a.shape.rt = kRt;
     a.shape.tile_shift = kTileShift;
+    a.shape.unit_cost = 2;
     a.part_stride = part_floats(kRt, a.g.head_dim);
     const uint32_t D = a.g.head_dim;
     const size_t smem = sizeof(float) * (static_cast<size_t>(kRt) * D + 4u * kT * (D + 16u) / 4u + 4u * kT + 2u * kRt * kT +

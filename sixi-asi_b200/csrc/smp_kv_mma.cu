@@ -1045,58 +1045,58 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     }
                     __syncwarp();
                     if (use >= 1) bar_wait(&sh.ofull[(n - G) % kRing], ((n - G) / kRing) & 1u, gave_up);  // the weights' buffer is free
-                    // two tokens at a time (they share a page), so that their bytes take few registers
+                    // all four tokens at a time, so that enough chains of exponential and rounding are under way; two for
+                    // the largest row tile, whose bytes would not fit the registers
+                    constexpr int kTok = NB > 5 ? 2 : 4, kWords = (NB + 1) / 2;
+                    const float vr0 = exp2_int(ev0), vr1 = exp2_int(ev1);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float vr = exp2_int(half == 0 ? ev0 : ev1);
-                        uint32_t hi[2][(V + 3) / 4], lo[2][(V + 3) / 4];
+                    for (int t0 = 0; t0 < 4; t0 += kTok) {
+                        uint32_t hi[kTok][kWords], lo[kTok][kWords];
 #pragma unroll
-                        for (int j = 0; j < static_cast<int>(V / 2); ++j) {
-                            if (j >= NB) {
-                                if (j & 1) continue;
-                                hi[0][j / 2] = hi[1][j / 2] = lo[0][j / 2] = lo[1][j / 2] = 0u;
-                                continue;
-                            }
+                        for (int j = 0; j < NB; ++j) {
                             const float4 rf = *reinterpret_cast<const float4*>(my_ref + q * V + 2 * j);
                             const float2 fr = *reinterpret_cast<const float2*>(frow + 2 * j);
-                            const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z), wf = mul2(f2(rf.y, rf.w), f2(vr, vr));
-                            F2 sum = f2(l[2 * j], l[2 * j + 1]);
+                            const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z);
+                            const F2 wf0 = mul2(f2(rf.y, rf.w), f2(vr0, vr0)), wf1 = mul2(f2(rf.y, rf.w), f2(vr1, vr1));
+                            F2 p[kTok];
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const float2 y = un2(fma2(f2(x[j][0][2 * half + i], x[j][1][2 * half + i]), scale2, minus));
-                                const F2 p = f2(ex2(y.x), ex2(y.y));
-                                sum = add2(sum, p);
+                            for (int i = 0; i < kTok; ++i) {
+                                const float2 y = un2(fma2(f2(x[j][0][t0 + i], x[j][1][t0 + i]), scale2, minus));
+                                p[i] = f2(ex2(y.x), ex2(y.y));
+                            }
+                            F2 sum = p[0];
+#pragma unroll
+                            for (int i = 1; i < kTok; ++i) sum = add2(sum, p[i]);
+                            const float2 s2 = un2(add2(f2(l[2 * j], l[2 * j + 1]), sum));
+                            l[2 * j] = s2.x, l[2 * j + 1] = s2.y;
+#pragma unroll
+                            for (int i = 0; i < kTok; ++i) {
                                 uint32_t h, g;
-                                split2(mul2(p, wf), &h, &g);
+                                split2(mul2(p[i], t0 + i < 2 ? wf0 : wf1), &h, &g);
                                 if (j & 1) {
                                     hi[i][j / 2] = __byte_perm(hi[i][j / 2], h, 0x6420);
                                     lo[i][j / 2] = __byte_perm(lo[i][j / 2], g, 0x5410);
-                                } else {
-                                    hi[i][j / 2] = h;
+                                } else {  // (an odd block without a partner is packed here)
+                                    hi[i][j / 2] = j + 1 < NB ? h : __byte_perm(h, 0u, 0x6420);
                                     lo[i][j / 2] = g;
                                 }
                             }
-                            const float2 s2 = un2(sum);
-                            l[2 * j] = s2.x, l[2 * j + 1] = s2.y;
                         }
-                        // an odd block without a partner: its bytes still lie apart
+                        const auto word = [&](const uint32_t(&w)[kWords], int k) { return k < kWords ? w[k < kWords ? k : 0] : 0u; };
 #pragma unroll
-                        for (int j = 0; j < static_cast<int>(V / 2); j += 2)
-                            if (j + 1 >= NB)
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) hi[i][j / 2] = __byte_perm(hi[i][j / 2], 0u, 0x6420);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            uint8_t* wp = w0 + (2 * half + i) * 128;
+                        for (int i = 0; i < kTok; ++i) {
+                            uint8_t* wp = w0 + (t0 + i) * 128;
                             if constexpr (V == 4) {
                                 *reinterpret_cast<uint32_t*>(wp) = hi[i][0];
                                 *reinterpret_cast<uint32_t*>(wp + R * kTile) = lo[i][0];
                             } else if constexpr (V == 8) {
-                                *reinterpret_cast<uint2*>(wp) = make_uint2(hi[i][0], hi[i][1]);
-                                *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(lo[i][0], lo[i][1]);
+                                *reinterpret_cast<uint2*>(wp) = make_uint2(word(hi[i], 0), word(hi[i], 1));
+                                *reinterpret_cast<uint2*>(wp + R * kTile) = make_uint2(word(lo[i], 0), word(lo[i], 1));
                             } else {
-                                *reinterpret_cast<uint4*>(wp) = make_uint4(hi[i][0], hi[i][1], hi[i][2], hi[i][3]);
-                                *reinterpret_cast<uint4*>(wp + R * kTile) = make_uint4(lo[i][0], lo[i][1], lo[i][2], lo[i][3]);
+                                *reinterpret_cast<uint4*>(wp) =
+                                    make_uint4(word(hi[i], 0), word(hi[i], 1), word(hi[i], 2), word(hi[i], 3));
+                                *reinterpret_cast<uint4*>(wp + R * kTile) =
+                                    make_uint4(word(lo[i], 0), word(lo[i], 1), word(lo[i], 2), word(lo[i], 3));
                             }
                         }
                     }
@@ -1234,6 +1234,7 @@ cudaError_t launch(const MmaArgs& m, const CUtensorMap& k, const CUtensorMap& v,
     args.a.shape.rt = rt;
     args.a.part_stride = part_floats(rt, m.a.g.head_dim);
     args.a.shape.tile_shift = kTileShift;
+    args.a.shape.unit_cost = R == 16 ? 2u : 4u;
     attend_mma_kernel<R, DC, NB, G><<<ctas, C::kThreads, C::kDyn, stream>>>(args, k, v);
     return cudaGetLastError();
 }
