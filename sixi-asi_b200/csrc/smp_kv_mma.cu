@@ -131,12 +131,20 @@ __device__ __forceinline__ bool elect_one() {
         : "=r"(p));
     return p != 0u;
 }
-// a bounded barrier of four warps; *times counts the caller's
-__device__ __forceinline__ void warps_meet(uint64_t* b, uint32_t* times, volatile uint32_t* gave_up) {
-    __syncwarp();
-    if ((threadIdx.x & 31u) == 0) bar_arrive(b);
-    bar_wait(b, *times & 1u, gave_up);
-    ++*times;
+// Barrier of a softmax group's four warps. It is not bounded, but its warps cannot miss it: they run through the same
+// tiles whatever happens to the waits, and agree before each piece on whether there is one (group_any).
+__device__ __forceinline__ void group_sync(uint32_t grp) { asm volatile("bar.sync %0, 128;" ::"r"(2u + grp) : "memory"); }
+__device__ __forceinline__ bool group_any(uint32_t grp, bool x) {
+    uint32_t y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"(x ? 1u : 0u), "r"(2u + grp)
+        : "memory");
+    return y != 0u;
 }
 
 __device__ __forceinline__ void tma_page(const CUtensorMap* map, void* dst, uint64_t* bar, int32_t x, int32_t z,
@@ -293,8 +301,7 @@ struct Shared {
     static constexpr int kNK = Cfg<R, DC, NB, G>::kNK, kNV = Cfg<R, DC, NB, G>::kNV, kNQ = Cfg<R, DC, NB, G>::kNQ;
     uint64_t kfull[kNK], vfull[kNV], scfull[kNV];
     uint64_t sfull[kRing], ofull[kRing];  // of tile n at n % kRing: its scores, its output are done
-    uint64_t sempty[G], wfull[G], oempty[G], qfull[kNQ], qempty[kNQ], rfull[kQSlots], pfull[kPieces], meet[G], lfull, lempty,
-        done;
+    uint64_t sempty[G], wfull[G], oempty[G], qfull[kNQ], qempty[kNQ], rfull[kQSlots], pfull[kPieces], lfull, lempty, done;
     unsigned long long scratch[Cfg<R, DC, NB, G>::kThreads / 32 + 2];
     SeqPlan found;
     PieceRec piece[kPieces], split[2];
@@ -546,7 +553,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
         if (lane < NK) bar_init(&sh.kfull[lane], 1);
         if (lane < NV) bar_init(&sh.vfull[lane], 1), bar_init(&sh.scfull[lane], 32);
         if (lane < kRing) bar_init(&sh.sfull[lane], 1), bar_init(&sh.ofull[lane], 1);
-        if (lane < G) bar_init(&sh.sempty[lane], 4), bar_init(&sh.wfull[lane], 4), bar_init(&sh.oempty[lane], 4), bar_init(&sh.meet[lane], 4);
+        if (lane < G) bar_init(&sh.sempty[lane], 4), bar_init(&sh.wfull[lane], 4), bar_init(&sh.oempty[lane], 4);
         if (lane < NQ) bar_init(&sh.qfull[lane], kHelp), bar_init(&sh.qempty[lane], 1);
         if (lane < kQSlots) bar_init(&sh.rfull[lane], kHelp);
         if (lane < kPieces) bar_init(&sh.pfull[lane], 1);
@@ -910,8 +917,10 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             uint8_t* w0 = wbuf + grp * C::kW + (quad * 4u) * 128u + tr * 16u + ((q * V) >> 4) * (16u * kTile) + ((q * V) & 15u);
             const auto max_op = [](float x, float y) { return fmaxf(x, y); };
             const auto add_op = [](float x, float y) { return x + y; };
-            uint32_t n = 0, np = 0, meets = 0;
-            for (; const PieceRec* rec = piece(np); ++np) {
+            uint32_t n = 0;
+            for (uint32_t np = 0;; ++np) {
+                const PieceRec* rec = piece(np);
+                if (group_any(grp, rec == nullptr)) break;
                 const PieceRec& pc = *rec;
                 const uint32_t rs = np % kQSlots;
                 bar_wait(&sh.rfull[rs], (np / kQSlots) & 1u, gave_up);
@@ -953,25 +962,33 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     tc_after();
                     float x[V / 2][2][4];  // [8-column block][column][token]
 #pragma unroll
-                    for (int j = 0; j < static_cast<int>(V / 2); ++j) {
-                        if (j >= NB) {  // columns without rows
+                    for (int j0 = 0; j0 < NB; j0 += 2) {  // (two blocks' loads under way)
+                        float f[2][8], g[2][8];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) x[j][0][i] = x[j][1][i] = kNegInf;
-                            continue;
+                        for (int j = j0; j < j0 + 2; ++j) {
+                            if (j >= NB) continue;
+                            tmem_ld_frag(t_lane + 8 * j, f[j - j0]);
+                            tmem_ld_frag(t_lane + (16u << 16) + 8 * j, f[j - j0] + 4);
+                            tmem_ld_frag(t_lane + R + 8 * j, g[j - j0]);
+                            tmem_ld_frag(t_lane + (16u << 16) + R + 8 * j, g[j - j0] + 4);
                         }
-                        float f[8], g[8];
-                        tmem_ld_frag(t_lane + 8 * j, f);
-                        tmem_ld_frag(t_lane + (16u << 16) + 8 * j, f + 4);
-                        tmem_ld_frag(t_lane + R + 8 * j, g);
-                        tmem_ld_frag(t_lane + (16u << 16) + R + 8 * j, g + 4);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float fk = i < 2 ? fk0 : fk1;
-                            const float2 y = un2(mul2(add2(f2(f[2 * i], f[2 * i + 1]), f2(g[2 * i], g[2 * i + 1])), f2(fk, fk)));
-                            x[j][0][i] = y.x, x[j][1][i] = y.y;
+                        for (int j = j0; j < j0 + 2; ++j) {
+                            if (j >= NB) continue;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float fk = i < 2 ? fk0 : fk1;
+                                const F2 sum = add2(f2(f[j - j0][2 * i], f[j - j0][2 * i + 1]), f2(g[j - j0][2 * i], g[j - j0][2 * i + 1]));
+                                const float2 y = un2(mul2(sum, f2(fk, fk)));
+                                x[j][0][i] = y.x, x[j][1][i] = y.y;
+                            }
                         }
                     }
+#pragma unroll
+                    for (int j = NB; j < static_cast<int>(V / 2); ++j)  // columns without rows
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[j][0][i] = x[j][1][i] = kNegInf;
                     tc_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh.sempty[grp]);
@@ -997,7 +1014,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     fold_lanes<kFold>(mx, lane, max_op);
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
-                    warps_meet(&sh.meet[grp], &meets, gave_up);
+                    group_sync(grp);
                     float mt[kOwn];
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i)
@@ -1012,10 +1029,10 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                             mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]) * frow[c] + static_cast<float>(ev0),
                                           fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]) * frow[c] + static_cast<float>(ev1));
                         fold_lanes<kFold>(mx, lane, max_op);
-                        warps_meet(&sh.meet[grp], &meets, gave_up);  // the first maxima have been read
+                        group_sync(grp);  // the first maxima have been read
 #pragma unroll
                         for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
-                        warps_meet(&sh.meet[grp], &meets, gave_up);
+                        group_sync(grp);
 #pragma unroll
                         for (int i = 0; i < kOwn; ++i)
                             mw[i] = fmaxf(fmaxf(wmax[0][own + i], wmax[1][own + i]),
