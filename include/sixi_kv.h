@@ -74,7 +74,7 @@ typedef struct sixi_kv_batch {
     const int64_t* offsets;  /* [n_seqs + 1], offsets[0] = 0, not decreasing */
     const int32_t* lens;     /* [n_seqs] */
     uint32_t n_seqs;         /* <= max_seqs */
-    uint32_t max_pages;      /* page-table entries per sequence */
+    uint32_t max_pages;      /* page-table entries per sequence; max_pages * page_size <= 2^30 */
     uint32_t n_tokens;       /* offsets[n_seqs] */
     uint32_t max_new;        /* the largest n_s (picks a variant; results do not depend on it) */
 } sixi_kv_batch;
@@ -128,8 +128,10 @@ SIXI_SMP_API int32_t sixi_kv_rope_apply(const sixi_kv_rope* r, const sixi_kv_ten
  * NaN is written as 0 and +-Inf as +-448 * scale, scaled without them, as the clamp policy of
  * sixi_smp_numeric_policy does; out_status[s] = SIXI_NUMERIC_NAN_OR_INF then. It is
  * SIXI_OUT_OF_BOUNDS when the sequence's numbers or a page id do not fit (negative or beyond
- * n_pages, lens beyond max_pages * page_size, more new tokens than lens, rows beyond n_tokens): nothing
- * is written for bad ids or numbers. Pages of different sequences must differ where they are written.
+ * n_pages, lens beyond max_pages * page_size, more new tokens than lens): nothing is written for bad
+ * ids or numbers. Offsets that are negative, decrease or pass n_tokens leave no sequence its rows: every
+ * sequence of the call reports it, and nothing is written. Pages of different sequences must differ
+ * where they are written.
  */
 SIXI_SMP_API int32_t sixi_kv_append(sixi_kv* h, const sixi_kv_tensor* k, const sixi_kv_tensor* v,
                                     const sixi_kv_batch* batch, const sixi_kv_rope* rope, int32_t* out_status,
@@ -157,7 +159,9 @@ SIXI_SMP_API int32_t sixi_kv_read(sixi_kv* h, const sixi_kv_batch* batch, const 
  *   out_lse   [n_tokens][n_q_heads] fp32 (natural logarithm), or NULL
  *   out_status [n_seqs]: SIXI_OUT_OF_BOUNDS for a sequence whose numbers (as sixi_kv_append; but lens
  *             may be below n_s, such rows are empty) or needed page ids do not fit; its out rows are
- *             unspecified
+ *             unspecified. SIXI_BACKEND_ERROR for all if a wait inside a kernel ever runs out (and
+ *             from then on for every call of the handle)
+ * n_tokens * n_q_heads / n_kv_heads < 2^30, and the call's tiles of 8 rows by 64 positions < 2^40.
  * Pages that lie wholly before every row's window are not read, and their table entries may be anything.
  * Sums and softmax statistics are fp32. With bf16 queries the weights exp(s_t - m) enter the product
  * with the values with 8 significant bits (as bf16 weights would), and the products run on the tensor

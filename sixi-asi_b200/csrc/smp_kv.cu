@@ -252,6 +252,10 @@ __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == k
         const uint32_t s = s0 + tid;
         before += __syncthreads_count(s < a.b.n_seqs && item_base(a.b, a.g.page_shift, s) <= blockIdx.x);
     }
+    if (__syncthreads_or(kv_offsets_ok(a.b, tid, kNT) ? 0 : 1)) {  // items cannot be told from one another
+        if (blockIdx.y == 0 && blockIdx.x < a.b.n_seqs && tid == 0) a.status[blockIdx.x] = SIXI_OUT_OF_BOUNDS;
+        return;
+    }
     if (before == 0) return;
     const uint32_t seq = before - 1;
     const KvSeq q = kv_seq(a.b, a.g.page_shift, seq);
@@ -439,10 +443,11 @@ struct ReadArgs {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
+    const bool in_order = __syncthreads_or(kv_offsets_ok(a.b, tid, kNT) ? 0 : 1) == 0;
     if (blockIdx.y == 0) {  // statuses, spread over the CTAs
         for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
             const KvSeq q = kv_seq(a.b, a.g.page_shift, s);
-            bool bad = !q.ok || q.len < q.n;
+            bool bad = !in_order || !q.ok || q.len < q.n;
             if (!bad && q.n > 0) {
                 const uint32_t p0 = static_cast<uint32_t>(q.len - q.n) >> a.g.page_shift;
                 const uint32_t p1 = static_cast<uint32_t>(q.len - 1) >> a.g.page_shift;
@@ -453,6 +458,7 @@ __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
             if (tid == 0) a.status[s] = bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK;
         }
     }
+    if (!in_order) return;
     const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * a.per;
     const uint64_t t1 = t0 + a.per < a.b.n_tokens ? t0 + a.per : a.b.n_tokens;
     uint32_t before = 0;
@@ -602,7 +608,7 @@ struct sixi_kv {
     uint32_t max_seqs;
     KvGeom g;
     uint32_t* seq_state;  // [2 * max_seqs], zero between calls
-    uint32_t* counter;    // [kAttnMaxCtas], zero between calls
+    uint32_t* counter;    // [kAttnMaxCtas + 1], as AttnArgs has it
     float* part;          // attention's partial results
     CUtensorMap k_map, v_map;  // pages as attention copies them
 };
@@ -614,7 +620,6 @@ struct sixi_kv_rope {
 };
 
 namespace {
-
 
 int32_t kv_from_cuda(cudaError_t e) {
     if (e == cudaSuccess) return SIXI_OK;
@@ -643,8 +648,9 @@ bool tensor_ok(const sixi_kv_tensor* t, uint64_t n_tokens) {
 bool batch_ok(const sixi_kv* h, const sixi_kv_batch* b) {
     if (b == nullptr || b->n_seqs > h->max_seqs || b->n_tokens > 0x7FFFFFFFu) return false;
     if (b->n_seqs == 0) return b->n_tokens == 0;
+    // (positions of a tile's end and of a window's beginning stay within 31 bits)
     return b->offsets != nullptr && b->lens != nullptr && b->page_table != nullptr && b->table_stride >= b->max_pages &&
-           b->max_pages > 0;
+           b->max_pages > 0 && static_cast<uint64_t>(b->max_pages) * h->g.page_size <= (1ull << 30);
 }
 
 KvBatchView batch_view(const sixi_kv_batch* b) {
@@ -729,11 +735,11 @@ int32_t sixi_kv_create(int32_t device, const sixi_kv_config* c, void* k_pages, v
     // 64 rows a CTA for one CTA per SM, or 16 for two
     const uint64_t part = 2ull * h->n_sms * part_floats(64, c->head_dim);
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&h->seq_state), sizeof(uint32_t) * 2u * c->max_seqs);
-    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&h->counter), sizeof(uint32_t) * kAttnMaxCtas);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&h->counter), sizeof(uint32_t) * (kAttnMaxCtas + 1u));
     if (e == cudaSuccess)
         e = cudaMalloc(reinterpret_cast<void**>(&h->part), sizeof(float) * part);
     if (e == cudaSuccess) e = cudaMemset(h->seq_state, 0, sizeof(uint32_t) * 2u * c->max_seqs);
-    if (e == cudaSuccess) e = cudaMemset(h->counter, 0, sizeof(uint32_t) * kAttnMaxCtas);
+    if (e == cudaSuccess) e = cudaMemset(h->counter, 0, sizeof(uint32_t) * (kAttnMaxCtas + 1u));
     if (e == cudaSuccess) e = make_page_map(k_pages, h->g, &h->k_map);
     if (e == cudaSuccess) e = make_page_map(v_pages, h->g, &h->v_map);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -854,6 +860,9 @@ int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch*
     const uint64_t group = q->n_heads / h->g.n_heads;
     if (static_cast<uint64_t>(b->n_tokens) * group > 0x3FFFFFFFull) return SIXI_INVALID_ARGUMENT;
     if (b->n_seqs == 0) return SIXI_OK;
+    // the schedule counts tiles (of 64 tokens and 8 rows at least) in 40 bits
+    const double units = (b->n_tokens * static_cast<double>(group) / 8 + 2.0 * b->n_seqs) * h->g.n_heads;
+    if (units * (b->max_pages * static_cast<double>(h->g.page_size) / 64 + 8) >= 1099511627776.0) return SIXI_INVALID_ARGUMENT;
     if (out_status == nullptr) return SIXI_INVALID_ARGUMENT;
     KvDeviceGuard guard(h->device);
     AttnArgs a;

@@ -66,6 +66,17 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatchView& b, uint32_t page_shif
     return q;
 }
 
+// Whether the offsets from `at` on, `step` apart, are in order and within the call's rows. Where any is not, rows could
+// belong to two sequences or to none, so every sequence of the call reports it.
+__device__ __forceinline__ bool kv_offsets_ok(const KvBatchView& b, uint32_t at, uint32_t step) {
+    bool ok = true;
+    for (uint32_t s = at; s < b.n_seqs; s += step) {
+        const int64_t r0 = b.offsets[s], r1 = b.offsets[s + 1];
+        ok &= r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(b.n_tokens);
+    }
+    return ok;
+}
+
 // ---------------------------------------------------------------------------------------------
 // e4m3 and its power-of-two scales
 
@@ -466,6 +477,8 @@ __device__ __forceinline__ uint32_t place_owner(uint64_t x, uint64_t total, uint
 // ---------------------------------------------------------------------------------------------
 // launches (host)
 
+constexpr uint32_t kAttnMaxCtas = 512;  // CTAs of an attention call at most
+
 struct AttnArgs {
     KvGeom g;
     KvBatchView b;
@@ -476,7 +489,7 @@ struct AttnArgs {
     float* lse;
     int32_t* status;
     float* part;        // [2 * ctas][part_stride]
-    uint32_t* counter;  // [ctas], zero between calls
+    uint32_t* counter;  // [kAttnMaxCtas], zero between calls; then one word: a wait of a call has run out
     uint64_t part_stride;
 };
 
@@ -488,7 +501,6 @@ inline bool rope_by_8(const RopeView& r) {
 // Partial results: two per CTA (a unit that the CTA continues, and one that it leaves to the next), each the row tile's
 // rows of head_dim unnormalised fp32 sums, then the rows' maxima (base 2) and sums. They lie close together: a step over
 // a large cache keeps few address translations alive, and joining results that were megabytes apart took 10 us more.
-constexpr uint32_t kAttnMaxCtas = 512;
 inline uint64_t part_floats(uint32_t rows, uint32_t head_dim) { return static_cast<uint64_t>(rows) * (head_dim + 2u); }
 
 // ---------------------------------------------------------------------------------------------

@@ -106,9 +106,9 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         sm.l = f;
     }
     for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
-        const bool ok = seq_pages_ok(a.shape, a.b, a.g.page_shift, a.g.n_pages, s, tid, kNT);
+        const bool ok = kv_offsets_ok(a.b, tid, kNT) && seq_pages_ok(a.shape, a.b, a.g.page_shift, a.g.n_pages, s, tid, kNT);
         const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
-        if (tid == 0) a.status[s] = bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK;
+        if (tid == 0) a.status[s] = a.counter[kAttnMaxCtas] ? SIXI_BACKEND_ERROR : (bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK);
     }
     PieceWalk walk;
     uint64_t total;

@@ -47,7 +47,8 @@ constexpr int kTile = 128;      // tokens of a tile
 constexpr int kTileShift = 7;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait (never expected to run out)
+constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait: a second and more (never expected to run out)
+constexpr uint32_t kSleepAfter = 1u << 12, kSleepNs = 256;
 constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
 constexpr uint32_t kPieces = 16; // piece records kept; the walk stays 12 ahead of the output at most
 constexpr int kQSlots = 16;  // pieces whose row records are kept: softmax lags the staging by fewer than 10
@@ -109,7 +110,10 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
 __device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
     if (!bar_try(b, parity)) {
         bool ok = false;
-        for (uint32_t i = 0; i < kWaitIters && !ok; ++i) ok = bar_try(b, parity) || *gave_up != 0u;
+        for (uint32_t i = 0; i < kWaitIters && !ok; ++i) {
+            ok = bar_try(b, parity) || *gave_up != 0u;
+            if (!ok && i >= kSleepAfter) __nanosleep(kSleepNs);  // (what waits for a whole piece may wait long)
+        }
         if (!ok) *gave_up = 1u;
     }
     __syncwarp();
@@ -1162,7 +1166,8 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 Piece pc;
                 const bool any = next_piece(a.shape, a.b, shift, walk, &pc);
                 volatile uint32_t* done = &sh.pieces_done;
-                for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i) __nanosleep(64);
+                for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i)
+                    __nanosleep(i < kSleepAfter ? 64u : 4u * kSleepNs);
                 __syncwarp();
                 if (__any_sync(kFull, np - *done > 12u)) break;  // (given up)
                 if (lane == 0) {
@@ -1206,9 +1211,14 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     if (warp == C::kThreads / 32 - 1) {
         // statuses, over the grid
         for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
-            const bool ok = seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
+            const bool ok = kv_offsets_ok(a.b, lane, 32u) && seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
             const bool bad = __any_sync(kFull, !ok);
-            if (lane == 0) a.status[s] = bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK;
+            if (lane == 0) {
+                volatile int32_t* st = a.status + s;
+                *st = bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK;
+                __threadfence();  // (a CTA that gives up raises the word first and writes its statuses after)
+                if (*const_cast<volatile uint32_t*>(a.counter + kAttnMaxCtas)) *st = SIXI_BACKEND_ERROR;
+            }
             __syncwarp();
         }
     }
@@ -1224,7 +1234,11 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             }
             __syncwarp();
         }
-        for (uint32_t s = tid; s < a.b.n_seqs; s += C::kThreads) a.status[s] = SIXI_BACKEND_ERROR;
+        // the counters of the units that this CTA shares are not what they were: every later call reports it too
+        if (tid == 0) *const_cast<volatile uint32_t*>(a.counter + kAttnMaxCtas) = 1u;
+        __threadfence();
+        __syncthreads();
+        for (uint32_t s = tid; s < a.b.n_seqs; s += C::kThreads) *const_cast<volatile int32_t*>(a.status + s) = SIXI_BACKEND_ERROR;
     }
     __syncthreads();
     if (warp == 1)

@@ -298,6 +298,28 @@ def test_append_and_read_report_what_does_not_fit():
     assert (k[12:] == 7).all() and (v[12:] == 7).all()  # bad numbers
 
 
+@pytest.mark.parametrize("offsets", [[0, 10, 5, 12], [0, 4, 8, 13], [-1, 4, 8, 12]])
+def test_offsets_out_of_order_are_reported_by_every_sequence(offsets):
+    w = World(10, [20, 20, 20], 16, 2, 32).fill()
+    b = w.batch([4, 4, 4])
+    x = torch.from_numpy(w.rng.normal(size=(12, 2, 32))).to(F32).to(DEV)
+    want = host(w.kv.attend(x, b)[0])
+    b.offsets.copy_(torch.tensor(offsets))
+    y = torch.full_like(x, 7.0)
+    for _ in range(2):  # (nothing is left behind that a later call would meet)
+        assert w.kv.append(x, x, b).tolist() == [2, 2, 2]
+        w.same_bytes()
+        st = torch.zeros(3, dtype=torch.int32, device=DEV)
+        w.kv.read(b, k=y, v=y.clone(), status=st)
+        assert st.tolist() == [2, 2, 2] and (y == 7).all()
+        for q in (x, x.to(BF)):
+            assert w.kv.attend(q, b)[2].tolist() == [2, 2, 2]
+    good = w.batch([4, 4, 4])
+    out, _, st = w.kv.attend(x, good)
+    assert st.tolist() == [0, 0, 0] and np.array_equal(host(out), want)
+    assert w.kv.append(x, x, good).tolist() == [0, 0, 0]
+
+
 def test_append_understated_max_new():
     """max_new picks a variant only."""
     w = World(9, [200], 64, 2, 128).fill([3])
@@ -568,3 +590,15 @@ def test_python_checks():
         Rope(64, layout="other", device=0)
     with pytest.raises(S.SixiError):
         KvCache(4, 24, 2, 32, device=0)
+
+
+def test_tables_beyond_2_30_positions_are_refused():
+    w = World(35, [20], 16, 2, 32).fill()
+    b = w.batch([2])
+    x = torch.zeros((2, 2, 32), device=DEV)
+    b.struct.table_stride = 2 ** 28
+    for pages in (2 ** 26 + 1, 2 ** 28):
+        b.struct.max_pages = pages
+        for call in (lambda: w.kv.append(x, x, b), lambda: w.kv.read(b, k=x, v=x), lambda: w.kv.attend(x, b)):
+            with pytest.raises(S.SixiError):
+                call()
