@@ -17,9 +17,12 @@ namespace {
 constexpr int kNT = 256;
 
 // ---------------------------------------------------------------------------------------------
-// sixi_kv_rope_apply. A thread takes VEC pairs (half layout) or VEC / 2 pairs (interleaved) of one
-// token, computes their sines once and turns those elements of `hpt` heads; the elements that are
-// passed through are further chunks. Bound by memory: every element is read and written once.
+// sixi_kv_rope_apply: (a, b) -> amp * (a cos - b sin, b cos + a sin) for pair i of a head's first rot_dim elements, the
+// angle position * f_i; the inverse has the sine's sign turned, which is also the gradient. Bound by memory: every element
+// is read and written once. A thread takes VEC pairs (half layout) or VEC / 2 pairs (interleaved) of one token, computes
+// their sines once and turns those elements of `hpt` heads; the elements that are passed through are further chunks.
+// 16,384 tokens of 40 heads of 128 bf16 elements (half layout): 58.2 us, 5.8 TB/s, 88 % of the copy rate. 5 tokens of 12
+// heads: 2.3 us, the launch.
 
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kNT) rope_kernel(RopeView r, KvView x, KvView out, const int32_t* __restrict__ positions,
@@ -140,13 +143,25 @@ cudaError_t rope_dispatch(const RopeView& r, const sixi_kv_tensor* x, const int3
 }
 
 // ---------------------------------------------------------------------------------------------
-// sixi_kv_append. An item is a page that a sequence's new tokens touch; a unit is one head's keys or
-// values of an item. The scale is a maximum over the unit's new rows, so a unit is the work of one
-// team: the lanes of one row (D / 8, 8 elements each) when an item has few rows, the whole CTA with
-// its rows side by side when it has many. The first kRowsHeld rows of a lane stay in registers
-// between the maximum and the rounding; further ones (a max_new below the real one) are read again.
-// Items are numbered so that the host needs no lengths: sequence s starts at floor(offsets[s] /
-// page_size) + 2 s, which leaves room for every page that it can touch.
+// sixi_kv_append. With m the largest magnitude of a page's and head's new rows, e the least exponent with m <= 448 * 2^e
+// and e' the page's own: scale 2^max(e, e'), bytes e4m3(x / scale). The scale is a maximum over rows, so a page's rows of
+// one head (a unit) are the work of one team, which holds the first kRowsHeld rows of a lane in registers between the
+// maximum and the rounding; further ones are read again. A row takes the lanes of D / 8 elements, 8 each.
+//
+// Bound: a prompt by memory (18,796 tokens of 8 heads of 128 bf16 elements: 116 MB in and out, 17.7 us at the copy rate,
+// 57 us with the keys' rotation and 40 without, of which the waits of a CTA's four steps - rows, maximum, scale, bytes -
+// are most); few tokens by latency: the chain of sequence, length, page, rows and scale is 4.7 us for 64 tokens of 64
+// sequences. So:
+// - few rows (up to kRowsFew a page): a unit is at most a warp's, and a CTA takes many units. 153 tokens of 37 sequences,
+//   9 at most: 6.1 us, and 8.1 with a CTA a unit.
+// - many rows: the whole CTA is the team, rows side by side, up to four heads one after the other, which share their
+//   tokens' sines.
+// - a page that holds older rows and whose scale grows: all its older rows are rounded again by the whole CTA, whoever's
+//   unit it is. It happens to few units at a time: 10.2 us where one head of 16 grows (64 tokens, pages of 64 with 60
+//   older rows, memory cold), 22.5 when the unit's team does it alone, 10.2 without growth.
+//
+// An item is a page that a sequence's new tokens touch. Items are numbered so that the host needs no lengths: sequence s
+// starts at floor(offsets[s] / page_size) + 2 s, which leaves room for every page that it can touch.
 
 struct AppendArgs {
     KvGeom g;
@@ -161,6 +176,7 @@ struct AppendArgs {
 };
 
 constexpr int kRowsHeld = 4;
+constexpr uint32_t kRowsFew = 16;
 constexpr size_t kSinesMax = 64u * 1024u;
 constexpr uint32_t kFlagNan = 1u, kFlagBounds = 2u;
 
@@ -225,6 +241,14 @@ __device__ __forceinline__ void clean8(float* x, float* m, bool* bad) {
     }
 }
 
+__device__ __forceinline__ void unpack8_e4m3(uint2 o, float* y) {
+    float2 f;
+    f = e4m3x2_to_float2(o.x), y[0] = f.x, y[1] = f.y;
+    f = e4m3x2_to_float2(o.x >> 16), y[2] = f.x, y[3] = f.y;
+    f = e4m3x2_to_float2(o.y), y[4] = f.x, y[5] = f.y;
+    f = e4m3x2_to_float2(o.y >> 16), y[6] = f.x, y[7] = f.y;
+}
+
 __device__ __forceinline__ uint2 round8(const float* x, float mul) {
     uint2 o;
     o.x = e4m3x2(x[0] * mul, x[1] * mul) | (e4m3x2(x[2] * mul, x[3] * mul) << 16);
@@ -239,8 +263,12 @@ template <typename T, int VEC, int MODE>
 __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == kSharedSines && VEC > 1 ? 3 : 2))
     append_kernel(AppendArgs a) {
     __shared__ float red[kNT / 32];
+    __shared__ uint32_t n_grown;
+    __shared__ uint8_t* grown_page[kNT / 2];  // (a row has two lanes at least)
+    __shared__ float grown_mul[kNT / 2];
     extern __shared__ float2 sines[];  // [new rows of the page][rot_dim / 2], with shared sines
     const uint32_t tid = threadIdx.x;
+    if (tid == 0) n_grown = 0u;
     // the sequences whose status needs no pages (no new tokens, or numbers that do not fit)
     if (blockIdx.y == 0 && blockIdx.x < a.b.n_seqs && tid == 0) {
         const KvSeq q = kv_seq(a.b, a.g.page_shift, blockIdx.x);
@@ -297,109 +325,126 @@ __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == k
     }
     bool bad = false;
     for (uint32_t unit = unit0; unit < unit_end; ++unit) {
-    const bool live = id_ok && unit < 2u * a.g.n_heads;
-    const bool is_v = unit >= a.g.n_heads;
-    const uint32_t head = is_v ? unit - a.g.n_heads : unit;
-    const KvView& src = is_v ? a.v : a.k;
-    const bool turn = MODE != kAsIs && !is_v;
-    const T* base = static_cast<const T*>(src.data) + head * src.head_stride;
-    const bool lane_on = live && i0 < D;
-    const auto row_of = [&](uint32_t slot) {
-        return base + (q.row0 + (page0 + static_cast<int32_t>(slot) - start)) * src.token_stride;
-    };
-    const auto turn_row = [&](uint32_t slot, float* y) {  // y: the row's elements as loaded
-        if constexpr (MODE == kSharedSines) turn8<T, VEC>(a.rope, row_of(slot), i0, sines + (slot - slot0) * half, y);
-        if constexpr (MODE == kOwnSines) load_row8<T, VEC>(a.rope, row_of(slot), i0, page0 + static_cast<int32_t>(slot), y);
-    };
-    const auto load = [&](uint32_t slot, float* y, float* mm) {
+        const bool live = id_ok && unit < 2u * a.g.n_heads;
+        const bool is_v = unit >= a.g.n_heads;
+        const uint32_t head = is_v ? unit - a.g.n_heads : unit;
+        const KvView& src = is_v ? a.v : a.k;
+        const bool turn = MODE != kAsIs && !is_v;
+        const T* base = static_cast<const T*>(src.data) + head * src.head_stride;
+        const bool lane_on = live && i0 < D;
+        const auto row_of = [&](uint32_t slot) {
+            return base + (q.row0 + (page0 + static_cast<int32_t>(slot) - start)) * src.token_stride;
+        };
+        const auto turn_row = [&](uint32_t slot, float* y) {  // y: the row's elements as loaded
+            if constexpr (MODE == kSharedSines) turn8<T, VEC>(a.rope, row_of(slot), i0, sines + (slot - slot0) * half, y);
+            if constexpr (MODE == kOwnSines) load_row8<T, VEC>(a.rope, row_of(slot), i0, page0 + static_cast<int32_t>(slot), y);
+        };
+        const auto load = [&](uint32_t slot, float* y, float* mm) {
 #pragma unroll
-        for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(row_of(slot) + i0 + j, y + j);
-        if (turn) turn_row(slot, y);
-        clean8(y, mm, &bad);
-    };
+            for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(row_of(slot) + i0 + j, y + j);
+            if (turn) turn_row(slot, y);
+            clean8(y, mm, &bad);
+        };
 
-    float x[kRowsHeld][8];
-    float m = 0.0f;
-    if (lane_on) {
-        // the held rows' elements are asked for together, then worked on
-#pragma unroll
-        for (int p = 0; p < kRowsHeld; ++p) {
-            const uint32_t slot = min(slot0 + p * rows_at_once + row_in, slot1 - 1u);
-            const T* r = row_of(slot);
-#pragma unroll
-            for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(r + i0 + j, x[p] + j);
-        }
-#pragma unroll
-        for (int p = 0; p < kRowsHeld; ++p) {
-            const uint32_t slot = slot0 + p * rows_at_once + row_in;
-            if (slot >= slot1) continue;
-            if (turn) turn_row(slot, x[p]);
-            clean8(x[p], &m, &bad);
-        }
-        for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
-            float y[8];
-            load(slot, y, &m);
-        }
-    }
-    // the unit's maximum: over the lanes of a row by shuffles, over the CTA's warps through shared memory
-    const uint32_t width = a.team < 32u ? a.team : 32u;
-    for (uint32_t o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (a.team > 32u) {
-        __syncthreads();  // (the last unit's have been read)
-        if ((tid & 31u) == 0) red[tid >> 5] = m;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kNT / 32; ++i) m = fmaxf(m, red[i]);
-    }
-    float* sp = nullptr;
-    int e = 0;
-    bool write_scale = false;
-    if (live) {
-        const uint64_t ph = static_cast<uint64_t>(id) * a.g.n_heads + head;
-        sp = (is_v ? a.g.v_scales : a.g.k_scales) + ph;
-        uint8_t* pg = (is_v ? a.g.v_pages : a.g.k_pages) + ph * a.g.page_size * D;
-        e = kv_scale_exp(m);
-        write_scale = true;
-        if (slot0 > 0) {
-            const int eo = scale_exp_of(*sp);
-            if (e > eo) {  // the page's scale grows: its older rows are rounded again at the new one
-                const float mul = exp2_int(max(eo - e, -126));
-                if (lane_on) {
-                    for (uint32_t slot = row_in; slot < slot0; slot += rows_at_once) {
-                        uint2* w = reinterpret_cast<uint2*>(pg + slot * D + i0);
-                        const uint2 o = *w;
-                        float y[8];
-                        float2 f;
-                        f = e4m3x2_to_float2(o.x), y[0] = f.x, y[1] = f.y;
-                        f = e4m3x2_to_float2(o.x >> 16), y[2] = f.x, y[3] = f.y;
-                        f = e4m3x2_to_float2(o.y), y[4] = f.x, y[5] = f.y;
-                        f = e4m3x2_to_float2(o.y >> 16), y[6] = f.x, y[7] = f.y;
-                        *w = round8(y, mul);
-                    }
-                }
-            } else {
-                e = eo;
-                write_scale = false;
-            }
-        }
-        const float mul = exp2_int(-e);
+        float x[kRowsHeld][8];
+        float m = 0.0f;
         if (lane_on) {
+            // the held rows' elements are asked for together, then worked on
+#pragma unroll
+            for (int p = 0; p < kRowsHeld; ++p) {
+                const uint32_t slot = min(slot0 + p * rows_at_once + row_in, slot1 - 1u);
+                const T* r = row_of(slot);
+#pragma unroll
+                for (int j = 0; j < 8; j += VEC) load_vec<T, VEC>(r + i0 + j, x[p] + j);
+            }
 #pragma unroll
             for (int p = 0; p < kRowsHeld; ++p) {
                 const uint32_t slot = slot0 + p * rows_at_once + row_in;
-                if (slot < slot1) *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(x[p], mul);
+                if (slot >= slot1) continue;
+                if (turn) turn_row(slot, x[p]);
+                clean8(x[p], &m, &bad);
             }
             for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
-                float y[8], again = 0.0f;
-                load(slot, y, &again);
-                *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(y, mul);
+                float y[8];
+                load(slot, y, &m);
             }
         }
-    }
-    // every lane of the team has read the old scale before it is replaced (by all threads of the CTA:
-    // lanes without a unit must not miss the barrier)
-    __syncthreads();
-    if (in_team == 0 && write_scale) *sp = exp2_int(e);
+        // the unit's maximum: over the lanes of a row by shuffles, over the CTA's warps through shared memory
+        const uint32_t width = a.team < 32u ? a.team : 32u;
+        for (uint32_t o = width >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if (a.team > 32u) {
+            __syncthreads();  // (the last unit's have been read)
+            if ((tid & 31u) == 0) red[tid >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kNT / 32; ++i) m = fmaxf(m, red[i]);
+        }
+        float* sp = nullptr;
+        int e = 0;
+        bool write_scale = false;
+        if (live) {
+            const uint64_t ph = static_cast<uint64_t>(id) * a.g.n_heads + head;
+            sp = (is_v ? a.g.v_scales : a.g.k_scales) + ph;
+            uint8_t* pg = (is_v ? a.g.v_pages : a.g.k_pages) + ph * a.g.page_size * D;
+            e = kv_scale_exp(m);
+            write_scale = true;
+            if (slot0 > 0) {
+                const int eo = scale_exp_of(*sp);
+                if (e > eo) {  // the page's scale grows
+                    if (in_team == 0) {
+                        const uint32_t g = atomicAdd(&n_grown, 1u);
+                        grown_page[g] = pg;
+                        grown_mul[g] = exp2_int(max(eo - e, -126));
+                    }
+                } else {
+                    e = eo;
+                    write_scale = false;
+                }
+            }
+            const float mul = exp2_int(-e);
+            if (lane_on) {
+#pragma unroll
+                for (int p = 0; p < kRowsHeld; ++p) {
+                    const uint32_t slot = slot0 + p * rows_at_once + row_in;
+                    if (slot < slot1) *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(x[p], mul);
+                }
+                for (uint32_t slot = slot0 + kRowsHeld * rows_at_once + row_in; slot < slot1; slot += rows_at_once) {
+                    float y[8], again = 0.0f;
+                    load(slot, y, &again);
+                    *reinterpret_cast<uint2*>(pg + slot * D + i0) = round8(y, mul);
+                }
+            }
+        }
+        // every lane of the team has read the old scale before it is replaced (by all threads of the CTA:
+        // lanes without a unit must not miss the barrier)
+        __syncthreads();
+        if (in_team == 0 && write_scale) *sp = exp2_int(e);
+        // The older rows of pages whose scale has grown are rounded again at it, by the whole CTA: they may be a page's worth
+        // for a single new token, and seldom of more than one of the CTA's units.
+        const uint32_t grown = n_grown;
+        if (grown > 0u) {
+            const uint32_t per_row = D / 8u, per_page = slot0 * per_row, all = grown * per_page;
+            for (uint32_t c0 = tid; c0 < all; c0 += 4u * kNT) {
+                uint2* at[4];
+                uint2 o[4];
+                float mul[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t c = min(c0 + u * kNT, all - 1u), g = c / per_page;
+                    at[u] = reinterpret_cast<uint2*>(grown_page[g]) + (c - g * per_page);
+                    mul[u] = grown_mul[g];
+                    o[u] = *at[u];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float y[8];
+                    unpack8_e4m3(o[u], y);
+                    if (c0 + u * kNT < all) *at[u] = round8(y, mul[u]);
+                }
+            }
+            __syncthreads();
+            if (tid == 0) n_grown = 0u;  // (the next unit's team meets before it adds to it)
+        }
     }
     // the sequence's status: the last of its CTAs to arrive writes it
     const bool any_bad = __syncthreads_or(bad ? 1 : 0) != 0;
@@ -430,7 +475,8 @@ __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == k
 
 // ---------------------------------------------------------------------------------------------
 // sixi_kv_read: bytes times scale, 8 elements a lane at a time; a warp takes a token, so that its page is looked up once,
-// and keeps four loads in flight. Bound by memory.
+// and keeps four loads in flight. Bound by memory: 18,796 tokens of 8 heads of 128 elements into bf16, keys and values:
+// 28.2 us, 4.1 TB/s. A token of each of 64 sequences: 4.7 us, the chain of lookups.
 
 struct ReadArgs {
     KvGeom g;
@@ -508,11 +554,9 @@ __global__ void __launch_bounds__(kNT) read_kernel(ReadArgs a) {
             for (int u = 0; u < kUnroll; ++u) {
                 if (c0 + 32u * u >= chunks) continue;
                 float y[8];
-                float2 v;
-                v = e4m3x2_to_float2(o[u].x), y[0] = v.x * f[u], y[1] = v.y * f[u];
-                v = e4m3x2_to_float2(o[u].x >> 16), y[2] = v.x * f[u], y[3] = v.y * f[u];
-                v = e4m3x2_to_float2(o[u].y), y[4] = v.x * f[u], y[5] = v.y * f[u];
-                v = e4m3x2_to_float2(o[u].y >> 16), y[6] = v.x * f[u], y[7] = v.y * f[u];
+                unpack8_e4m3(o[u], y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] *= f[u];
                 T* p = out + head[u] * dst.head_stride + i0[u];
 #pragma unroll
                 for (int j = 0; j < 8; j += VEC) store_vec<T, VEC>(p + j, y + j);
@@ -538,7 +582,10 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
     a.row_lanes = 2;
     while (a.row_lanes < g.head_dim / 8) a.row_lanes *= 2;
     const uint32_t rows = max_new < g.page_size ? max_new : g.page_size;
-    a.team = rows <= kRowsHeld ? a.row_lanes : kNT;
+    // few rows: up to a warp a unit, so that many units share a CTA's way to them
+    a.team = kNT;
+    if (rows <= kRowsFew)
+        for (a.team = a.row_lanes; a.team < 32u && a.team / a.row_lanes * kRowsHeld < rows;) a.team *= 2;
     const uint32_t teams = kNT / a.team;
     // A CTA's way to its rows is a chain of lookups (sequence, length, page: some 3 us), and the sines of a page's tokens
     // are the same for every head. So with a team of the whole CTA it takes up to four heads one after the other, while
