@@ -180,8 +180,8 @@ constexpr uint32_t kRowsFew = 16;
 constexpr size_t kSinesMax = 64u * 1024u;
 constexpr uint32_t kFlagNan = 1u, kFlagBounds = 2u;
 
-__device__ __forceinline__ uint32_t item_base(const KvBatchView& b, uint32_t page_shift, uint32_t s) {
-    return static_cast<uint32_t>(static_cast<uint64_t>(b.offsets[s]) >> page_shift) + 2u * s;
+__device__ __forceinline__ uint32_t item_base(int64_t row0, uint32_t page_shift, uint32_t s) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(row0) >> page_shift) + 2u * s;
 }
 
 // 8 elements of a row, turned
@@ -263,6 +263,9 @@ template <typename T, int VEC, int MODE>
 __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == kSharedSines && VEC > 1 ? 3 : 2))
     append_kernel(AppendArgs a) {
     __shared__ float red[kNT / 32];
+    __shared__ KvSeq item_q;
+    __shared__ uint32_t item_seq, item_page;
+    __shared__ int32_t item_id;
     __shared__ uint32_t n_grown;
     __shared__ uint8_t* grown_page[kNT / 2];  // (a row has two lanes at least)
     __shared__ float grown_mul[kNT / 2];
@@ -275,28 +278,41 @@ __global__ void __launch_bounds__(kNT, MODE == kAsIs && VEC > 1 ? 4 : (MODE == k
         const bool ok = q.ok && q.len >= q.n;
         if (!ok || q.n == 0) a.status[blockIdx.x] = ok ? SIXI_OK : SIXI_OUT_OF_BOUNDS;
     }
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += kNT) {
-        const uint32_t s = s0 + tid;
-        before += __syncthreads_count(s < a.b.n_seqs && item_base(a.b, a.g.page_shift, s) <= blockIdx.x);
+    // the item's sequence and page: found by the thread that comes upon the sequence, so that a CTA's way to its rows is
+    // three loads long
+    bool in_order = true, mine = false;
+    for (uint32_t s = tid; s < a.b.n_seqs; s += kNT) {
+        const int64_t r0 = a.b.offsets[s], r1 = a.b.offsets[s + 1];
+        const int32_t len = a.b.lens[s];
+        in_order &= r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(a.b.n_tokens);
+        const uint32_t at = item_base(r0, a.g.page_shift, s), next = item_base(r1, a.g.page_shift, s + 1u);
+        if (at <= blockIdx.x && (blockIdx.x < next || s + 1u == a.b.n_seqs)) {
+            const KvSeq q = kv_seq_of(a.b, a.g.page_shift, r0, r1, len);
+            const int32_t start = q.len - q.n;
+            const uint32_t pi = (static_cast<uint32_t>(start) >> a.g.page_shift) + (blockIdx.x - at);
+            mine = q.ok && q.n > 0 && start >= 0 && pi <= static_cast<uint32_t>(q.len - 1) >> a.g.page_shift;
+            if (mine) {
+                item_q = q;
+                item_seq = s;
+                item_page = pi;
+                item_id = a.b.page_table[s * a.b.table_stride + pi];
+            }
+        }
     }
-    if (__syncthreads_or(kv_offsets_ok(a.b, tid, kNT) ? 0 : 1)) {  // items cannot be told from one another
+    if (__syncthreads_or(in_order ? 0 : 1)) {  // items cannot be told from one another
         if (blockIdx.y == 0 && blockIdx.x < a.b.n_seqs && tid == 0) a.status[blockIdx.x] = SIXI_OUT_OF_BOUNDS;
         return;
     }
-    if (before == 0) return;
-    const uint32_t seq = before - 1;
-    const KvSeq q = kv_seq(a.b, a.g.page_shift, seq);
-    if (!q.ok || q.n == 0 || q.len < q.n) return;
+    if (!__syncthreads_or(mine ? 1 : 0)) return;
+    const uint32_t seq = item_seq, pi = item_page;
+    const KvSeq q = item_q;
     const int32_t start = q.len - q.n;
     const uint32_t first_page = static_cast<uint32_t>(start) >> a.g.page_shift;
     const uint32_t last_page = static_cast<uint32_t>(q.len - 1) >> a.g.page_shift;
-    const uint32_t pi = first_page + (blockIdx.x - item_base(a.b, a.g.page_shift, seq));
-    if (pi > last_page) return;
     const int32_t page0 = static_cast<int32_t>(pi << a.g.page_shift);
     const uint32_t slot0 = static_cast<uint32_t>(max(start, page0) - page0);
     const uint32_t slot1 = static_cast<uint32_t>(min(q.len - page0, static_cast<int32_t>(a.g.page_size)));
-    const int32_t id = a.b.page_table[seq * a.b.table_stride + pi];
+    const int32_t id = item_id;
     const bool id_ok = static_cast<uint32_t>(id) < a.g.n_pages;
 
     const uint32_t teams = kNT / a.team;

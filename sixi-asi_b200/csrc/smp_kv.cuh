@@ -55,15 +55,17 @@ struct KvSeq {
     bool ok;
 };
 
-__device__ __forceinline__ KvSeq kv_seq(const KvBatchView& b, uint32_t page_shift, uint32_t s) {
-    const int64_t r0 = b.offsets[s], r1 = b.offsets[s + 1];
+__device__ __forceinline__ KvSeq kv_seq_of(const KvBatchView& b, uint32_t page_shift, int64_t r0, int64_t r1, int32_t len) {
     KvSeq q;
     q.row0 = r0;
-    q.len = b.lens[s];
-    q.ok = r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(b.n_tokens) && q.len >= 0 &&
-           static_cast<uint64_t>(q.len) <= (static_cast<uint64_t>(b.max_pages) << page_shift);
+    q.len = len;
+    q.ok = r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(b.n_tokens) && len >= 0 &&
+           static_cast<uint64_t>(len) <= (static_cast<uint64_t>(b.max_pages) << page_shift);
     q.n = q.ok ? static_cast<int32_t>(r1 - r0) : 0;
     return q;
+}
+__device__ __forceinline__ KvSeq kv_seq(const KvBatchView& b, uint32_t page_shift, uint32_t s) {
+    return kv_seq_of(b, page_shift, b.offsets[s], b.offsets[s + 1], b.lens[s]);
 }
 
 // Whether the offsets from `at` on, `step` apart, are in order and within the call's rows. Where any is not, rows could
