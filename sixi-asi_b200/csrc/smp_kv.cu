@@ -149,13 +149,12 @@ cudaError_t rope_dispatch(const RopeView& r, const sixi_kv_tensor* x, const int3
 // maximum and the rounding; further ones are read again. A row takes the lanes of D / 8 elements, 8 each.
 //
 // Bound: a prompt by memory (18,796 tokens of 8 heads of 128 bf16 elements: 116 MB in and out, 17.7 us at the copy rate,
-// 57 us with the keys' rotation and 40 without, of which the waits of a CTA's four steps - rows, maximum, scale, bytes -
-// are most); few tokens by latency: the chain of sequence, length, page, rows and scale is 4.7 us for 64 tokens of 64
-// sequences. So:
+// 55.5 us with the keys' rotation and 38 without, most of it the waits of a CTA's steps: rows, maximum, bytes); few tokens
+// by latency: the chain of sequence, page, rows and scale is 4.7 us for 64 tokens of 64 sequences. So:
 // - few rows (up to kRowsFew a page): a unit is at most a warp's, and a CTA takes many units. 153 tokens of 37 sequences,
-//   9 at most: 6.1 us, and 8.1 with a CTA a unit.
+//   9 at most: 6.0 us, and 8.1 with a CTA a unit.
 // - many rows: the whole CTA is the team, rows side by side, up to four heads one after the other, which share their
-//   tokens' sines.
+//   tokens' sines (with two heads 62 us with the rotation and 38 without, with eight 54.5 and 45).
 // - a page that holds older rows and whose scale grows: all its older rows are rounded again by the whole CTA, whoever's
 //   unit it is. It happens to few units at a time: 10.2 us where one head of 16 grows (64 tokens, pages of 64 with 60
 //   older rows, memory cold), 22.5 when the unit's team does it alone, 10.2 without growth.
@@ -603,9 +602,8 @@ cudaError_t launch_kv_append(const KvGeom& g, const KvBatchView& b, const sixi_k
     if (rows <= kRowsFew)
         for (a.team = a.row_lanes; a.team < 32u && a.team / a.row_lanes * kRowsHeld < rows;) a.team *= 2;
     const uint32_t teams = kNT / a.team;
-    // A CTA's way to its rows is a chain of lookups (sequence, length, page: some 3 us), and the sines of a page's tokens
-    // are the same for every head. So with a team of the whole CTA it takes up to four heads one after the other, while
-    // that leaves enough CTAs for the GPU.
+    // A CTA's way to its rows is a chain of lookups, and the sines of a page's tokens are the same for every head. So with
+    // a team of the whole CTA it takes up to four heads one after the other, while that leaves enough CTAs for the GPU.
     const uint32_t items = b.n_tokens / g.page_size + 2u * b.n_seqs;
     a.heads = 0;
     if (a.team == kNT) {

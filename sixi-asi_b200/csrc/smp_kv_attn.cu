@@ -4,7 +4,13 @@
 // One pass over the cached bytes with the running maximum and sum of a softmax. A CTA works on up to 16
 // query rows of one key head at a time (the query heads that share it, times new tokens), so a cached
 // byte is brought in once for all of them; 64-token tiles of keys and values are double-buffered in
-// shared memory by 16-byte asynchronous copies and widened to fp32 where they are used.
+// shared memory by 16-byte asynchronous copies and widened to fp32 where they are used. Scores: a thread
+// takes one token and four rows; values: four elements of a head and every groups-th token.
+//
+// The work is cut over two CTAs per SM as smp_kv.cuh describes. fp32 products have no tensor-core form that
+// keeps 24 bits, so the bound is the fp32 pipes and the shared-memory reads that feed them, and for small
+// calls the chain of steps of a tile: 15 tokens of 6 sequences, up to 3,000 cached ones, 21 heads of 80
+// elements on 3: 39 us (the bytes alone would take 0.4 us at the copy rate).
 #include <cuda_runtime.h>
 
 #include "smp_kernels.cuh"
@@ -84,7 +90,6 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, const Smem& sm, con
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
-template <typename T>
 __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ unsigned long long scratch[kNT / 32 + 2];
@@ -128,16 +133,15 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         load_ids(a, pc, lo, pc.t0, ids);
         __syncthreads();
         load_tile(a, sm, pc, lo, pc.t0, 0, ids);
-        // queries, turned and rounded to their type, then scaled; a NaN or Inf makes the row NaN
+        // queries, turned, then scaled; a NaN or Inf makes the row NaN
         for (uint32_t i = tid; i < kRt * D; i += kNT) {
             const uint32_t r = i / D, d = i - r * D;
             float x = 0.0f;
             if (r < pc.rows) {
                 const uint32_t tok = (r_base + r) / a.shape.group, g = (r_base + r) - tok * a.shape.group;
-                const T* p = static_cast<const T*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                const float* p = static_cast<const float*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
                              (pc.head * a.shape.group + g) * a.q.head_stride;
-                load_turned<T, 1>(a.rope, p, d, pc.plan.p0 + static_cast<int32_t>(tok), &x);
-                if constexpr (sizeof(T) == 2) x = __bfloat162float(__float2bfloat16_rn(x));
+                load_turned<float, 1>(a.rope, p, d, pc.plan.p0 + static_cast<int32_t>(tok), &x);
                 x = fabsf(x) < __builtin_huge_valf() ? x * (a.scale * kLog2e) : __uint_as_float(0x7FC00000u);
             }
             sm.q[i] = x;
@@ -274,10 +278,9 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
                 if (whole) {
                     const uint32_t rr = r_base + rb + r, tok = rr / a.shape.group, g = rr - tok * a.shape.group;
                     const float l = sm.l[rb + r];
-                    T* p = static_cast<T*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
+                    float* p = static_cast<float*>(a.out.data) + (pc.plan.row0 + tok) * a.out.token_stride +
                            (pc.head * a.shape.group + g) * a.out.head_stride + d;
-                    const float y = l == 0.0f ? 0.0f : o / l;
-                    store_vec<T, 1>(p, &y);
+                    *p = l == 0.0f ? 0.0f : o / l;
                 } else {
                     part[(rb + r) * D + d] = o;
                 }
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         if (!last_flag) continue;
         __threadfence();
         // the last CTA of the unit joins the pieces
-        join_rows<T, 2>(a, a.part + (2ull * c0 + 1u) * a.part_stride, a.part + 2ull * c0 * a.part_stride, c1 - c0 + 1u,
+        join_rows<float, 2>(a, a.part + (2ull * c0 + 1u) * a.part_stride, a.part + 2ull * c0 * a.part_stride, c1 - c0 + 1u,
                         pc.rows, r_base, pc.plan.row0, pc.head, tid >> 5);
     }
 }
@@ -323,11 +326,10 @@ cudaError_t launch_attend_f32(AttnArgs a, uint32_t n_sms, cudaStream_t stream) {
     const uint32_t D = a.g.head_dim;
     const size_t smem = sizeof(float) * (static_cast<size_t>(kRt) * D + 4u * kT * (D + 16u) / 4u + 4u * kT + 2u * kRt * kT +
                                          4096u + 3u * kRt);
-    auto fn = attend_f32_kernel<float>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(attend_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     const uint32_t ctas = 2u * n_sms < kAttnMaxCtas ? 2u * n_sms : kAttnMaxCtas;
-    fn<<<ctas, kNT, smem, stream>>>(a);
+    attend_f32_kernel<<<ctas, kNT, smem, stream>>>(a);
     return cudaGetLastError();
 }
 

@@ -32,6 +32,16 @@
 // softmax groups that take the tiles in turn, each with its own running maximum, and of the last 4 three stage
 // queries (turned, split) and one walks the work and checks page tables. A tile's softmax is a chain of waits; two or three
 // at a time, with the scores of the next ready before one ends, hide it.
+//
+// Bound and measured (one B200, bytes at its copy rate of 6.54 TB/s, products at 1.65 PFLOP/s):
+//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 115 us, 5.3 TB/s (82 % of the copy rate)
+//   2 sequences, one token, up to 262,144 cached, 32 on 4 of 128:       93 us, 5.6 TB/s (85 %)
+//   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         190 us; 26 us of bytes
+//   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       840 us; 163 us of products
+//   one token over 700 cached, 32 on 8 of 128:                          14 us, a chain of waits
+// With few rows memory is the bound. With 64 rows a tile it is the softmax's chain of waits for scores, barriers and
+// weights: 37 % of the issue slots, 25 % of the ALU and 16 % of the tensor pipe are busy. A tile of the sizes above holds
+// R x 128 exponentials and as many roundings to two e4m3 terms, about ten operations each.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -78,6 +88,7 @@ struct Cfg {
     static constexpr uint32_t kColsUsed = G * 2u * R * (1u + DC);  // scores and outputs, hi and lo, one of each a group
     static constexpr uint32_t kTmem = kColsUsed <= 64 ? 64u : (kColsUsed <= 128 ? 128u : (kColsUsed <= 256 ? 256u : 512u));
     static_assert(kNK >= 2 && kNV >= 2 && kColsUsed <= 512, "does not fit");
+    static_assert(kRing > kNK && kRing > kNV, "a waiter's phase could come round again");
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -618,134 +629,134 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             return &sh.piece[np % kPieces];
         };
         if (warp < 4) {
-        set_regs<C::kRegsIssue, C::kRegsLaunch>();
-        if (warp == 0 || warp == 3) {
-            // ---- pages: warp 0 copies the keys', warp 3 the values' and both's scales; a lane a page ----
-            const bool is_v = warp == 3;
-            const uint32_t ppt = args.pages_per_tile, n_buf = is_v ? NV : NK;
-            const uint32_t none = a.g.n_pages * a.g.n_heads;  // a coordinate past the end: zeros
-            const uint32_t slot = lane & 7u, window_mask = 32u / ppt - 1u;
-            const CUtensorMap* map = is_v ? &v_map : &k_map;
-            uint8_t* buf = is_v ? vbuf : kbuf;
-            uint64_t* full = is_v ? sh.vfull : sh.kfull;
-            uint64_t* done = is_v ? sh.ofull : sh.sfull;  // of tile n - n_buf: its buffer is free
-            // pages that one row tile reads once leave L2 first: partial results and queries stay
-            uint64_t policy;
-            if (args.read_once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-            else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
-            uint32_t n = 0, st = 0;
-            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
-                const PieceRec& pc = *rec;
-                const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
-                const uint32_t n_pg = (static_cast<uint32_t>(pc.len) + a.g.page_size - 1u) >> shift, head = pc.head;
-                uint32_t lo_pg = 0;  // pages wholly before the window of the unit's first row are not read
-                if (a.shape.window) {
-                    const int32_t lo = pc.p0 + static_cast<int32_t>(pc.row_tile * a.shape.rt / a.shape.group) -
-                                       static_cast<int32_t>(a.shape.window) + 1;
-                    lo_pg = lo > 0 ? static_cast<uint32_t>(lo) >> shift : 0u;
-                }
-                // 32 page ids at a time, the next 32 asked for before they are needed
-                const uint32_t tiles = static_cast<uint32_t>(pc.t1 - pc.t0);
-                uint32_t idx = static_cast<uint32_t>(pc.t0) * ppt + lane;
-                int32_t ids = -1, ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
-                for (uint32_t i = 0; i < tiles; ++i, ++n) {
-                    const uint32_t in = i & window_mask;
-                    if (in == 0) {
-                        ids = ids_next;
-                        idx += 32u;
-                        ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
+            set_regs<C::kRegsIssue, C::kRegsLaunch>();
+            if (warp == 0 || warp == 3) {
+                // ---- pages: warp 0 copies the keys', warp 3 the values' and both's scales; a lane a page ----
+                const bool is_v = warp == 3;
+                const uint32_t ppt = args.pages_per_tile, n_buf = is_v ? NV : NK;
+                const uint32_t none = a.g.n_pages * a.g.n_heads;  // a coordinate past the end: zeros
+                const uint32_t slot = lane & 7u, window_mask = 32u / ppt - 1u;
+                const CUtensorMap* map = is_v ? &v_map : &k_map;
+                uint8_t* buf = is_v ? vbuf : kbuf;
+                uint64_t* full = is_v ? sh.vfull : sh.kfull;
+                uint64_t* done = is_v ? sh.ofull : sh.sfull;  // of tile n - n_buf: its buffer is free
+                // pages that one row tile reads once leave L2 first: partial results and queries stay
+                uint64_t policy;
+                if (args.read_once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+                else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+                uint32_t n = 0, st = 0;
+                for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                    const PieceRec& pc = *rec;
+                    const int32_t* table = a.b.page_table + pc.seq * a.b.table_stride;
+                    const uint32_t n_pg = (static_cast<uint32_t>(pc.len) + a.g.page_size - 1u) >> shift, head = pc.head;
+                    uint32_t lo_pg = 0;  // pages wholly before the window of the unit's first row are not read
+                    if (a.shape.window) {
+                        const int32_t lo = pc.p0 + static_cast<int32_t>(pc.row_tile * a.shape.rt / a.shape.group) -
+                                           static_cast<int32_t>(a.shape.window) + 1;
+                        lo_pg = lo > 0 ? static_cast<uint32_t>(lo) >> shift : 0u;
                     }
-                    const int32_t id = __shfl_sync(kFull, ids, in * ppt + (slot & (ppt - 1u)));
-                    const bool good = static_cast<uint32_t>(id) < a.g.n_pages;
-                    const uint32_t z = good ? static_cast<uint32_t>(id) * a.g.n_heads + head : none;
-                    if (n >= n_buf) bar_wait(&done[(n - n_buf) % kRing], ((n - n_buf) / kRing) & 1u, gave_up);
-                    if (__any_sync(kFull, *gave_up != 0u)) break;
-                    if (lane == 0) bar_expect(&full[st], C::kBuf);
-                    __syncwarp();
-                    if (lane < ppt) {
-#pragma unroll
-                        for (int c = 0; c < DC; ++c)
-                            tma_page(map, buf + st * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &full[st], c * 128, z, policy);
-                    }
-                    if (is_v) {
-                        if (lane >= 16u) {
-                            const float* src = (lane >= 24u ? a.g.v_scales : a.g.k_scales) + (good ? z : 0u);
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                             s32(lane >= 24u ? &sh.vscale[st][slot] : &sh.kscale[st][slot])),
-                                         "l"(src), "r"(good ? 4u : 0u)
-                                         : "memory");
+                    // 32 page ids at a time, the next 32 asked for before they are needed
+                    const uint32_t tiles = static_cast<uint32_t>(pc.t1 - pc.t0);
+                    uint32_t idx = static_cast<uint32_t>(pc.t0) * ppt + lane;
+                    int32_t ids = -1, ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
+                    for (uint32_t i = 0; i < tiles; ++i, ++n) {
+                        const uint32_t in = i & window_mask;
+                        if (in == 0) {
+                            ids = ids_next;
+                            idx += 32u;
+                            ids_next = idx < n_pg && idx >= lo_pg ? table[idx] : -1;
                         }
-                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.scfull[st])) : "memory");
+                        const int32_t id = __shfl_sync(kFull, ids, in * ppt + (slot & (ppt - 1u)));
+                        const bool good = static_cast<uint32_t>(id) < a.g.n_pages;
+                        const uint32_t z = good ? static_cast<uint32_t>(id) * a.g.n_heads + head : none;
+                        if (n >= n_buf) bar_wait(&done[(n - n_buf) % kRing], ((n - n_buf) / kRing) & 1u, gave_up);
+                        if (__any_sync(kFull, *gave_up != 0u)) break;
+                        if (lane == 0) bar_expect(&full[st], C::kBuf);
+                        __syncwarp();
+                        if (lane < ppt) {
+#pragma unroll
+                            for (int c = 0; c < DC; ++c)
+                                tma_page(map, buf + st * C::kBuf + c * C::kChunk + slot * a.g.page_size * 128u, &full[st], c * 128, z, policy);
+                        }
+                        if (is_v) {
+                            if (lane >= 16u) {
+                                const float* src = (lane >= 24u ? a.g.v_scales : a.g.k_scales) + (good ? z : 0u);
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                                                 s32(lane >= 24u ? &sh.vscale[st][slot] : &sh.kscale[st][slot])),
+                                             "l"(src), "r"(good ? 4u : 0u)
+                                             : "memory");
+                            }
+                            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(&sh.scfull[st])) : "memory");
+                        }
+                        if (++st == n_buf) st = 0;
                     }
-                    if (++st == n_buf) st = 0;
+                }
+                if (*gave_up) {  // the copies in flight land before the shared memory is given back
+                    for (uint32_t i = n > n_buf ? n - n_buf : 0u; i < n; ++i)
+                        for (uint32_t w = 0; w < kWaitIters && !bar_try(&full[i % n_buf], (i / n_buf) & 1u); ++w) {}
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                }
+            } else if (warp == 1) {
+                // ---- scores: hi and lo rows of the queries are one operand of 2 R rows ----
+                const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
+                const uint32_t ksteps = (D + 31u) / 32u;
+                const uint64_t k_desc = desc_sw128(s32(kbuf)), q_desc = desc_sw128(s32(qbuf));
+                uint32_t n = 0;
+                for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                    const PieceRec& pc = *rec;
+                    const uint32_t qb = np % NQ;
+                    bar_wait(&sh.qfull[qb], (np / NQ) & 1u, gave_up);
+                    for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
+                        const uint32_t ks = n % NK, b = n % G;
+                        bar_wait(&sh.kfull[ks], (n / NK) & 1u, gave_up);
+                        if (n >= G) bar_wait(&sh.sempty[b], (n / G - 1u) & 1u, gave_up);
+                        tc_after();
+                        if (__any_sync(kFull, *gave_up != 0u)) continue;
+                        const uint64_t kd = k_desc + ks * (C::kBuf >> 4), qd = q_desc + qb * (C::kQ >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4 * DC; ++k)
+                                if (static_cast<uint32_t>(k) < ksteps)
+                                    mma_f8(tmem + b * 2u * R, kd + (((k >> 2) * C::kChunk + (k & 3) * 32u) >> 4),
+                                           qd + (((k >> 2) * (2u * R * 128u) + (k & 3) * 32u) >> 4), idesc, k > 0);
+                        }
+                        __syncwarp();
+                        if (elect_one()) {
+                            tc_commit(&sh.sfull[n % kRing]);
+                            if (t + 1 == pc.t1) tc_commit(&sh.qempty[qb]);
+                        }
+                        __syncwarp();
+                    }
+                }
+            } else {
+                // ---- outputs: hi and lo columns of the weights are one operand of 2 R columns ----
+                const uint32_t idesc = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
+                const uint64_t v_desc = desc_sw128(s32(vbuf)), w_desc = desc_plain(s32(wbuf), 128u, 16u * kTile);
+                uint32_t n = 0;
+                for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                    const PieceRec& pc = *rec;
+                    for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
+                        const uint32_t vs = n % NV, b = n % G;
+                        bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
+                        // (the softmax has waited for the output buffer to be free)
+                        bar_wait(&sh.wfull[b], (n / G) & 1u, gave_up);
+                        tc_after();
+                        if (__any_sync(kFull, *gave_up != 0u)) continue;
+                        const uint64_t vd = v_desc + vs * (C::kBuf >> 4), wd = w_desc + b * (C::kW >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int c = 0; c < DC; ++c)
+#pragma unroll
+                                for (int k = 0; k < kTile / 32; ++k)
+                                    mma_f8(tmem + G * 2u * R + (b * DC + c) * 2u * R, vd + ((c * C::kChunk + k * 4096u) >> 4),
+                                           wd + ((k * 512u) >> 4), idesc, k > 0);
+                        }
+                        __syncwarp();
+                        if (elect_one()) tc_commit(&sh.ofull[n % kRing]);
+                        __syncwarp();
+                    }
                 }
             }
-            if (*gave_up) {  // the copies in flight land before the shared memory is given back
-                for (uint32_t i = n > n_buf ? n - n_buf : 0u; i < n; ++i)
-                    for (uint32_t w = 0; w < kWaitIters && !bar_try(&full[i % n_buf], (i / n_buf) & 1u); ++w) {}
-                asm volatile("cp.async.wait_all;" ::: "memory");
-            }
-        } else if (warp == 1) {
-            // ---- scores: hi and lo rows of the queries are one operand of 2 R rows ----
-            const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
-            const uint32_t ksteps = (D + 31u) / 32u;
-            const uint64_t k_desc = desc_sw128(s32(kbuf)), q_desc = desc_sw128(s32(qbuf));
-            uint32_t n = 0;
-            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
-                const PieceRec& pc = *rec;
-                const uint32_t qb = np % NQ;
-                bar_wait(&sh.qfull[qb], (np / NQ) & 1u, gave_up);
-                for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t ks = n % NK, b = n % G;
-                    bar_wait(&sh.kfull[ks], (n / NK) & 1u, gave_up);
-                    if (n >= G) bar_wait(&sh.sempty[b], (n / G - 1u) & 1u, gave_up);
-                    tc_after();
-                    if (__any_sync(kFull, *gave_up != 0u)) continue;
-                    const uint64_t kd = k_desc + ks * (C::kBuf >> 4), qd = q_desc + qb * (C::kQ >> 4);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 0; k < 4 * DC; ++k)
-                            if (static_cast<uint32_t>(k) < ksteps)
-                                mma_f8(tmem + b * 2u * R, kd + (((k >> 2) * C::kChunk + (k & 3) * 32u) >> 4),
-                                       qd + (((k >> 2) * (2u * R * 128u) + (k & 3) * 32u) >> 4), idesc, k > 0);
-                    }
-                    __syncwarp();
-                    if (elect_one()) {
-                        tc_commit(&sh.sfull[n % kRing]);
-                        if (t + 1 == pc.t1) tc_commit(&sh.qempty[qb]);
-                    }
-                    __syncwarp();
-                }
-            }
-        } else {
-            // ---- outputs: hi and lo columns of the weights are one operand of 2 R columns ----
-            const uint32_t idesc = (1u << 4) | (1u << 15) | (1u << 16) | (static_cast<uint32_t>(R >> 2) << 17) | (8u << 24);
-            const uint64_t v_desc = desc_sw128(s32(vbuf)), w_desc = desc_plain(s32(wbuf), 128u, 16u * kTile);
-            uint32_t n = 0;
-            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
-                const PieceRec& pc = *rec;
-                for (int32_t t = pc.t0; t < pc.t1; ++t, ++n) {
-                    const uint32_t vs = n % NV, b = n % G;
-                    bar_wait(&sh.vfull[vs], (n / NV) & 1u, gave_up);
-                    // (the softmax has waited for the output buffer to be free)
-                    bar_wait(&sh.wfull[b], (n / G) & 1u, gave_up);
-                    tc_after();
-                    if (__any_sync(kFull, *gave_up != 0u)) continue;
-                    const uint64_t vd = v_desc + vs * (C::kBuf >> 4), wd = w_desc + b * (C::kW >> 4);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int c = 0; c < DC; ++c)
-#pragma unroll
-                            for (int k = 0; k < kTile / 32; ++k)
-                                mma_f8(tmem + G * 2u * R + (b * DC + c) * 2u * R, vd + ((c * C::kChunk + k * 4096u) >> 4),
-                                       wd + ((k * 512u) >> 4), idesc, k > 0);
-                    }
-                    __syncwarp();
-                    if (elect_one()) tc_commit(&sh.ofull[n % kRing]);
-                    __syncwarp();
-                }
-            }
-        }
         } else if (warp < 8) {
             set_regs<C::kRegsOut, C::kRegsLaunch>();
             // ---- output sums: thread d of a chunk holds element d of every row ----
@@ -1159,53 +1170,53 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             }
             if (grp == 0) join_pieces<DC>(a, sh, warp - 4u);
         } else {
-        set_regs<C::kRegsHelp, C::kRegsLaunch>();
-        if (warp == C::kThreads / 32 - 1) {
-            // ---- the walk: pieces are published ahead of the roles ----
-            for (uint32_t np = 1; sh.piece[(np - 1u) % kPieces].rows != 0u; ++np) {
-                Piece pc;
-                const bool any = next_piece(a.shape, a.b, shift, walk, &pc);
-                volatile uint32_t* done = &sh.pieces_done;
-                for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i)
-                    __nanosleep(i < kSleepAfter ? 64u : 4u * kSleepNs);
-                __syncwarp();
-                if (__any_sync(kFull, np - *done > 12u)) break;  // (given up)
-                if (lane == 0) {
-                    sh.piece[np % kPieces] = rec_of(any, pc);
-                    bar_arrive(&sh.pfull[np % kPieces]);
-                }
-                // the piece's queries into L2: while the pages stream in, a load from memory takes some 5 us
-                if (any)
-                    for (uint32_t i = lane; i < pc.rows * 4u; i += 32u) {
-                        const uint32_t rr = pc.row_tile * a.shape.rt + (i >> 2), tok = rr / a.shape.group;
-                        const uint32_t d = min((i & 3u) * 64u, D - 1u);
-                        const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
-                                                 (pc.head * a.shape.group + rr - tok * a.shape.group) * a.q.head_stride + d;
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+            set_regs<C::kRegsHelp, C::kRegsLaunch>();
+            if (warp == C::kThreads / 32 - 1) {
+                // ---- the walk: pieces are published ahead of the roles ----
+                for (uint32_t np = 1; sh.piece[(np - 1u) % kPieces].rows != 0u; ++np) {
+                    Piece pc;
+                    const bool any = next_piece(a.shape, a.b, shift, walk, &pc);
+                    volatile uint32_t* done = &sh.pieces_done;
+                    for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i)
+                        __nanosleep(i < kSleepAfter ? 64u : 4u * kSleepNs);
+                    __syncwarp();
+                    if (__any_sync(kFull, np - *done > 12u)) break;  // (given up)
+                    if (lane == 0) {
+                        sh.piece[np % kPieces] = rec_of(any, pc);
+                        bar_arrive(&sh.pfull[np % kPieces]);
                     }
-                __syncwarp();
-            }
-        } else {
-            // ---- queries: of the pieces after the first ----
-            const uint32_t h = warp - (8u + 4u * G);
-            for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
-                if (kHelp == 1 && np % 3u != h) continue;
-                const uint32_t qb = np % NQ, rs = np % kQSlots;
-                constexpr int kU = R == 16 ? 4 : 3;
-                const uint32_t at = kHelp == 1 ? 0u : h;
-                uint4 raw[kU];
-                if (np > 0) fetch_queries<DC, kU>(args, *rec, at * (2u / DC), kHelp, raw);
-                if (np >= NQ) bar_wait(&sh.qempty[qb], (np / NQ - 1u) & 1u, gave_up);
-                if (np > 0)
-                    stage_queries<R, DC, NB, G, kU>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], at, kHelp,
-                                                    sh.sines[h], raw);
-                __syncwarp();
-                if (lane == 0) {
-                    bar_arrive(&sh.qfull[qb]);
-                    bar_arrive(&sh.rfull[rs]);
+                    // the piece's queries into L2: while the pages stream in, a load from memory takes some 5 us
+                    if (any)
+                        for (uint32_t i = lane; i < pc.rows * 4u; i += 32u) {
+                            const uint32_t rr = pc.row_tile * a.shape.rt + (i >> 2), tok = rr / a.shape.group;
+                            const uint32_t d = min((i & 3u) * 64u, D - 1u);
+                            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                                                     (pc.head * a.shape.group + rr - tok * a.shape.group) * a.q.head_stride + d;
+                            asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+                        }
+                    __syncwarp();
+                }
+            } else {
+                // ---- queries: of the pieces after the first ----
+                const uint32_t h = warp - (8u + 4u * G);
+                for (uint32_t np = 0; const PieceRec* rec = piece(np); ++np) {
+                    if (kHelp == 1 && np % 3u != h) continue;
+                    const uint32_t qb = np % NQ, rs = np % kQSlots;
+                    constexpr int kU = R == 16 ? 4 : 3;
+                    const uint32_t at = kHelp == 1 ? 0u : h;
+                    uint4 raw[kU];
+                    if (np > 0) fetch_queries<DC, kU>(args, *rec, at * (2u / DC), kHelp, raw);
+                    if (np >= NQ) bar_wait(&sh.qempty[qb], (np / NQ - 1u) & 1u, gave_up);
+                    if (np > 0)
+                        stage_queries<R, DC, NB, G, kU>(args, *rec, qbuf + qb * C::kQ, sh.frow[rs], sh.qpos[rs], at, kHelp,
+                                                        sh.sines[h], raw);
+                    __syncwarp();
+                    if (lane == 0) {
+                        bar_arrive(&sh.qfull[qb]);
+                        bar_arrive(&sh.rfull[rs]);
+                    }
                 }
             }
-        }
         }
     }
     if (warp == C::kThreads / 32 - 1) {
