@@ -516,20 +516,21 @@ __device__ __forceinline__ float kv_ex2(float x) {
 
 // Eight warps (w: 0 to 7) join a unit's n pieces in CTA order: piece 0 is its CTA's last result (first), the others are
 // their CTAs' first ones (rest + 2 c results on). Rows of `rt`-row results; row r goes to query token
-// (row_base + r) / group of row0 on. DC: 128-element chunks of a head.
-template <typename T, int DC>
+// (row_base + r) / group of row0 on. DC: 128-element chunks of a head; U rows at a time, the loads of kAhead pieces in
+// flight: a round is a chain of loads, so units of many rows (and then few pieces) take more rows at a time.
+template <typename T, int DC, int U, int kAhead>
 __device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first, const float* rest, uint32_t n, uint32_t rows,
                                           uint32_t row_base, int64_t row0, uint32_t head, uint32_t w) {
-    constexpr int kAhead = DC == 1 ? 4 : 2;  // pieces whose loads are in flight
     const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
     const auto piece_of = [&](uint32_t c) { return c == 0 ? first : rest + 2ull * c * a.part_stride; };
-    // a warp a row, four elements a lane, two rows at a time; a lane holds the factor of a piece (of every 32nd)
-    for (uint32_t r0 = w; r0 < rows; r0 += 16u) {
-        const uint32_t row[2] = {r0, min(r0 + 8u, rows - 1u)};
-        float m[2], l[2], f[2], norm[2];
-        float4 o[2][DC], v[2][DC][kAhead];
+    // a warp a row, four elements a lane, U rows at a time; a lane holds the factor of a piece (of every 32nd)
+    for (uint32_t r0 = w; r0 < rows; r0 += 8u * U) {
+        uint32_t row[U];
+        float m[U], l[U], f[U], norm[U];
+        float4 o[U][DC], v[U][DC][kAhead];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
+            row[u] = min(r0 + 8u * u, rows - 1u);
             m[u] = kNegInf, l[u] = 0.0f;
 #pragma unroll
             for (int k = 0; k < DC; ++k) o[u][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -537,7 +538,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first,
         // (the first pieces' sums are on their way before the factors are known)
         const auto fetch = [&](uint32_t c) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int k = 0; k < DC; ++k)
 #pragma unroll
@@ -549,15 +550,15 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first,
         fetch(0);
         for (uint32_t c = lane; c < n; c += 32u)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __ldcg(piece_of(c) + a.shape.rt * D + row[u]));
+            for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __ldcg(piece_of(c) + a.shape.rt * D + row[u]));
 #pragma unroll
         for (int o2 = 16; o2 > 0; o2 >>= 1)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o2));
+            for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xFFFFFFFFu, m[u], o2));
         for (uint32_t c0l = 0; c0l < n; c0l += 32u) {
             const uint32_t c = c0l + lane;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 f[u] = 0.0f;
                 if (c < n) {
                     const float* p = piece_of(c) + a.shape.rt * D + row[u];
@@ -570,7 +571,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first,
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < U; ++u) {
                         const float g = __shfl_sync(0xFFFFFFFFu, f[u], i0 + i);  // (0 past the last piece)
 #pragma unroll
                         for (int k = 0; k < DC; ++k) {
@@ -585,10 +586,10 @@ __device__ __forceinline__ void join_rows(const AttnArgs& a, const float* first,
 #pragma unroll
         for (int o2 = 16; o2 > 0; o2 >>= 1)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], o2);
+            for (int u = 0; u < U; ++u) l[u] += __shfl_xor_sync(0xFFFFFFFFu, l[u], o2);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (u == 1 && r0 + 8u >= rows) continue;
+        for (int u = 0; u < U; ++u) {
+            if (r0 + 8u * u >= rows) continue;
             norm[u] = l[u] == 0.0f ? 0.0f : 1.0f / l[u];
             const uint32_t rr = row_base + row[u], tok = rr / a.shape.group;
             const uint32_t hq = head * a.shape.group + rr - tok * a.shape.group;

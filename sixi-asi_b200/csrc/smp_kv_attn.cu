@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         if (!last_flag) continue;
         __threadfence();
         // the last CTA of the unit joins the pieces
-        join_rows<float, 2>(a, a.part + (2ull * c0 + 1u) * a.part_stride, a.part + 2ull * c0 * a.part_stride, c1 - c0 + 1u,
+        join_rows<float, 2, 2, 2>(a, a.part + (2ull * c0 + 1u) * a.part_stride, a.part + 2ull * c0 * a.part_stride, c1 - c0 + 1u,
                         pc.rows, r_base, pc.plan.row0, pc.head, tid >> 5);
     }
 }

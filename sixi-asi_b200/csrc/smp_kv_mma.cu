@@ -508,7 +508,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
 // Units that were cut: the last of their CTAs to arrive joins the pieces, in CTA order. The output's four warps and
 // four of the softmax's do it (w: 0 to 7) after all of this CTA's own tiles, so that nothing of it waits for the
 // joining.
-template <int DC, typename Sh>
+template <int R, int DC, typename Sh>
 __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, uint32_t w) {
     const uint32_t lane = threadIdx.x & 31u;
     __threadfence();
@@ -537,7 +537,7 @@ __device__ __forceinline__ void join_pieces(const AttnArgs& a, Sh& sh, uint32_t 
         const uint32_t n = place_owner(pc.start + static_cast<uint64_t>(pc.end - pc.first) - 1u, sh.total, sh.ctas) - c0 + 1u;
         const float* first = a.part + (2ull * c0 + 1u) * a.part_stride;       // the piece of c0 is its CTA's last
         const float* rest = a.part + (2ull * c0) * a.part_stride;             // the others' are their CTA's first
-        join_rows<__nv_bfloat16, DC>(a, first, rest, n, pc.rows, pc.row_tile * a.shape.rt, pc.row0, pc.head, w);
+        join_rows<__nv_bfloat16, DC, R == 16 ? 2 : 4, R == 16 ? 4 / DC : 2 / DC>(a, first, rest, n, pc.rows, pc.row_tile * a.shape.rt, pc.row0, pc.head, w);
     }
 }
 
@@ -917,7 +917,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 __syncwarp();
                 if (warp == 4 && lane == 0) *const_cast<volatile uint32_t*>(&sh.pieces_done) = np + 1u;
             }
-            join_pieces<DC>(a, sh, warp - 4u);
+            join_pieces<R, DC>(a, sh, warp - 4u);
         } else if (warp < 8 + 4 * G) {
             set_regs<C::kRegsSoft, C::kRegsLaunch>();
             // ---- softmax: group g takes the tiles n with n % G == g ----
@@ -1168,7 +1168,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&sh.lfull);
             }
-            if (grp == 0) join_pieces<DC>(a, sh, warp - 4u);
+            if (grp == 0) join_pieces<R, DC>(a, sh, warp - 4u);
         } else {
             set_regs<C::kRegsHelp, C::kRegsLaunch>();
             if (warp == C::kThreads / 32 - 1) {
