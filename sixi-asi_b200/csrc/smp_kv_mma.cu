@@ -57,8 +57,7 @@ constexpr int kTile = 128;      // tokens of a tile
 constexpr int kTileShift = 7;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kWaitIters = 1u << 22;  // bound of every wait: a second and more (never expected to run out)
-constexpr uint32_t kSleepAfter = 1u << 12, kSleepNs = 256;
+constexpr uint32_t kWaitIters = 1u << 24;  // bound of a wait: a tenth of a second at the least (never expected to run out)
 constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
 constexpr uint32_t kPieces = 16; // piece records kept; the walk stays 12 ahead of the output at most
 constexpr int kQSlots = 16;  // pieces whose row records are kept: softmax lags the staging by fewer than 10
@@ -121,10 +120,7 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
 __device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, volatile uint32_t* gave_up) {
     if (!bar_try(b, parity)) {
         bool ok = false;
-        for (uint32_t i = 0; i < kWaitIters && !ok; ++i) {
-            ok = bar_try(b, parity) || *gave_up != 0u;
-            if (!ok && i >= kSleepAfter) __nanosleep(kSleepNs);  // (what waits for a whole piece may wait long)
-        }
+        for (uint32_t i = 0; i < kWaitIters && !ok; ++i) ok = bar_try(b, parity) || *gave_up != 0u;
         if (!ok) *gave_up = 1u;
     }
     __syncwarp();
@@ -340,6 +336,7 @@ struct MmaArgs {
     AttnArgs a;
     uint32_t pages_per_tile;
     uint32_t read_once;  // no page is read by more than one row tile
+    uint32_t out_pair;   // two elements of an output row can be stored together
     uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
 };
 
@@ -867,6 +864,28 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     }
                     __syncwarp();
                     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out.data) + d0;
+                    if (R == 16 && args.out_pair) {
+                        // Two neighbours of a warp exchange halves of two rows: each stores two elements of one row. For small
+                        // tiles only (64 sequences of one token: 113.6 us without, 111.2 with it): in the larger ones, which
+                        // are bound by fetching instructions, the second form costs more than it saves (809 against 841 us
+                        // for chunks of 32 rows of 256 elements).
+                        const uint32_t odd = lane & 1u, sel = odd ? 0x3276u : 0x5410u;
+                        out -= odd;
+#pragma unroll
+                        for (int col = 0; col < R; col += 2) {
+                            if (row_of<V>(col) >= 8u * NB) continue;
+                            const float2 inv = *reinterpret_cast<const float2*>(facold + col);
+                            const uint64_t at = sh.row_at[quad][col + odd];
+                            const bool on = row_of<V>(col) + odd < rows;
+#pragma unroll
+                            for (int c = 0; c < DC; ++c) {
+                                const float2 y = un2(mul2(acc[c][col / 2], f2(inv.x, inv.y)));
+                                const uint32_t two = bf16x2_bits(y.x, y.y);
+                                const uint32_t w = __byte_perm(two, __shfl_xor_sync(kFull, two, 1), sel);
+                                if (on && c * 128u + d0 < D) *reinterpret_cast<uint32_t*>(out + at + c * 128u) = w;
+                            }
+                        }
+                    } else
                     // (four columns at a time: their places and factors are read together, the stores are predicated)
 #pragma unroll
                     for (int col = 0; col < R; col += 4) {
@@ -1178,7 +1197,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     const bool any = next_piece(a.shape, a.b, shift, walk, &pc);
                     volatile uint32_t* done = &sh.pieces_done;
                     for (uint32_t i = 0; i < kWaitIters && np - *done > 12u && *gave_up == 0u; ++i)
-                        __nanosleep(i < kSleepAfter ? 64u : 4u * kSleepNs);
+                        __nanosleep(64);
                     __syncwarp();
                     if (__any_sync(kFull, np - *done > 12u)) break;  // (given up)
                     if (lane == 0) {
@@ -1317,6 +1336,7 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
                       rope_by_8(a.rope)
                   ? 1u
                   : 0u;
+    m.out_pair = ((reinterpret_cast<uintptr_t>(a.out.data) | 2u * a.out.token_stride | 2u * a.out.head_stride) & 3u) == 0 ? 1u : 0u;
     const uint64_t rows = static_cast<uint64_t>(max_new ? max_new : 1u) * a.shape.group;
     // rows of a row tile: what deals `rows` out evenly, in the blocks of 8 rows that the softmax works in (72 rows
     // are 40 and 32, not 64 and 8)
