@@ -34,14 +34,14 @@
 // at a time, with the scores of the next ready before one ends, hide it.
 //
 // Bound and measured (one B200, bytes at its copy rate of 6.54 TB/s, products at 1.65 PFLOP/s):
-//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 115 us, 5.3 TB/s (82 % of the copy rate)
+//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 112 us, 5.5 TB/s (84 % of the copy rate)
 //   2 sequences, one token, up to 262,144 cached, 32 on 4 of 128:       93 us, 5.6 TB/s (85 %)
-//   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         190 us; 26 us of bytes
-//   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       840 us; 163 us of products
+//   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         177 to 190 us; 26 us of bytes
+//   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       790 to 810 us; 163 us of products
 //   one token over 700 cached, 32 on 8 of 128:                          14 us, a chain of waits
 // With few rows memory is the bound. With 64 rows a tile it is the softmax's chain of waits for scores, barriers and
-// weights: 37 % of the issue slots, 25 % of the ALU and 16 % of the tensor pipe are busy. A tile of the sizes above holds
-// R x 128 exponentials and as many roundings to two e4m3 terms, about ten operations each.
+// weights, and instruction fetch: 37 % of the issue slots, 25 % of the ALU and 16 % of the tensor pipe are busy, and code
+// that is never run moves these times by 3 to 5 %.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
