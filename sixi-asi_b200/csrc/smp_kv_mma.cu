@@ -34,7 +34,8 @@
 // at a time, with the scores of the next ready before one ends, hide it.
 //
 // Bound and measured (one B200, bytes at its copy rate of 6.54 TB/s, products at 1.65 PFLOP/s):
-//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 112 us, 5.5 TB/s (84 % of the copy rate)
+//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 111 to 117 us, 5.2 to 5.5 TB/s (80 to 84 %
+//     of the copy rate)
 //   2 sequences, one token, up to 262,144 cached, 32 on 4 of 128:       93 us, 5.6 TB/s (85 %)
 //   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         177 to 190 us; 26 us of bytes
 //   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       790 to 810 us; 163 us of products
