@@ -76,14 +76,18 @@ class _Caller:
             return self.raw_stream(self.device)
         return int(self.torch.cuda.current_stream(self.device).cuda_stream)
 
+    def here(self, t, what: str) -> None:
+        """Refuses a tensor that does not lie on the handle's device: its address would be read or written there."""
+        if not t.is_cuda or t.get_device() != self.device:
+            raise ValueError(f"{what}: on {t.device}, not cuda:{self.device}")
+
     def view(self, i: int, t, tokens: int, dim: int, what: str) -> int:
         """Record i filled with t [tokens, heads, dim] (unit stride along dim); its address."""
         dt = self.dtypes.get(t.dtype)
         shape = t.shape
         if dt is None or len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
             raise ValueError(f"{what}: fp32 or bf16 [{tokens}, heads, {dim}] expected, got {t.dtype} {tuple(shape)}")
-        if not t.is_cuda or t.get_device() != self.device:
-            raise ValueError(f"{what}: on {t.device}, not cuda:{self.device}")
+        self.here(t, what)
         stride = t.stride()
         if stride[2] != 1:
             raise ValueError(f"{what}: the last dimension must have unit stride")
@@ -128,6 +132,7 @@ class Rope:
         c, n, dim = self.call, x.shape[0], x.shape[-1]
         if positions.dtype != c.torch.int32 or positions.shape != (n,) or not positions.is_contiguous():
             raise ValueError("positions: contiguous int32 [tokens] expected")
+        c.here(positions, "positions")
         if out is None:
             out = c.torch.empty_like(x)
         elif out.shape != x.shape:
@@ -140,8 +145,8 @@ class Rope:
 
 class KvBatch:
     """The positions a call works on (sixi_kv_batch): page_table int32 [seqs, max_pages], offsets int64
-    [seqs + 1], lens int32 [seqs] (device tensors, kept alive here), and on the host the total number of
-    tokens and the most of one sequence."""
+    [seqs + 1], lens int32 [seqs] (tensors of the cache's device, kept alive here), and on the host the total
+    number of tokens and the most of one sequence."""
 
     def __init__(self, page_table, offsets, lens, n_tokens: int, max_new: int):
         import torch
@@ -153,6 +158,9 @@ class KvBatch:
             raise ValueError(f"offsets: contiguous int64 [{n + 1}] expected")
         if lens.dtype != torch.int32 or lens.shape != (n,) or not lens.is_contiguous():
             raise ValueError(f"lens: contiguous int32 [{n}] expected")
+        if not page_table.is_cuda or not (page_table.device == offsets.device == lens.device):
+            raise ValueError("page_table, offsets, lens: one CUDA device expected, got "
+                             f"{page_table.device}, {offsets.device}, {lens.device}")
         self.page_table, self.offsets, self.lens = page_table, offsets, lens
         self.n_seqs, self.n_tokens, self.max_new = n, int(n_tokens), int(max_new)
         self.struct = KvBatchStruct(page_table.data_ptr(), page_table.stride(0), offsets.data_ptr(), lens.data_ptr(), n,
@@ -208,11 +216,14 @@ class KvCache:
             pass
 
     def _status(self, status, batch: KvBatch):
+        """The call's status tensor, once the batch is known to lie on this device."""
         t = self.call.torch
+        self.call.here(batch.page_table, "batch")
         if status is None:
             return t.empty(batch.n_seqs, dtype=t.int32, device=self.call.dev)
         if status.dtype != t.int32 or status.shape != (batch.n_seqs,) or not status.is_contiguous():
             raise ValueError(f"status: contiguous int32 [{batch.n_seqs}] expected")
+        self.call.here(status, "status")
         return status
 
     def append(self, k, v, batch: KvBatch, rope: Rope | None = None, status=None, stream=None):
@@ -251,6 +262,7 @@ class KvCache:
             lse = c.torch.empty(q.shape[:2], dtype=c.torch.float32, device=c.dev)
         elif lse.dtype != c.torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous():
             raise ValueError(f"lse: contiguous fp32 {tuple(q.shape[:2])} expected")
+        c.here(lse, "lse")
         status = self._status(status, batch)
         st = _lib().sixi_kv_attend(self.h, c.view(0, q, n, dim, "q"), batch.at,
                                    dim ** -0.5 if scale is None else scale, window, 0 if causal else ATTEND_ALL,

@@ -1,0 +1,169 @@
+"""The cache's Python binding (sixi_smp.kv_cache) without a GPU: what it hands to the library, and what it refuses.
+
+The library is a recorder, tensors are stand-ins that say where they lie: nothing is dereferenced."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from sixi_smp import kv_cache as K
+
+I32, I64, F32, BF = torch.int32, torch.int64, torch.float32, torch.bfloat16
+
+
+class Tensor:
+    """What the binding asks a tensor for."""
+
+    def __init__(self, shape, dtype, device="cuda:0", at=0x1000):
+        self.shape, self.dtype, self.device, self.at = torch.Size(shape), dtype, torch.device(device), at
+        self.is_cuda = self.device.type == "cuda"
+        self.used_on = []
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        s = tuple(math.prod(self.shape[j + 1:]) for j in range(len(self.shape)))
+        return s if i is None else s[i]
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.device.index if self.is_cuda else -1
+
+    def data_ptr(self):
+        return self.at
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def record_stream(self, stream):
+        self.used_on.append(stream)
+
+
+class Library:
+    """Every entry point answers OK and is written down; `hook` sees the arguments first."""
+
+    def __init__(self):
+        self.calls, self.hook = [], None
+
+    def __getattr__(self, name):
+        def call(*args):
+            if name.endswith("_create"):
+                args[-1]._obj.value = 0x77
+            if self.hook is not None:
+                self.hook(name, args)
+            self.calls.append(name)
+            return 0
+
+        return call
+
+
+class Stream:
+    cuda_stream = 7
+
+
+HANDLES = []
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    lib = Library()
+    monkeypatch.setattr(K, "_lib", lambda: lib)
+    yield lib
+    for x in HANDLES:  # (the recorder's handles are nothing to the real library)
+        x.h = None
+    HANDLES.clear()
+
+
+def make_cache(n_kv_heads=2, head_dim=32):
+    pages = [Tensor((8, n_kv_heads, 16, head_dim), torch.uint8) for _ in range(2)]
+    scales = [Tensor((8, n_kv_heads), F32) for _ in range(2)]
+    HANDLES.append(K.KvCache(8, 16, n_kv_heads, head_dim, *pages, *scales, device=0))
+    return HANDLES[-1]
+
+
+def make_rope(rot_dim=32):
+    HANDLES.append(K.Rope(rot_dim, device=0))
+    return HANDLES[-1]
+
+
+def batch(device="cuda:0", **where):
+    at = {**dict.fromkeys(("page_table", "offsets", "lens"), device), **where}
+    return K.KvBatch(Tensor((1, 4), I32, at["page_table"]), Tensor((2,), I64, at["offsets"]),
+                     Tensor((1,), I32, at["lens"]), 3, 3)
+
+
+# ---------------------------------------------------------------------------------------------
+# where tensors lie: every address that reaches the library is one of the handle's device
+
+
+@pytest.mark.parametrize("which", ["page_table", "offsets", "lens"])
+@pytest.mark.parametrize("where", ["cpu", "cuda:1"])
+def test_batch_refuses_tensors_elsewhere(which, where):
+    with pytest.raises(ValueError, match=which):
+        batch(**{which: where})
+
+
+def test_batch_refuses_host_tensors():
+    """Real ones, as a caller would pass them."""
+    with pytest.raises(ValueError, match="page_table"):
+        K.KvBatch(torch.zeros((1, 4), dtype=I32), torch.tensor([0, 3]), torch.tensor([3], dtype=I32), 3, 3)
+
+
+def calls_of(cache, b, status=None, lse=None):
+    q, kv = Tensor((3, 4, 32), BF), Tensor((3, 2, 32), BF)
+    status = status or Tensor((1,), I32)
+    lse = lse or Tensor((3, 4), F32)
+    return {"append": lambda: cache.append(kv, kv, b, status=status, stream=Stream),
+            "read": lambda: cache.read(b, k=kv, v=kv, status=status, stream=Stream),
+            "attend": lambda: cache.attend(q, b, out=q, lse=lse, status=status, stream=Stream)}
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attend"])
+def test_cache_refuses_a_batch_of_another_device(lib, name):
+    cache = make_cache()
+    with pytest.raises(ValueError, match="batch"):
+        calls_of(cache, batch("cuda:1"))[name]()
+    assert lib.calls == ["sixi_kv_create"]
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda:1"])
+@pytest.mark.parametrize("name", ["append", "read", "attend"])
+def test_cache_refuses_a_status_elsewhere(lib, name, where):
+    cache = make_cache()
+    with pytest.raises(ValueError, match="status"):
+        calls_of(cache, batch(), status=Tensor((1,), I32, where))[name]()
+    assert lib.calls == ["sixi_kv_create"]
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda:1"])
+def test_attend_refuses_an_lse_elsewhere(lib, where):
+    cache = make_cache()
+    with pytest.raises(ValueError, match="lse"):
+        calls_of(cache, batch(), lse=Tensor((3, 4), F32, where))["attend"]()
+    assert lib.calls == ["sixi_kv_create"]
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda:1"])
+def test_rope_refuses_positions_elsewhere(lib, where):
+    rope = make_rope()
+    x = Tensor((3, 2, 32), BF)
+    with pytest.raises(ValueError, match="positions"):
+        rope.apply(x, Tensor((3,), I32, where), out=x, stream=Stream)
+    assert lib.calls == ["sixi_kv_rope_create"]
+
+
+def test_what_lies_on_the_device_is_passed_on(lib):
+    cache = make_cache()
+    for call in calls_of(cache, batch()).values():
+        call()
+    rope = make_rope()
+    x = Tensor((3, 2, 32), BF)
+    rope.apply(x, Tensor((3,), I32), out=x, stream=Stream)
+    assert lib.calls == ["sixi_kv_create", "sixi_kv_append", "sixi_kv_read", "sixi_kv_attend", "sixi_kv_rope_create",
+                         "sixi_kv_rope_apply"]
