@@ -8,7 +8,8 @@
  * values), array arguments are DEVICE pointers, every call is asynchronous on the caller's stream
  * and neither synchronises nor allocates (create excepted), and failures of a single sequence are
  * reported in out_status without affecting the other sequences. A cache handle owns a workspace: its
- * calls are serialised by the caller (one stream, or streams ordered by events).
+ * calls are serialised by the caller (one stream, or streams ordered by events). A rotary handle is
+ * only read: several threads and streams may use one at a time.
  */
 #ifndef SIXI_KV_H
 #define SIXI_KV_H

@@ -16,6 +16,7 @@ a of k drafts, lens for the next batch continues from lens - k + a.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 from . import BF16, F32, _check, _lib, _ptr
 
@@ -55,10 +56,17 @@ def _dev_index(device) -> int:
     return d.index if d.index is not None else torch.cuda.current_device()
 
 
+class _Records(threading.local):
+    """The records that a call passes, one set a thread: the interpreter lock is dropped while the library reads them."""
+
+    def __init__(self):
+        self.views = (KvTensor(), KvTensor())
+        self.at = tuple(ctypes.addressof(v) for v in self.views)
+
+
 class _Caller:
     """What the calls of one handle share: a step makes one or two of them a layer, so the records that they pass
-    are made once and filled in place (a handle serves one thread at a time), and the stream is asked for
-    without making a torch object of it."""
+    are made once (a thread) and filled in place, and the stream is asked for without making a torch object of it."""
 
     def __init__(self, device: int):
         import torch
@@ -66,8 +74,7 @@ class _Caller:
         self.torch, self.device, self.dev = torch, device, torch.device("cuda", device)
         self.dtypes = {torch.float32: F32, torch.bfloat16: BF16}
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self.views = (KvTensor(), KvTensor())
-        self.at = tuple(ctypes.addressof(v) for v in self.views)
+        self.records = _Records()
 
     def stream(self, stream) -> int:
         if stream is not None:
@@ -91,14 +98,16 @@ class _Caller:
         stride = t.stride()
         if stride[2] != 1:
             raise ValueError(f"{what}: the last dimension must have unit stride")
-        v = self.views[i]
+        r = self.records
+        v = r.views[i]
         v.data, v.dtype, v.n_heads, v.token_stride, v.head_stride = t.data_ptr(), dt, shape[1], stride[0], stride[1]
-        return self.at[i]
+        return r.at[i]
 
 
 class Rope:
     """Rotary frequencies on one device (sixi_kv_rope_create). layout "half" or "interleaved"; scaling
-    "none", "linear", "ntk" or "yarn" (factor; yarn also original_max_position and the betas)."""
+    "none", "linear", "ntk" or "yarn" (factor; yarn also original_max_position and the betas). Calls only read
+    it, so several threads and streams may use one at a time."""
 
     def __init__(self, rot_dim: int, base: float = 10000.0, layout: str = "half", scaling: str = "none",
                  factor: float = 1.0, original_max_position: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
@@ -171,7 +180,8 @@ class KvBatch:
 class KvCache:
     """A cache on one device (sixi_kv_create). The pages are torch tensors: uint8 or float8_e4m3fn
     [n_pages, n_kv_heads, page_size, head_dim] and fp32 scales [n_pages, n_kv_heads], allocated here
-    unless given."""
+    unless given. Its calls share a workspace: the caller puts them in order (one stream, or streams
+    ordered by events)."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, k_pages=None, v_pages=None,
                  k_scales=None, v_scales=None, max_seqs: int = 4096, device=None):

@@ -5,6 +5,7 @@ The library is a recorder, tensors are stand-ins that say where they lie: nothin
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -167,3 +168,37 @@ def test_what_lies_on_the_device_is_passed_on(lib):
     rope.apply(x, Tensor((3,), I32), out=x, stream=Stream)
     assert lib.calls == ["sixi_kv_create", "sixi_kv_append", "sixi_kv_read", "sixi_kv_attend", "sixi_kv_rope_create",
                          "sixi_kv_rope_apply"]
+
+
+# ---------------------------------------------------------------------------------------------
+# threads: a call's records are its own while the library reads them
+
+
+def test_two_threads_on_one_rope_keep_their_tensors(lib):
+    """The interpreter may run another thread while a call is in the library: its records stay what they were."""
+    rope = make_rope()
+    meet, seen = threading.Barrier(2, timeout=20), {}
+
+    def record(at):
+        v = K.KvTensor.from_address(at)
+        return v.data, v.token_stride, v.head_stride, v.n_heads
+
+    def hook(name, args):
+        meet.wait()  # both calls are inside the library
+        before = record(args[1]), record(args[6])
+        meet.wait()
+        seen[before[0][0]] = before
+        meet.wait()
+
+    def work(i):
+        x = Tensor((3, 2 + i, 32), BF, at=0x10000 * (i + 1))
+        rope.apply(x, Tensor((3,), I32), out=Tensor((3, 2 + i, 32), BF, at=0x10000 * (i + 1) + 0x100), stream=Stream)
+
+    lib.hook = hook
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert seen == {0x10000 * (i + 1): ((0x10000 * (i + 1), (2 + i) * 32, 32, 2 + i),
+                                        (0x10000 * (i + 1) + 0x100, (2 + i) * 32, 32, 2 + i)) for i in range(2)}
