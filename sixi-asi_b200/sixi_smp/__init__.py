@@ -16,6 +16,8 @@ the 8-bit paged key/value cache with its attention (include/sixi_kv.h, kv_cache.
 from __future__ import annotations
 
 import ctypes
+import functools
+import inspect
 import os
 from pathlib import Path
 
@@ -206,6 +208,48 @@ def make_params(n: int, **fields) -> np.ndarray:
 def _ptr(t) -> int:
     """Device pointer of a torch tensor, or 0 for None."""
     return 0 if t is None else int(t.data_ptr())
+
+
+def _device_tensors(x):
+    """The device tensors among a call's arguments or results."""
+    if isinstance(x, dict):
+        x = tuple(x.values())
+    if isinstance(x, (tuple, list)):
+        for y in x:
+            yield from _device_tensors(y)
+    elif hasattr(x, "record_stream"):
+        if x.is_cuda:
+            yield x
+    elif hasattr(x, "tensors"):  # a record of tensors (kv_cache.KvBatch)
+        yield from _device_tensors(x.tensors)
+
+
+def on_stream(fn):
+    """For a call with a `stream` argument: where that names another stream than the current one, the call runs with it
+    as the current one. So what the call allocates is that stream's (the current one may still be using memory that it
+    has given back), and what the call was given is not handed out again before that stream is through with it.
+    When either stream's work has to wait for the other's is the caller's to say (events)."""
+    at = list(inspect.signature(fn).parameters).index("stream")
+
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        s = args[at] if len(args) > at else kw.get("stream")
+        if s is None:
+            return fn(*args, **kw)
+        import torch
+
+        current = torch.cuda.current_stream(s.device)
+        if s.cuda_stream == current.cuda_stream:
+            return fn(*args, **kw)
+        with torch.cuda.stream(s):
+            out = fn(*args, **kw)
+        for t in _device_tensors((args, kw)):
+            t.record_stream(s)
+        for t in _device_tensors(out):  # the caller reads them on its own stream next
+            t.record_stream(current)
+        return out
+
+    return call
 
 
 class Sampler:

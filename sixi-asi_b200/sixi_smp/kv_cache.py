@@ -11,6 +11,10 @@ A serving step on a batch of streams, before the sampler or the verifier sees it
 `batch` names each sequence's last offsets[s + 1] - offsets[s] positions: one token a stream for a
 decode step, 1 + k for speculative verification, a chunk of a prompt. After the verifier has accepted
 a of k drafts, lens for the next batch continues from lens - k + a.
+
+Calls run on the current stream, or on `stream`: what they allocate then belongs to that stream, and what
+they are given stays as it is until that stream is through with it. Which stream waits for which is the
+caller's to say (events).
 """
 
 from __future__ import annotations
@@ -18,7 +22,7 @@ from __future__ import annotations
 import ctypes
 import threading
 
-from . import BF16, F32, _check, _lib, _ptr
+from . import BF16, F32, _check, _lib, _ptr, on_stream
 
 _P = ctypes.c_void_p
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
@@ -135,6 +139,7 @@ class Rope:
         except Exception:
             pass
 
+    @on_stream
     def apply(self, x, positions, inverse: bool = False, out=None, stream=None):
         """x [tokens, heads, dim] turned by positions [tokens] (int32); inverse turns back (the gradient).
         out may be x."""
@@ -171,6 +176,7 @@ class KvBatch:
             raise ValueError("page_table, offsets, lens: one CUDA device expected, got "
                              f"{page_table.device}, {offsets.device}, {lens.device}")
         self.page_table, self.offsets, self.lens = page_table, offsets, lens
+        self.tensors = (page_table, offsets, lens)
         self.n_seqs, self.n_tokens, self.max_new = n, int(n_tokens), int(max_new)
         self.struct = KvBatchStruct(page_table.data_ptr(), page_table.stride(0), offsets.data_ptr(), lens.data_ptr(), n,
                                     page_table.shape[1], self.n_tokens, self.max_new)
@@ -236,6 +242,7 @@ class KvCache:
         self.call.here(status, "status")
         return status
 
+    @on_stream
     def append(self, k, v, batch: KvBatch, rope: Rope | None = None, status=None, stream=None):
         """Writes k, v [tokens, n_kv_heads, head_dim] at the batch's positions, the keys turned by rope.
         Returns the status of each sequence (int32, device)."""
@@ -246,6 +253,7 @@ class KvCache:
         _check("sixi_kv_append", st)
         return status
 
+    @on_stream
     def read(self, batch: KvBatch, dtype=None, k=None, v=None, status=None, stream=None):
         """The batch's positions as values: k, v [tokens, n_kv_heads, head_dim] (dtype bf16 or fp32)."""
         c, n, dim = self.call, batch.n_tokens, self.head_dim
@@ -259,6 +267,7 @@ class KvCache:
         _check("sixi_kv_read", st)
         return k, v
 
+    @on_stream
     def attend(self, q, batch: KvBatch, scale: float | None = None, window: int = 0, causal: bool = True,
                rope: Rope | None = None, out=None, lse=None, status=None, stream=None):
         """Attention of q [tokens, n_q_heads, head_dim] over the cache: (out like q, lse fp32 [tokens,

@@ -4,6 +4,7 @@ The library is a recorder, tensors are stand-ins that say where they lie: nothin
 
 from __future__ import annotations
 
+import contextlib
 import math
 import threading
 
@@ -65,16 +66,34 @@ class Library:
 
 
 class Stream:
-    cuda_stream = 7
+    def __init__(self, raw):
+        self.cuda_stream, self.device = raw, torch.device("cuda:0")
 
 
+MAIN, SIDE = Stream(7), Stream(8)
 HANDLES = []
 
 
 @pytest.fixture
 def lib(monkeypatch):
     lib = Library()
+    lib.current, lib.made = [MAIN], []
     monkeypatch.setattr(K, "_lib", lambda: lib)
+
+    @contextlib.contextmanager
+    def use(stream):
+        lib.current.append(stream)
+        yield
+        lib.current.pop()
+
+    def empty(shape, dtype=None, device=None):
+        lib.made.append((lib.current[-1], Tensor((shape,) if isinstance(shape, int) else shape, dtype)))
+        return lib.made[-1][1]
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: lib.current[-1])
+    monkeypatch.setattr(torch.cuda, "stream", use)
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(torch, "empty_like", lambda t: empty(t.shape, t.dtype))
     yield lib
     for x in HANDLES:  # (the recorder's handles are nothing to the real library)
         x.h = None
@@ -120,9 +139,9 @@ def calls_of(cache, b, status=None, lse=None):
     q, kv = Tensor((3, 4, 32), BF), Tensor((3, 2, 32), BF)
     status = status or Tensor((1,), I32)
     lse = lse or Tensor((3, 4), F32)
-    return {"append": lambda: cache.append(kv, kv, b, status=status, stream=Stream),
-            "read": lambda: cache.read(b, k=kv, v=kv, status=status, stream=Stream),
-            "attend": lambda: cache.attend(q, b, out=q, lse=lse, status=status, stream=Stream)}
+    return {"append": lambda: cache.append(kv, kv, b, status=status, stream=MAIN),
+            "read": lambda: cache.read(b, k=kv, v=kv, status=status, stream=MAIN),
+            "attend": lambda: cache.attend(q, b, out=q, lse=lse, status=status, stream=MAIN)}
 
 
 @pytest.mark.parametrize("name", ["append", "read", "attend"])
@@ -155,7 +174,7 @@ def test_rope_refuses_positions_elsewhere(lib, where):
     rope = make_rope()
     x = Tensor((3, 2, 32), BF)
     with pytest.raises(ValueError, match="positions"):
-        rope.apply(x, Tensor((3,), I32, where), out=x, stream=Stream)
+        rope.apply(x, Tensor((3,), I32, where), out=x, stream=MAIN)
     assert lib.calls == ["sixi_kv_rope_create"]
 
 
@@ -165,7 +184,7 @@ def test_what_lies_on_the_device_is_passed_on(lib):
         call()
     rope = make_rope()
     x = Tensor((3, 2, 32), BF)
-    rope.apply(x, Tensor((3,), I32), out=x, stream=Stream)
+    rope.apply(x, Tensor((3,), I32), out=x, stream=MAIN)
     assert lib.calls == ["sixi_kv_create", "sixi_kv_append", "sixi_kv_read", "sixi_kv_attend", "sixi_kv_rope_create",
                          "sixi_kv_rope_apply"]
 
@@ -192,7 +211,7 @@ def test_two_threads_on_one_rope_keep_their_tensors(lib):
 
     def work(i):
         x = Tensor((3, 2 + i, 32), BF, at=0x10000 * (i + 1))
-        rope.apply(x, Tensor((3,), I32), out=Tensor((3, 2 + i, 32), BF, at=0x10000 * (i + 1) + 0x100), stream=Stream)
+        rope.apply(x, Tensor((3,), I32), out=Tensor((3, 2 + i, 32), BF, at=0x10000 * (i + 1) + 0x100), stream=MAIN)
 
     lib.hook = hook
     threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
@@ -202,3 +221,44 @@ def test_two_threads_on_one_rope_keep_their_tensors(lib):
         t.join()
     assert seen == {0x10000 * (i + 1): ((0x10000 * (i + 1), (2 + i) * 32, 32, 2 + i),
                                         (0x10000 * (i + 1) + 0x100, (2 + i) * 32, 32, 2 + i)) for i in range(2)}
+
+
+# ---------------------------------------------------------------------------------------------
+# streams: with `stream` given, nothing that the call touches is memory that another stream may still use, or be handed
+
+
+def on_side(cache):
+    q, k, v = Tensor((3, 4, 32), BF), Tensor((3, 2, 32), BF), Tensor((3, 2, 32), BF)
+    b = batch()
+    rope, pos = make_rope(), Tensor((3,), I32)
+    own = [b.page_table, b.offsets, b.lens]
+    return {"append": (lambda: cache.append(k, v, b, stream=SIDE), [k, v, *own]),
+            "read": (lambda: cache.read(b, stream=SIDE), own),
+            "attend": (lambda: cache.attend(q, b, stream=SIDE), [q, *own]),
+            "apply": (lambda: rope.apply(q, pos, stream=SIDE), [q, pos])}
+
+
+@pytest.mark.parametrize("name", ["append", "read", "attend", "apply"])
+def test_a_named_stream_owns_what_the_call_makes(lib, name):
+    call, given = on_side(make_cache())[name]
+    result = call()
+    assert lib.made and all(s is SIDE for s, _ in lib.made)
+    assert all(t.used_on == [SIDE] for t in given)  # not handed out again before the side stream is through
+    for t in result if isinstance(result, tuple) else (result,):
+        assert t.used_on == [MAIN]  # the caller's stream reads it next
+    assert lib.current == [MAIN]
+
+
+def test_the_current_stream_costs_nothing(lib):
+    cache = make_cache()
+    q, b = Tensor((3, 4, 32), BF), batch()
+    result = cache.attend(q, b, stream=MAIN)
+    assert [s for s, _ in lib.made] == [MAIN] * 3
+    assert not any(t.used_on for t in (*result, q, b.lens))
+
+
+def test_a_stream_given_by_position(lib):
+    cache = make_cache()
+    k, v = Tensor((3, 2, 32), BF), Tensor((3, 2, 32), BF)
+    cache.append(k, v, batch(), None, None, SIDE)
+    assert [s for s, _ in lib.made] == [SIDE] and k.used_on == [SIDE]
