@@ -238,6 +238,8 @@ def on_stream(fn):
             return fn(*args, **kw)
         import torch
 
+        if not hasattr(s, "device"):  # another library's stream
+            s = torch.cuda.ExternalStream(s.cuda_stream)
         current = torch.cuda.current_stream(s.device)
         if s.cuda_stream == current.cuda_stream:
             return fn(*args, **kw)
@@ -291,6 +293,7 @@ class Sampler:
         s = stream if stream is not None else torch.cuda.current_stream()
         return int(s.cuda_stream)
 
+    @on_stream
     def sample(self, logits, params, masks=None, hist=None, hist_off=None, uniforms=None, step=0,
                out_tokens=None, out_status=None, stream=None):
         import torch
@@ -308,6 +311,7 @@ class Sampler:
         _check("sixi_smp_sample", st)
         return out_tokens, out_status
 
+    @on_stream
     def sample_indexed(self, logits, row_map, params, out_tokens, out_status, masks=None, hist=None, hist_off=None,
                        uniforms=None, step=0, stream=None):
         """sixi_smp_sample_indexed: row j of `logits` sampled as batch row row_map[j] (int32 device
@@ -319,6 +323,7 @@ class Sampler:
         _check("sixi_smp_sample_indexed", st)
         return out_tokens, out_status
 
+    @on_stream
     def gather_rows(self, src, row_index, width: int, out=None, stream=None):
         """sixi_smp_gather_rows: out[j, :width] = src[row_index[j], :width] (device tensors)."""
         import torch
@@ -332,6 +337,7 @@ class Sampler:
         _check("sixi_smp_gather_rows", st)
         return out
 
+    @on_stream
     def greedy_argmax(self, logits, masks=None, stream=None):
         import torch
 
@@ -344,6 +350,7 @@ class Sampler:
         _check("sixi_smp_greedy_argmax", st)
         return tok, sts
 
+    @on_stream
     def candidates(self, logits, params, max_out=256, masks=None, hist=None, hist_off=None,
                    stream=None):
         import torch
@@ -361,6 +368,7 @@ class Sampler:
         _check("sixi_smp_candidates", st)
         return ids, probs, cnt, sts
 
+    @on_stream
     def verify(self, target, drafts, params, draft_probs=None, n_drafts=None, masks=None, hist=None,
                hist_off=None, uniforms=None, step=0, stream=None):
         import torch
@@ -382,6 +390,7 @@ class Sampler:
         return dict(accepted=acc, tokens=toks, n_tokens=ntok, first_reject=frej, uniforms_used=used,
                     status=sts)
 
+    @on_stream
     def verify_draft_logits(self, target, draft_logits, draft_temperatures, drafts, params, n_drafts=None,
                             masks=None, hist=None, hist_off=None, uniforms=None, step=0, stream=None):
         """verify with q = full_distribution(draft_logits, draft_temperatures), never stored."""
@@ -405,6 +414,7 @@ class Sampler:
         return dict(accepted=acc, tokens=toks, n_tokens=ntok, first_reject=frej, uniforms_used=used,
                     status=sts)
 
+    @on_stream
     def full_distribution(self, logits, temperatures, stream=None):
         """compute_full_distribution per row: fp32 probabilities [n_rows, vocab]."""
         import torch
@@ -416,6 +426,7 @@ class Sampler:
         _check("sixi_smp_full_distribution", st)
         return out
 
+    @on_stream
     def numeric_policy(self, logits, policy: int = NUMERIC_FAIL, clamp_abs_max: float = 0.0, out=None, stream=None):
         """inspect_and_apply_numeric_policy per row of fp32 `logits` [n_rows, >= vocab] (a row view
         of wider rows is fine), in place under NUMERIC_CLAMP. Returns the reports as a uint8 device
@@ -432,6 +443,7 @@ class Sampler:
         _check("sixi_smp_numeric_policy", st)
         return out
 
+    @on_stream
     def suffix_draft(self, hist, hist_off, k: int = 8, min_match_len: int = 3, max_window_tokens: int = 16384,
                      anchors=None, out=None, out_match=None, stream=None):
         """SuffixDrafter::propose (or ::propose_anchored with `anchors` [n_streams]) for the CSR
@@ -452,6 +464,7 @@ class Sampler:
         return out, out_match
 
     # -- vocab-sharded mode ----------------------------------------------------------------------
+    @on_stream
     def shard_candidates(self, shard_logits, vocab_offset: int, shard_vocab: int, params, top_n: int = 64,
                          masks=None, hist=None, hist_off=None, stream=None):
         """Stage 1 on this rank's slice: shard_logits [n_rows, >= shard_vocab] (a column slice of the
@@ -469,6 +482,7 @@ class Sampler:
         _check("sixi_smp_shard_candidates", st)
         return cand, stats
 
+    @on_stream
     def merge_shards(self, gathered_cand, gathered_stats, params, uniforms=None, step: int = 0, stream=None):
         """Stage 2: gathered_cand [n_shards, n_rows, top_n, 2], gathered_stats [n_shards, n_rows, 24]."""
         import torch
@@ -508,6 +522,7 @@ class Sampler:
 STATIC_VERIFY_ROWS = 4096  # SIXI_SMP_STATIC_VERIFY_ROWS
 
 
+@on_stream
 def verify_static(vocab: int, target, drafts, params, draft_probs=None, n_drafts=None, masks=None, hist=None,
                   hist_off=None, uniforms=None, step=0, stream=None):
     """sixi_smp_verify_static: the verifier without a handle or any allocation inside the call

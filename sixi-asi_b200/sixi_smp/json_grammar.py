@@ -19,7 +19,7 @@ import json
 
 import numpy as np
 
-from . import INVALID_ARGUMENT, OK, SixiError, _check, _lib, _ptr  # noqa: F401
+from . import INVALID_ARGUMENT, OK, SixiError, _check, _lib, _ptr, on_stream  # noqa: F401
 
 STATE_BYTES = 32
 TOKEN_SPECIAL = 1
@@ -76,9 +76,11 @@ class JsonGrammar:
 
         return torch.zeros((n, STATE_BYTES), dtype=torch.uint8, device=torch.device("cuda", self.device))
 
+    @on_stream
     def reset(self, states, stream=None) -> None:
         _check("sixi_json_reset", _lib().sixi_json_reset(self.h, _ptr(states), states.shape[0], _stream(stream)))
 
+    @on_stream
     def fill_masks(self, states, out=None, stream=None):
         """int32 [n, ceil(V/32)] mask words (bit i % 32 of word i / 32: token i allowed)."""
         import torch
@@ -90,6 +92,7 @@ class JsonGrammar:
                                                                      out.stride(0), _stream(stream)))
         return out
 
+    @on_stream
     def advance(self, states, tokens, n_tokens=None, out_status=None, stream=None):
         """Applies tokens ([n] or [n, m] with n_tokens [n]) to the states; returns int32 statuses."""
         import torch
@@ -102,6 +105,7 @@ class JsonGrammar:
                                                                _ptr(n_tokens), _ptr(out_status), _stream(stream)))
         return out_status
 
+    @on_stream
     def expand_drafts(self, states, drafts, n_drafts=None, out=None, stream=None):
         """[S * (k + 1), 32] states: row j of stream s after its first j drafts."""
         import torch

@@ -20,7 +20,7 @@ import json
 
 import numpy as np
 
-from . import INVALID_ARGUMENT, _check, _lib, _ptr  # noqa: F401
+from . import INVALID_ARGUMENT, _check, _lib, _ptr, on_stream  # noqa: F401
 from .json_grammar import csr
 
 STATE_BYTES = 800  # SIXI_SCHEMA_STATE_BYTES
@@ -85,9 +85,11 @@ class SchemaGrammar:
         self.reset(st)
         return st
 
+    @on_stream
     def reset(self, states, stream=None) -> None:
         _check("sixi_schema_reset", _lib().sixi_schema_reset(self.h, _ptr(states), states.shape[0], _stream(stream)))
 
+    @on_stream
     def fill_masks(self, states, out=None, stream=None):
         import torch
 
@@ -98,6 +100,7 @@ class SchemaGrammar:
                                                                        out.stride(0), _stream(stream)))
         return out
 
+    @on_stream
     def advance(self, states, tokens, n_tokens=None, out_status=None, stream=None):
         import torch
 

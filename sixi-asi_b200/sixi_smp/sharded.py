@@ -21,6 +21,8 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Callable
 
+from . import on_stream
+
 
 @dataclass(frozen=True)
 class ShardLayout:
@@ -42,6 +44,7 @@ class ShardLayout:
 OUT_OF_BOUNDS = 2
 
 
+@on_stream
 def sample_vocab_sharded(shard_logits, layout: ShardLayout, rank: int, params, *, top_n: int = 64,
                          masks=None, hist=None, hist_off=None, uniforms=None, step: int = 0,
                          stage1: Callable | None = None, stage2: Callable | None = None,

@@ -12,8 +12,10 @@ pytestmark = pytest.mark.gpu
 if not has_gpu():
     pytest.skip("no CUDA device", allow_module_level=True)
 
+import numpy as np  # noqa: E402
 import torch  # noqa: E402
 
+import sixi_smp as S  # noqa: E402
 from sixi_smp.kv_cache import KvBatch, KvCache, Rope  # noqa: E402
 
 DEV = torch.device("cuda:0")
@@ -63,3 +65,26 @@ def test_what_a_call_was_given_is_not_handed_out_again(name):
     again = [torch.empty_like(x).fill_(7.0) for _ in range(4)]
     torch.cuda.synchronize()
     assert torch.equal(got, want) and len(again) == 4
+
+
+@pytest.mark.parametrize("delayed", ["current", "named"])
+def test_sampler_candidates_on_a_named_stream(delayed):
+    """Its outputs are filled before the call: on the stream that the call runs on."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    logits = torch.randn((32, 4096), device=DEV, generator=g)
+    smp = S.Sampler(0, 32, 4096)
+    params = torch.from_numpy(S.make_params(32, temperature=0.7, top_k=20).view(np.uint8)).to(DEV)
+    want = [t.clone() for t in smp.candidates(logits, params, max_out=32)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.current_stream() if delayed == "current" else side):
+        torch.cuda._sleep(DELAY)
+    mine = logits.clone() if delayed == "named" else logits
+    torch.cuda.current_stream().synchronize() if delayed == "named" else None
+    got = smp.candidates(mine, params, max_out=32, stream=side)
+    del mine
+    again = torch.empty_like(logits).fill_(7.0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and again is not None
+    smp.close()

@@ -11,6 +11,8 @@ import threading
 import pytest
 import torch
 
+import sixi_smp
+from sixi_smp import json_grammar, json_schema
 from sixi_smp import kv_cache as K
 
 I32, I64, F32, BF = torch.int32, torch.int64, torch.float32, torch.bfloat16
@@ -78,7 +80,8 @@ HANDLES = []
 def lib(monkeypatch):
     lib = Library()
     lib.current, lib.made = [MAIN], []
-    monkeypatch.setattr(K, "_lib", lambda: lib)
+    for module in (K, sixi_smp, json_grammar, json_schema):
+        monkeypatch.setattr(module, "_lib", lambda: lib)
 
     @contextlib.contextmanager
     def use(stream):
@@ -93,6 +96,8 @@ def lib(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: lib.current[-1])
     monkeypatch.setattr(torch.cuda, "stream", use)
     monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(torch, "zeros", empty)
+    monkeypatch.setattr(torch, "full", lambda shape, value, dtype=None, device=None: empty(shape, dtype))
     monkeypatch.setattr(torch, "empty_like", lambda t: empty(t.shape, t.dtype))
     yield lib
     for x in HANDLES:  # (the recorder's handles are nothing to the real library)
