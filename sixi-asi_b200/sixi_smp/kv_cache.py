@@ -108,6 +108,15 @@ class _Caller:
         return r.at[i]
 
 
+def _rope_handle(rope):
+    """The rotation that a call passes; a closed one is refused, since no handle means no rotation."""
+    if rope is None:
+        return None
+    if not rope.h:
+        raise ValueError("rope: closed")
+    return rope.h
+
+
 class Rope:
     """Rotary frequencies on one device (sixi_kv_rope_create). layout "half" or "interleaved"; scaling
     "none", "linear", "ntk" or "yarn" (factor; yarn also original_max_position and the betas). Calls only read
@@ -249,7 +258,7 @@ class KvCache:
         c, n, dim = self.call, batch.n_tokens, self.head_dim
         status = self._status(status, batch)
         st = _lib().sixi_kv_append(self.h, c.view(0, k, n, dim, "k"), c.view(1, v, n, dim, "v"), batch.at,
-                                   rope.h if rope is not None else None, status.data_ptr(), c.stream(stream))
+                                   _rope_handle(rope), status.data_ptr(), c.stream(stream))
         _check("sixi_kv_append", st)
         return status
 
@@ -284,8 +293,8 @@ class KvCache:
         c.here(lse, "lse")
         status = self._status(status, batch)
         st = _lib().sixi_kv_attend(self.h, c.view(0, q, n, dim, "q"), batch.at,
-                                   dim ** -0.5 if scale is None else scale, window, 0 if causal else ATTEND_ALL,
-                                   rope.h if rope is not None else None, c.view(1, out, n, dim, "out"), lse.data_ptr(),
-                                   status.data_ptr(), c.stream(stream))
+                                   dim ** -0.5 if scale is None else scale, window,
+                                   0 if causal else ATTEND_ALL, _rope_handle(rope), c.view(1, out, n, dim, "out"),
+                                   lse.data_ptr(), status.data_ptr(), c.stream(stream))
         _check("sixi_kv_attend", st)
         return out, lse, status

@@ -267,3 +267,18 @@ def test_a_stream_given_by_position(lib):
     k, v = Tensor((3, 2, 32), BF), Tensor((3, 2, 32), BF)
     cache.append(k, v, batch(), None, None, SIDE)
     assert [s for s, _ in lib.made] == [SIDE] and k.used_on == [SIDE]
+
+
+# ---------------------------------------------------------------------------------------------
+# arguments that would be taken for others
+
+
+@pytest.mark.parametrize("name", ["append", "attend"])
+def test_a_closed_rope_is_refused(lib, name):
+    """Its handle is nothing, which the library takes for a call without a rotation."""
+    cache, rope = make_cache(), make_rope()
+    rope.close()
+    q, kv, b = Tensor((3, 4, 32), BF), Tensor((3, 2, 32), BF), batch()
+    with pytest.raises(ValueError, match="rope"):
+        cache.append(kv, kv, b, rope=rope, stream=MAIN) if name == "append" else cache.attend(q, b, rope=rope, stream=MAIN)
+    assert not {"sixi_kv_append", "sixi_kv_attend"} & set(lib.calls)
