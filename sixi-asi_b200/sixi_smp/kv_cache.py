@@ -127,6 +127,9 @@ class Rope:
                  device=None):
         if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
             raise ValueError(f"unknown rotary layout {layout!r} or scaling {scaling!r}")
+        for what, v in (("rot_dim", rot_dim), ("original_max_position", original_max_position)):
+            if not 0 <= v < 2 ** 32:  # (ctypes would take its low 32 bits)
+                raise ValueError(f"{what}: {v} does not fit 32 bits")
         self.h = None
         self.device = _dev_index(device)
         self.call = _Caller(self.device)
@@ -282,6 +285,8 @@ class KvCache:
         """Attention of q [tokens, n_q_heads, head_dim] over the cache: (out like q, lse fp32 [tokens,
         n_q_heads], status int32 [seqs]). scale defaults to head_dim ** -0.5; window 0 is none."""
         c, n, dim = self.call, batch.n_tokens, self.head_dim
+        if window < 0:
+            raise ValueError(f"window: {window} is negative")
         if out is None:
             out = c.torch.empty_like(q)
         elif out.shape != q.shape:
@@ -293,7 +298,7 @@ class KvCache:
         c.here(lse, "lse")
         status = self._status(status, batch)
         st = _lib().sixi_kv_attend(self.h, c.view(0, q, n, dim, "q"), batch.at,
-                                   dim ** -0.5 if scale is None else scale, window,
+                                   dim ** -0.5 if scale is None else scale, min(window, 0xFFFFFFFF),
                                    0 if causal else ATTEND_ALL, _rope_handle(rope), c.view(1, out, n, dim, "out"),
                                    lse.data_ptr(), status.data_ptr(), c.stream(stream))
         _check("sixi_kv_attend", st)

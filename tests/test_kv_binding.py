@@ -5,6 +5,7 @@ The library is a recorder, tensors are stand-ins that say where they lie: nothin
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import math
 import threading
 
@@ -282,3 +283,23 @@ def test_a_closed_rope_is_refused(lib, name):
     with pytest.raises(ValueError, match="rope"):
         cache.append(kv, kv, b, rope=rope, stream=MAIN) if name == "append" else cache.attend(q, b, rope=rope, stream=MAIN)
     assert not {"sixi_kv_append", "sixi_kv_attend"} & set(lib.calls)
+
+
+def test_windows_beyond_32_bits(lib):
+    cache, seen = make_cache(), []
+    lib.hook = lambda name, args: seen.append(ctypes.c_uint32(args[4]).value)
+    q, b = Tensor((3, 4, 32), BF), batch()
+    for window in (0, 5, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1):
+        cache.attend(q, b, window=window, stream=MAIN)
+    assert seen == [0, 5] + [2 ** 32 - 1] * 4
+    for window in (-1, -2 ** 32 + 5):
+        with pytest.raises(ValueError, match="window"):
+            cache.attend(q, b, window=window, stream=MAIN)
+
+
+@pytest.mark.parametrize("field", ["rot_dim", "original_max_position"])
+@pytest.mark.parametrize("value", [-1, 2 ** 32 + 64])
+def test_rope_numbers_beyond_32_bits_are_refused(lib, field, value):
+    args = dict(rot_dim=64, scaling="yarn", factor=2.0, original_max_position=4096)
+    with pytest.raises(ValueError, match=field):
+        K.Rope(device=0, **{**args, field: value})
