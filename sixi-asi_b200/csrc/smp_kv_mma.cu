@@ -324,7 +324,7 @@ struct Shared {
     alignas(16) float frow[kQSlots][R];                 // a row's factor from the product to the score, base 2; positive
     int32_t qpos[kQSlots][R];               // a row's position
     float wmax[G][2][4][R];                 // [group][its tiles' parity][warp] a tile's maxima
-    alignas(16) float2 ref[4 * G][R];                       // [softmax warp] running maximum, weight factor
+    alignas(16) float2 ref[4 * G][R];       // [softmax warp] running maximum, weight factor; before: score factors
     float rescale[4 * G][R];                    // [softmax warp] factor of the older sums
     float osc[G][R], mgrp[G][R];            // a tile's factor, and the running maximum that its weights are under
     float2 sines[3][128];                   // [staging warp] of a token's pairs
@@ -494,7 +494,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             *reinterpret_cast<uint2*>(dst + to + R * 128u) = make_uint2(l[0], l[1]);
             if (d0 == 0u) {
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
-                // (positive, so that a masked score stays -inf; at 1e-30 scores are zero all the same)
+                // (at 1e-30 scores are zero all the same)
                 frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
                 qpos[col] = pc.p0 + static_cast<int32_t>((base + r) / group);
             }
@@ -948,6 +948,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             constexpr int kOwn = kFold > 8 ? kFold / 8 : 1;             // those that a lane ends with where they are dealt out
             const uint32_t own = q * V + first_of<kFold>(lane);
             float2* my_ref = sh.ref[warp - 8u];
+            float* my_fac = reinterpret_cast<float*>(my_ref);  // (the same place, until the tile's maxima are known)
             float* my_rescale = sh.rescale[warp - 8u];
             uint8_t* w0 = wbuf + grp * C::kW + (quad * 4u) * 128u + tr * 16u + ((q * V) >> 4) * (16u * kTile) + ((q * V) & 15u);
             const auto max_op = [](float x, float y) { return fmaxf(x, y); };
@@ -959,7 +960,6 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 const PieceRec& pc = *rec;
                 const uint32_t rs = np % kQSlots;
                 bar_wait(&sh.rfull[rs], (np / kQSlots) & 1u, gave_up);
-                const float* frow = sh.frow[rs] + q * V;
                 const int32_t* qpos = sh.qpos[rs] + q * V;
                 // tiles in [safe_from, reach) are inside every row's positions
                 const int32_t p_first = pc.p0 + static_cast<int32_t>(pc.row_tile * a.shape.rt / a.shape.group);
@@ -980,7 +980,14 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     const uint32_t vs = n % NV, use = n / G;
                     float(*wmax)[R] = sh.wmax[grp][use & 1u];  // (its last readers met since)
                     bar_wait(&sh.scfull[vs], (n / NV) & 1u, gave_up);
-                    const float fk0 = sh.kscale[vs][pg0], fk1 = sh.kscale[vs][pg1];
+                    // From products to scores, base 2, by one factor a row and half of the warp's tokens (which may lie in
+                    // two pages). A score is rounded here and nowhere later: the same value is compared and taken to its
+                    // weight, so no weight is above 1 however large the scores are.
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i) {
+                        my_fac[own + i] = f_own[i] * sh.kscale[vs][pg0];
+                        my_fac[R + own + i] = f_own[i] * sh.kscale[vs][pg1];
+                    }
                     // exponents of the values' scales, relative to the tile's largest: they go into the weights.
                     // Where they differ by much, the weights' factor has to come from the largest product of
                     // weight and scale: the largest weight's own value could be below others' rounding.
@@ -1011,11 +1018,12 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
 #pragma unroll
                         for (int j = j0; j < j0 + 2; ++j) {
                             if (j >= NB) continue;
+                            const float2 a0 = *reinterpret_cast<const float2*>(my_fac + q * V + 2 * j);
+                            const float2 a1 = *reinterpret_cast<const float2*>(my_fac + R + q * V + 2 * j);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float fk = i < 2 ? fk0 : fk1;
                                 const F2 sum = add2(f2(f[j - j0][2 * i], f[j - j0][2 * i + 1]), f2(g[j - j0][2 * i], g[j - j0][2 * i + 1]));
-                                const float2 y = un2(mul2(sum, f2(fk, fk)));
+                                const float2 y = un2(mul2(sum, i < 2 ? f2(a0.x, a0.y) : f2(a1.x, a1.y)));
                                 x[j][0][i] = y.x, x[j][1][i] = y.y;
                             }
                         }
@@ -1054,15 +1062,15 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i)
                         mt[i] = fmaxf(fmaxf(wmax[0][own + i], wmax[1][own + i]),
-                                      fmaxf(wmax[2][own + i], wmax[3][own + i])) * f_own[i];
+                                      fmaxf(wmax[2][own + i], wmax[3][own + i]));
                     float mw[kOwn];  // of weight times value scale
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) mw[i] = mt[i];
                     if (wide) {
 #pragma unroll
                         for (int c = 0; c < kFold; ++c)
-                            mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]) * frow[c] + static_cast<float>(ev0),
-                                          fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]) * frow[c] + static_cast<float>(ev1));
+                            mx[c] = fmaxf(fmaxf(x[c >> 1][c & 1][0], x[c >> 1][c & 1][1]) + static_cast<float>(ev0),
+                                          fmaxf(x[c >> 1][c & 1][2], x[c >> 1][c & 1][3]) + static_cast<float>(ev1));
                         fold_lanes<kFold>(mx, lane, max_op);
                         group_sync(grp);  // the first maxima have been read
 #pragma unroll
@@ -1107,13 +1115,12 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
 #pragma unroll
                         for (int j = 0; j < NB; ++j) {
                             const float4 rf = *reinterpret_cast<const float4*>(my_ref + q * V + 2 * j);
-                            const float2 fr = *reinterpret_cast<const float2*>(frow + 2 * j);
-                            const F2 scale2 = f2(fr.x, fr.y), minus = f2(rf.x, rf.z);
+                            const F2 minus = f2(rf.x, rf.z);
                             const F2 wf0 = mul2(f2(rf.y, rf.w), f2(vr0, vr0)), wf1 = mul2(f2(rf.y, rf.w), f2(vr1, vr1));
                             F2 p[kTok];
 #pragma unroll
                             for (int i = 0; i < kTok; ++i) {
-                                const float2 y = un2(fma2(f2(x[j][0][t0 + i], x[j][1][t0 + i]), scale2, minus));
+                                const float2 y = un2(add2(f2(x[j][0][t0 + i], x[j][1][t0 + i]), minus));
                                 p[i] = f2(ex2(y.x), ex2(y.y));
                             }
                             F2 sum = p[0];
