@@ -47,6 +47,8 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
+#include <cstring>
 
 #include "smp_kernels.cuh"
 #include "smp_kv.cuh"
@@ -56,7 +58,6 @@ namespace {
 
 constexpr int kTile = 128;      // tokens of a tile
 constexpr int kTileShift = 7;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitIters = 1u << 24;  // bound of a wait: a tenth of a second at the least (never expected to run out)
 constexpr int kRing = 8;    // more than the tiles in flight, so that a waiter a few tiles behind finds its phase
@@ -321,7 +322,7 @@ struct Shared {
     uint32_t tmem, gave_up, ctas, pieces_done, split_mask, join_mask;
     float kscale[kNV][8], vscale[kNV][8];   // by page of the tile
     // by column of the weights:
-    alignas(16) float frow[kQSlots][R];                 // a row's factor from the product to the score, base 2; positive
+    uint32_t frow[kQSlots][R];              // a row's factor from products to scores: score_factor's code
     int32_t qpos[kQSlots][R];               // a row's position
     float wmax[G][2][4][R];                 // [group][its tiles' parity][warp] a tile's maxima
     alignas(16) float2 ref[4 * G][R];       // [softmax warp] running maximum, weight factor; before: score factors
@@ -339,7 +340,23 @@ struct MmaArgs {
     uint32_t read_once;  // no page is read by more than one row tile
     uint32_t out_pair;   // two elements of an output row can be stored together
     uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
+    // |scale| log2(e) = (1 + mant / 2^23) 2^exp; the sign goes to the queries (0: a scale of 0)
+    uint32_t scale_mant;
+    int32_t scale_exp;
+    float scale_sign;
 };
+
+// The factor from products to scores is a significand times 2^(exponents of scale, query row, and page of keys). Queries and
+// keys may have any magnitude that a float has, and theirs may cancel, so the exponents are added as integers before
+// anything is rounded. A row's code: its own two in bits 23 up (plus 256), the significand below. Beyond what a float holds
+// the factor ends at 2^-126 (products are below 2^26, so scores are nothing there) or at 2^127.
+__device__ __forceinline__ uint32_t score_code(const MmaArgs& m, int e) {
+    return static_cast<uint32_t>(min(max(e + m.scale_exp, -256), 255) + 256) << 23 | m.scale_mant;
+}
+__device__ __forceinline__ float score_factor(uint32_t code, int ek) {
+    const int e = min(max(static_cast<int>(code >> 23) - 256 + ek, -126), 127);
+    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23 | (code & 0x7FFFFFu));
+}
 
 // row of a column of the weights, and of the output
 template <uint32_t V>
@@ -375,13 +392,12 @@ __device__ __forceinline__ void fetch_queries(const MmaArgs& args, const PieceRe
 // Sines cost most, and the rows of one token share them: where a warp's rows at a time belong to one token, its lanes
 // work the token's pairs out between them, in tab (128 places of shared memory; NULL: none).
 template <int R, int DC, int NB, int G, int U>
-__device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRec& pc, uint8_t* dst, float* frow, int32_t* qpos,
+__device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRec& pc, uint8_t* dst, uint32_t* frow, int32_t* qpos,
                                               uint32_t at, uint32_t step, float2* tab, uint4* raw) {
     constexpr uint32_t kRowLanes = DC * 16u, kAtOnce = 32u / kRowLanes, V = Cfg<R, DC, NB, G>::V;
     const AttnArgs& a = args.a;
     const uint32_t lane = threadIdx.x & 31u, D = a.g.head_dim;
     const uint32_t sub = lane / kRowLanes, d0 = (lane % kRowLanes) * 8u;
-    const float sign = a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : 0.0f);
     const bool vec = args.q_vec != 0u, turn = a.rope.turns != nullptr, mine = d0 < D;
     const uint32_t half = a.rope.rot_dim >> 1, base = pc.row_tile * a.shape.rt, group = a.shape.group;
     uint32_t turned = 0xFFFFFFFFu;  // the token that tab holds
@@ -478,7 +494,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             if (r >= pc.rows) continue;
             const bool bad = m[u] == __builtin_huge_valf();
             const int e = bad ? 0 : kv_scale_exp(m[u]);
-            const float mul = exp2_int(-e) * sign;  // the sign of the scale is the query's here
+            const float mul = exp2_int(-e) * args.scale_sign;  // the sign of the scale is the query's here
             uint32_t h[2], l[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -494,8 +510,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             *reinterpret_cast<uint2*>(dst + to + R * 128u) = make_uint2(l[0], l[1]);
             if (d0 == 0u) {
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
-                // (at 1e-30 scores are zero all the same)
-                frow[col] = fmaxf(exp2_int(e) * (fabsf(a.scale) * kLog2e), 1e-30f);
+                frow[col] = score_code(args, e);
                 qpos[col] = pc.p0 + static_cast<int32_t>((base + r) / group);
             }
         }
@@ -969,7 +984,8 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                 float l[V];
 #pragma unroll
                 for (uint32_t i = 0; i < V; ++i) l[i] = 0.0f;
-                float M[kOwn], f_own[kOwn];
+                float M[kOwn];
+                uint32_t f_own[kOwn];
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
                     M[i] = kNegInf;
@@ -980,13 +996,14 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     const uint32_t vs = n % NV, use = n / G;
                     float(*wmax)[R] = sh.wmax[grp][use & 1u];  // (its last readers met since)
                     bar_wait(&sh.scfull[vs], (n / NV) & 1u, gave_up);
+                    const int ek0 = scale_exp_of(sh.kscale[vs][pg0]), ek1 = scale_exp_of(sh.kscale[vs][pg1]);
                     // From products to scores, base 2, by one factor a row and half of the warp's tokens (which may lie in
                     // two pages). A score is rounded here and nowhere later: the same value is compared and taken to its
                     // weight, so no weight is above 1 however large the scores are.
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) {
-                        my_fac[own + i] = f_own[i] * sh.kscale[vs][pg0];
-                        my_fac[R + own + i] = f_own[i] * sh.kscale[vs][pg1];
+                        my_fac[own + i] = score_factor(f_own[i], ek0);
+                        my_fac[R + own + i] = score_factor(f_own[i], ek1);
                     }
                     // exponents of the values' scales, relative to the tile's largest: they go into the weights.
                     // Where they differ by much, the weights' factor has to come from the largest product of
@@ -1344,6 +1361,15 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
                       rope_by_8(a.rope)
                   ? 1u
                   : 0u;
+    const double c = std::fabs(static_cast<double>(a.scale)) * 1.4426950408889634;
+    int e = 0;
+    float sig = static_cast<float>(2.0 * std::frexp(c, &e));  // in [1, 2)
+    if (sig >= 2.0f) sig = 1.0f, ++e;
+    uint32_t bits;
+    std::memcpy(&bits, &sig, sizeof(bits));
+    m.scale_mant = bits & 0x7FFFFFu;
+    m.scale_exp = e - 1;
+    m.scale_sign = a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : 0.0f);
     m.out_pair = ((reinterpret_cast<uintptr_t>(a.out.data) | 2u * a.out.token_stride | 2u * a.out.head_stride) & 3u) == 0 ? 1u : 0u;
     const uint64_t rows = static_cast<uint64_t>(max_new ? max_new : 1u) * a.shape.group;
     // rows of a row tile: what deals `rows` out evenly, in the blocks of 8 rows that the softmax works in (72 rows

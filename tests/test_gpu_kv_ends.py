@@ -1,6 +1,12 @@
-"""Attention over the 8-bit cache at the ends of its range."""
+"""Attention over the 8-bit cache at the ends of its range, against the definition in 64 bits (kv_reference.py).
+
+Tolerances as in test_gpu_kv.py: a score errs by (dim + 8) u R at most, R the row's largest sum of scale |q| |k|; a
+weight by a factor e^(2 err) and, with bf16 queries, by b / 2 for its 8 significant bits; the output by b / 2 for its type
+(u = 2^-24, b = 2^-8; b / 2 is half a last place)."""
 
 from __future__ import annotations
+
+import math
 
 import numpy as np
 import pytest
@@ -14,6 +20,7 @@ if not has_gpu():
 
 import torch  # noqa: E402
 
+import kv_reference as R  # noqa: E402
 from test_gpu_kv import B, BF, DEV, F32, U, World, host  # noqa: E402
 
 
@@ -25,10 +32,63 @@ def contents(w, k, v):
     return w
 
 
+def check(w, q, scale=None, window=0):
+    """q [new, query heads, dim] (host, of its type) over the cache's one sequence."""
+    n, length = q.shape[0], w.lens[0]
+    sc = w.dim ** -0.5 if scale is None else scale
+    out, lse, st = w.kv.attend(q.to(DEV), w.batch([n]), scale=scale, window=window)
+    assert st.tolist() == [0]
+    ro, rl, mag, reach = R.attend(w.rk, w.rv, w.table[0], length, host(q), sc, window)
+    bf = q.dtype == BF
+    err = (w.dim + 8) * U * reach
+    weights = 2 * err + (length / 16 + 64) * U + (B / 2 if bf else 0)
+    tol = weights * mag * math.e + (B / 2 if bf else 2 * U) * np.abs(ro) + 1e-30
+    got, gl = host(out), host(lse)
+    assert np.all(np.abs(got - ro) <= tol), float((np.abs(got - ro) / tol).max())
+    assert np.all(np.abs(gl - rl) <= err + (length / 16 + 64) * U + 4 * U * np.abs(rl))
+
+
+# ---------------------------------------------------------------------------------------------
+# scores: queries and keys whose magnitudes cancel
+
+
+@pytest.mark.parametrize("heads,group,dim,page", [(1, 4, 128, 64), (2, 8, 64, 16), (1, 20, 256, 32), (1, 64, 80, 128)])
+@pytest.mark.parametrize("mag", [1e-28, 1e-32, 1e-36, 1e-20, 1e20, 1e30, 1e33])
+def test_small_queries_on_large_keys_and_the_other_way_round(mag, heads, group, dim, page):
+    w = World(41, [400], page, heads, dim)
+    k = w.rng.normal(size=(400, heads, dim)) / mag
+    contents(w, np.clip(k, -3e38, 3e38), w.rng.normal(size=(400, heads, dim)))
+    for n in (1, 3):
+        check(w, torch.from_numpy(w.rng.normal(size=(n, heads * group, dim)) * mag).to(BF))
+
+
+@pytest.mark.parametrize("mag", [1e-32, 1e-28, 1e-20, 1e20, 1e28])
+def test_small_queries_on_large_keys_in_fp32(mag):
+    w = World(42, [400], 64, 2, 64)
+    contents(w, w.rng.normal(size=(400, 2, 64)) / mag, w.rng.normal(size=(400, 2, 64)))
+    check(w, torch.from_numpy(w.rng.normal(size=(3, 8, 64)) * mag).to(F32))
+
+
+def test_small_queries_over_pages_of_very_different_scales():
+    """Keys of some pages 2^90 times others', values too: the maxima of weight times value scale come from other tokens."""
+    w = World(43, [96], 16, 1, 64)
+    mag = np.repeat(2.0 ** np.array([90, 0, 85, 20, 89, -10]), 16)[:, None, None]
+    contents(w, w.rng.normal(size=(96, 1, 64)) * mag,
+             w.rng.normal(size=(96, 1, 64)) * np.repeat(2.0 ** np.array([0, -12, 9, -30, 3, 20]), 16)[:, None, None])
+    check(w, torch.from_numpy(w.rng.normal(size=(4, 2, 64)) * 2.0 ** -90).to(BF))
+
+
+@pytest.mark.parametrize("scale,mag", [(1e-30, 1e30), (1e-38, 1e36), (1e30, 1e-30), (3e38, 1e-38)])
+def test_scales_that_cancel_the_queries(scale, mag):
+    w = World(44, [300], 32, 1, 128)
+    contents(w, w.rng.normal(size=(300, 1, 128)) * 0.1, w.rng.normal(size=(300, 1, 128)))
+    check(w, torch.from_numpy(w.rng.normal(size=(2, 8, 128)) * mag).to(BF), scale=scale)
+
+
 @pytest.mark.parametrize("dt", [BF, F32])
 @pytest.mark.parametrize("heads,group,dim,page", [(1, 16, 64, 64), (2, 4, 128, 16), (1, 40, 128, 32), (1, 32, 256, 128)])
 def test_scores_beyond_24_bits(dt, heads, group, dim, page):
-    """One token far above the others, by scores from 12 to 10^29 whose roundings are whole numbers or more: its weight is
+    """One token far above the others, by scores from 20 to 10^29 whose roundings are whole numbers or more: its weight is
     1 and theirs 0 all the same. A score here is one product, so lse is off by the roundings of its factors only."""
     n, at = 300, 137
     w = World(45, [n], page, heads, dim)
