@@ -937,7 +937,7 @@ int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch*
     a.shape.window = window >= 0x3FFFFFFFu ? 0u : window;  // wider than any sequence
     a.shape.all = (flags & SIXI_KV_ATTEND_ALL) ? 1u : 0u;
     a.shape.n_heads = h->g.n_heads;
-    a.scale = scale;
+    a.score = score_scale(scale);
     a.lse = out_lse;
     a.status = out_status;
     a.part = h->part;

@@ -9,7 +9,9 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
+#include <cstring>
 
 #include "../../include/sixi_kv.h"
 
@@ -99,6 +101,40 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t v) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v & 0xFFFFu), __NV_E4M3);
     return __half22float2(__half2(h));
+}
+
+// ---------------------------------------------------------------------------------------------
+// from products to scores
+//
+// The factor is a significand times 2^(exponents of scale, query row, and page of keys). Queries and keys may have any
+// magnitude that a float has, and theirs may cancel, so rows are brought to e4m3's range and the exponents are added as
+// integers before anything is rounded.
+struct ScoreScale {  // |scale| log2(e) = (1 + mant / 2^23) 2^exp; the sign (0: a scale of 0) goes to the queries
+    uint32_t mant;
+    int32_t exp;
+    float sign;
+};
+
+inline ScoreScale score_scale(float scale) {
+    int e = 0;
+    float sig = static_cast<float>(2.0 * std::frexp(std::fabs(static_cast<double>(scale)) * 1.4426950408889634, &e));
+    if (sig >= 2.0f) sig = 1.0f, ++e;  // (it was in [1, 2) before it was rounded)
+    ScoreScale s;
+    std::memcpy(&s.mant, &sig, sizeof(sig));
+    s.mant &= 0x7FFFFFu;
+    s.exp = e - 1;
+    s.sign = scale < 0.0f ? -1.0f : (scale > 0.0f ? 1.0f : 0.0f);
+    return s;
+}
+
+// A row's code, its elements divided by 2^e: its exponents in bits 23 up (plus 256), the significand below. Beyond what a
+// float holds the factor ends at 2^-126 (products are below 2^26, so scores are nothing there) or at 2^127.
+__device__ __forceinline__ uint32_t score_code(const ScoreScale& s, int e) {
+    return static_cast<uint32_t>(min(max(e + s.exp, -256), 255) + 256) << 23 | s.mant;
+}
+__device__ __forceinline__ float score_factor(uint32_t code, int ek) {
+    const int e = min(max(static_cast<int>(code >> 23) - 256 + ek, -126), 127);
+    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23 | (code & 0x7FFFFFu));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -487,7 +523,7 @@ struct AttnArgs {
     KvView q, out;
     RopeView rope;
     AttnShape shape;
-    float scale;
+    ScoreScale score;
     float* lse;
     int32_t* status;
     float* part;        // [2 * ctas][part_stride]

@@ -24,7 +24,6 @@ constexpr int kRt = 16;         // rows of a row tile
 constexpr int kTileShift = 6;   // 64 tokens
 constexpr int kT = 1 << kTileShift;
 constexpr uint32_t kWindow = 32;  // tiles whose page ids are kept
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool on) {
@@ -34,7 +33,7 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool on) 
 }
 
 struct Smem {
-    float* q;       // [kRt][D], times scale * log2(e)
+    float* q;       // [kRt][D], a row divided by a power of two
     uint8_t* kv;    // [2 stages][2][kT][D + 16]
     float* tok;     // [2 stages][2][kT] scales of the tile's tokens
     float* s;       // [kRt][kT]
@@ -96,6 +95,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     __shared__ SeqPlan found;
     __shared__ uint32_t last_flag;
     __shared__ int32_t ids[kWindow * 4];
+    __shared__ uint32_t code[kRt];  // of score_factor
     const uint32_t tid = threadIdx.x, D = a.g.head_dim, row = D + 16u;
     Smem sm;
     {
@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         load_ids(a, pc, lo, pc.t0, ids);
         __syncthreads();
         load_tile(a, sm, pc, lo, pc.t0, 0, ids);
-        // queries, turned, then scaled; a NaN or Inf makes the row NaN
+        // queries, turned; then a row is divided by a power of two, which keeps its products with the cached bytes within
+        // fp32's range. A NaN or Inf makes the row NaN.
         for (uint32_t i = tid; i < kRt * D; i += kNT) {
             const uint32_t r = i / D, d = i - r * D;
             float x = 0.0f;
@@ -142,9 +143,24 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
                 const float* p = static_cast<const float*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
                              (pc.head * a.shape.group + g) * a.q.head_stride;
                 load_turned<float, 1>(a.rope, p, d, pc.plan.p0 + static_cast<int32_t>(tok), &x);
-                x = fabsf(x) < __builtin_huge_valf() ? x * (a.scale * kLog2e) : __uint_as_float(0x7FC00000u);
             }
             sm.q[i] = x;
+        }
+        __syncthreads();
+        for (uint32_t r = tid >> 5; r < kRt; r += kNT / 32) {
+            const uint32_t lane = tid & 31u;
+            float m = 0.0f;
+            for (uint32_t d = lane; d < D; d += 32u) {
+                const float ab = fabsf(sm.q[r * D + d]);
+                m = ab < __builtin_huge_valf() ? fmaxf(m, ab) : __builtin_huge_valf();
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            const bool bad = m == __builtin_huge_valf();
+            const int e = bad ? 0 : kv_scale_exp(m);
+            const float mul = bad ? __uint_as_float(0x7FC00000u) : exp2_int(-e) * a.score.sign;
+            for (uint32_t d = lane; d < D; d += 32u) sm.q[r * D + d] *= mul;
+            if (lane == 0) code[r] = score_code(a.score, e);
         }
         if (tid < kRt) sm.m[tid] = kNegInf, sm.l[tid] = 0.0f;
         float acc[kRt][4];
@@ -185,13 +201,13 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
                         }
                     }
                     const int32_t pos = tile * kT + static_cast<int32_t>(t);
-                    const float f = sm.tok[st * 2u * kT + t];
+                    const int ek = scale_exp_of(sm.tok[st * 2u * kT + t]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int32_t qp = pc.plan.p0 + static_cast<int32_t>((r_base + r0 + r) / a.shape.group);
                         bool on = pos < pc.plan.len && (a.shape.all || pos <= qp);
                         if (a.shape.window) on = on && pos > qp - static_cast<int32_t>(a.shape.window);
-                        sm.s[(r0 + r) * kT + t] = on ? s[r] * f : kNegInf;
+                        sm.s[(r0 + r) * kT + t] = on ? s[r] * score_factor(code[r0 + r], ek) : kNegInf;
                     }
                 }
             }

@@ -47,8 +47,6 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
-#include <cmath>
-#include <cstring>
 
 #include "smp_kernels.cuh"
 #include "smp_kv.cuh"
@@ -340,23 +338,7 @@ struct MmaArgs {
     uint32_t read_once;  // no page is read by more than one row tile
     uint32_t out_pair;   // two elements of an output row can be stored together
     uint32_t q_vec;  // 8 query elements can be loaded (and are turned) together
-    // |scale| log2(e) = (1 + mant / 2^23) 2^exp; the sign goes to the queries (0: a scale of 0)
-    uint32_t scale_mant;
-    int32_t scale_exp;
-    float scale_sign;
 };
-
-// The factor from products to scores is a significand times 2^(exponents of scale, query row, and page of keys). Queries and
-// keys may have any magnitude that a float has, and theirs may cancel, so the exponents are added as integers before
-// anything is rounded. A row's code: its own two in bits 23 up (plus 256), the significand below. Beyond what a float holds
-// the factor ends at 2^-126 (products are below 2^26, so scores are nothing there) or at 2^127.
-__device__ __forceinline__ uint32_t score_code(const MmaArgs& m, int e) {
-    return static_cast<uint32_t>(min(max(e + m.scale_exp, -256), 255) + 256) << 23 | m.scale_mant;
-}
-__device__ __forceinline__ float score_factor(uint32_t code, int ek) {
-    const int e = min(max(static_cast<int>(code >> 23) - 256 + ek, -126), 127);
-    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23 | (code & 0x7FFFFFu));
-}
 
 // row of a column of the weights, and of the output
 template <uint32_t V>
@@ -494,7 +476,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             if (r >= pc.rows) continue;
             const bool bad = m[u] == __builtin_huge_valf();
             const int e = bad ? 0 : kv_scale_exp(m[u]);
-            const float mul = exp2_int(-e) * args.scale_sign;  // the sign of the scale is the query's here
+            const float mul = exp2_int(-e) * a.score.sign;  // the sign of the scale is the query's here
             uint32_t h[2], l[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -510,7 +492,7 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
             *reinterpret_cast<uint2*>(dst + to + R * 128u) = make_uint2(l[0], l[1]);
             if (d0 == 0u) {
                 const uint32_t col = ((r >> 1) & 3u) * V + (r >> 3) * 2u + (r & 1u);
-                frow[col] = score_code(args, e);
+                frow[col] = score_code(a.score, e);
                 qpos[col] = pc.p0 + static_cast<int32_t>((base + r) / group);
             }
         }
@@ -1361,15 +1343,6 @@ cudaError_t launch_attend_bf16(const AttnArgs& a, const CUtensorMap& k_map, cons
                       rope_by_8(a.rope)
                   ? 1u
                   : 0u;
-    const double c = std::fabs(static_cast<double>(a.scale)) * 1.4426950408889634;
-    int e = 0;
-    float sig = static_cast<float>(2.0 * std::frexp(c, &e));  // in [1, 2)
-    if (sig >= 2.0f) sig = 1.0f, ++e;
-    uint32_t bits;
-    std::memcpy(&bits, &sig, sizeof(bits));
-    m.scale_mant = bits & 0x7FFFFFu;
-    m.scale_exp = e - 1;
-    m.scale_sign = a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : 0.0f);
     m.out_pair = ((reinterpret_cast<uintptr_t>(a.out.data) | 2u * a.out.token_stride | 2u * a.out.head_stride) & 3u) == 0 ? 1u : 0u;
     const uint64_t rows = static_cast<uint64_t>(max_new ? max_new : 1u) * a.shape.group;
     // rows of a row tile: what deals `rows` out evenly, in the blocks of 8 rows that the softmax works in (72 rows

@@ -105,3 +105,12 @@ def test_scores_beyond_24_bits(dt, heads, group, dim, page):
     assert np.all(np.abs(host(out) - want) <= b * np.abs(want) + 1e-9)
     score = host(q)[:, :, 0] * dim ** -0.5
     assert np.all(np.abs(host(lse) - score) <= 6 * U * score)
+
+
+@pytest.mark.parametrize("mag", [1e-36, 1e-33, 1e33, 1e36, 1e37])
+def test_queries_near_the_ends_of_fp32(mag):
+    """A product of a query element and a cached byte may pass fp32's range although the score does not."""
+    w = World(46, [400], 64, 2, 128)
+    k = w.rng.normal(size=(400, 2, 128)) / mag
+    contents(w, np.clip(k, -3e38, 3e38), w.rng.normal(size=(400, 2, 128)))
+    check(w, torch.from_numpy(w.rng.normal(size=(3, 8, 128)) * mag).to(F32))
