@@ -3,9 +3,9 @@
 //
 // Mathematics. Both products are fp8 products with fp32 accumulation, and the 16-bit side of each is
 // split into two e4m3 terms that are multiplied side by side:
-//   S^T = K (q_hi + q_lo)^T       a bf16 value has 8 significant bits, an e4m3 one has 4: after a row is
+//   S^T = K (q_hi + q_lo / 16)^T  a bf16 value has 8 significant bits, an e4m3 one has 4: after a row is
 //                                 scaled by a power of two the split is exact (but for elements below
-//                                 1/1792 of the row's largest, which err by 2^-19 of it at most)
+//                                 1/14,336 of the row's largest, which err by 2^-21.8 of it at most)
 //   O^T = V^T (w_hi + w_lo)       weights keep 8 significant bits, as bf16 weights would
 // The scale of a page and head is a power of two, so it multiplies scores and weights exactly. Weights
 // are scaled by a power of two per tile and row such that the tile's largest lies in (128, 256]; the tile's
@@ -369,6 +369,10 @@ __device__ __forceinline__ void fetch_queries(const MmaArgs& args, const PieceRe
     }
 }
 
+// A query's lo row holds 16 times what its hi row leaves: a query is up to 448 after scaling, so hi leaves 16 at most, and e4m3's
+// last places reach 16 times further down.
+constexpr float kLoQuery = 16.0f;
+
 // A piece's queries as e4m3 hi and lo rows at dst (128-byte swizzle). raw: the first rows' elements, already asked for
 // (fetch_queries); further ones are asked for a round ahead, as a load may take microseconds while the pages stream in.
 // Sines cost most, and the rows of one token share them: where a warp's rows at a time belong to one token, its lanes
@@ -484,7 +488,8 @@ __device__ __forceinline__ void stage_queries(const MmaArgs& args, const PieceRe
                 const float v2 = x[u][4 * j + 2] * mul, v3 = x[u][4 * j + 3] * mul;
                 h[j] = e4m3x2(v0, v1) | (e4m3x2(v2, v3) << 16);
                 const float2 h01 = e4m3x2_to_float2(h[j]), h23 = e4m3x2_to_float2(h[j] >> 16);
-                l[j] = e4m3x2(v0 - h01.x, v1 - h01.y) | (e4m3x2(v2 - h23.x, v3 - h23.y) << 16);
+                l[j] = e4m3x2((v0 - h01.x) * kLoQuery, (v1 - h01.y) * kLoQuery) |
+                       (e4m3x2((v2 - h23.x) * kLoQuery, (v3 - h23.y) * kLoQuery) << 16);
                 if (bad) h[j] = 0x7F7F7F7Fu, l[j] = 0u;  // a NaN or Inf makes the row NaN
             }
             const uint32_t to = (d0 >> 7) * (2u * R * 128u) + r * 128u + ((((d0 & 127u) >> 4) ^ (r & 7u)) << 4) + (d0 & 8u);
@@ -1021,7 +1026,8 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                             const float2 a1 = *reinterpret_cast<const float2*>(my_fac + R + q * V + 2 * j);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const F2 sum = add2(f2(f[j - j0][2 * i], f[j - j0][2 * i + 1]), f2(g[j - j0][2 * i], g[j - j0][2 * i + 1]));
+                                const F2 sum = fma2(f2(g[j - j0][2 * i], g[j - j0][2 * i + 1]), f2(1.0f / kLoQuery, 1.0f / kLoQuery),
+                                                    f2(f[j - j0][2 * i], f[j - j0][2 * i + 1]));
                                 const float2 y = un2(mul2(sum, i < 2 ? f2(a0.x, a0.y) : f2(a1.x, a1.y)));
                                 x[j][0][i] = y.x, x[j][1][i] = y.y;
                             }

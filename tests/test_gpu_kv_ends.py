@@ -1,8 +1,8 @@
 """Attention over the 8-bit cache at the ends of its range, against the definition in 64 bits (kv_reference.py).
 
 Tolerances as in test_gpu_kv.py: a score errs by (dim + 8) u R at most, R the row's largest sum of scale |q| |k|; a
-weight by a factor e^(2 err) and, with bf16 queries, by b / 2 for its 8 significant bits; the output by b / 2 for its type
-(u = 2^-24, b = 2^-8; b / 2 is half a last place)."""
+weight by a factor e^(2 err) and, with bf16 queries, by 2^-9 (its two terms) + 2^-11 (its fp16 form on the way); the output
+by its type (u = 2^-24, b = 2^-8)."""
 
 from __future__ import annotations
 
@@ -41,8 +41,8 @@ def check(w, q, scale=None, window=0):
     ro, rl, mag, reach = R.attend(w.rk, w.rv, w.table[0], length, host(q), sc, window)
     bf = q.dtype == BF
     err = (w.dim + 8) * U * reach
-    weights = 2 * err + (length / 16 + 64) * U + (B / 2 if bf else 0)
-    tol = weights * mag * math.e + (B / 2 if bf else 2 * U) * np.abs(ro) + 1e-30
+    weights = 2 * err + (length / 16 + 64) * U + (2.0 ** -9 + 2.0 ** -11 if bf else 0)
+    tol = weights * mag * math.e + (B if bf else 2 * U) * np.abs(ro) + 1e-30
     got, gl = host(out), host(lse)
     assert np.all(np.abs(got - ro) <= tol), float((np.abs(got - ro) / tol).max())
     assert np.all(np.abs(gl - rl) <= err + (length / 16 + 64) * U + 4 * U * np.abs(rl))
@@ -114,3 +114,21 @@ def test_queries_near_the_ends_of_fp32(mag):
     k = w.rng.normal(size=(400, 2, 128)) / mag
     contents(w, np.clip(k, -3e38, 3e38), w.rng.normal(size=(400, 2, 128)))
     check(w, torch.from_numpy(w.rng.normal(size=(3, 8, 128)) * mag).to(F32))
+
+
+# ---------------------------------------------------------------------------------------------
+# bits: bf16 queries and weights are split into two e4m3 terms
+
+
+@pytest.mark.parametrize("dim,group", [(64, 8), (128, 40), (256, 32)])
+def test_small_elements_of_a_query_keep_their_bits(dim, group):
+    """A query whose largest element, 900 to 14,000 times the others, meets keys that are zero there: the scores come from
+    the others alone, exactly."""
+    w = World(47, [200], 32, 1, dim)
+    k = w.rng.normal(size=(200, 1, dim)) * 20
+    k[:, :, 0] = 0.0
+    contents(w, k, w.rng.normal(size=(200, 1, dim)))
+    q = w.rng.normal(size=(3, group, dim)) * 0.5
+    q[:, :, 0] = 500.0 * 2.0 ** w.rng.uniform(0, 4, size=(3, group))
+    q[:, :, 1:] *= (np.abs(q[:, :, 1:]) > q[:, :, :1] / 13_000)
+    check(w, torch.from_numpy(q).to(BF), scale=1.0 / (20 * dim ** 0.5))
