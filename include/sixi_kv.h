@@ -164,9 +164,12 @@ SIXI_SMP_API int32_t sixi_kv_read(sixi_kv* h, const sixi_kv_batch* batch, const 
  *             from then on for every call of the handle)
  * n_tokens * n_q_heads / n_kv_heads < 2^30, and the call's tiles of 8 rows by 64 positions < 2^40.
  * Pages that lie wholly before every row's window are not read, and their table entries may be anything.
- * Sums and softmax statistics are fp32. With bf16 queries the weights exp(s_t - m) enter the product
- * with the values with 8 significant bits (as bf16 weights would), and the products run on the tensor
- * cores straight from the cached bytes; with fp32 queries everything is fp32.
+ * Sums and softmax statistics are fp32. With fp32 queries everything is. With bf16 queries the products
+ * run on the tensor cores straight from the cached bytes, and the weights exp(s_t - m) enter theirs
+ * rounded: 8 significant bits (as bf16 weights would have) for those above 2^-13 of the largest of
+ * their tile (positions 128 i to 128 i + 127), and an error of 2^-21.6 of that largest weight at most for
+ * smaller ones. That is less than the output's own rounding, unless the tokens with the large weights
+ * have values near zero and only the small ones' sum is left (fp32 queries keep it).
  */
 enum { SIXI_KV_ATTEND_ALL = 1u };
 SIXI_SMP_API int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch* batch, float scale,

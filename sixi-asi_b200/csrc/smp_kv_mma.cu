@@ -6,14 +6,16 @@
 //   S^T = K (q_hi + q_lo / 16)^T  a bf16 value has 8 significant bits, an e4m3 one has 4: after a row is
 //                                 scaled by a power of two the split is exact (but for elements below
 //                                 1/14,336 of the row's largest, which err by 2^-21.8 of it at most)
-//   O^T = V^T (w_hi + w_lo)       weights keep 8 significant bits, as bf16 weights would
+//   O^T = V^T (w_hi + w_lo / 32)  weights keep 8 significant bits, as bf16 weights would, down to 2^-13 of the largest of
+//                                 their tile
 // The scale of a page and head is a power of two, so it multiplies scores and weights exactly. Weights
 // are scaled by a power of two per tile and row such that the tile's largest lies in (128, 256]; the tile's
 // product is added to fp32 sums in registers with the factor taken out again, so a row whose running
 // maximum lies far above a tile (a sink token) does not push that tile's weights below e4m3's range.
 //
-// Weights below 2^-18 of the tile's largest lose bits, below 2^-23 they vanish: for a tile's 128 tokens
-// together less than 2^-16 of its sum.
+// A weight below 2^-13 of its tile's largest is off by 2^-21.6 of that at most (the last place of the low term, and of the
+// weight's fp16 form), so the tile's 128 tokens together by 2^-14.6 of its sum. It shows only where the tokens with the
+// large weights have values near zero and the others' sum is all that is left (fp32 queries keep it).
 //
 // Layout. Tokens are the M side of the scores (128 of them a tile, one per TMEM lane), query rows the N
 // side (16 to 64: the query heads of one key head times new tokens); head elements are the M side of the
@@ -246,15 +248,15 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
     return r;
 }
 
-// Two weights in [0, 1] as e4m3 codes of 256 times their value: hi = the nearest, lo = 16 times what hi leaves.
+// Two weights in [0, 1] as e4m3 codes of 256 times their value: hi = the nearest, lo = 32 times what hi leaves (8 at most).
 // In f16, w has the exponent field that 256 w has in e4m3 (and subnormals have the same steps times 2^-7), so
 // hi's code is w's f16 pattern rounded at bit 7. hi: the codes in bytes 0 and 2; lo: in bytes 0 and 1.
-constexpr float kLoInv = 1.0f / 16.0f;
+constexpr float kLoInv = 1.0f / 32.0f;
 __device__ __forceinline__ void split2(F2 w, uint32_t* hi, uint32_t* lo) {
     const float2 f = un2(w);
     const __half2 h = __floats2half2_rn(f.x, f.y);
     const uint32_t top = (*reinterpret_cast<const uint32_t*>(&h) + 0x00400040u) & 0xFF80FF80u;
-    const __half2_raw rest = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&top)), __float2half2_rn(4096.0f));
+    const __half2_raw rest = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&top)), __float2half2_rn(8192.0f));
     *hi = top >> 7;
     *lo = __nv_cvt_halfraw2_to_fp8x2(rest, __NV_SATFINITE, __NV_E4M3);
 }

@@ -132,3 +132,29 @@ def test_small_elements_of_a_query_keep_their_bits(dim, group):
     q[:, :, 0] = 500.0 * 2.0 ** w.rng.uniform(0, 4, size=(3, group))
     q[:, :, 1:] *= (np.abs(q[:, :, 1:]) > q[:, :, :1] / 13_000)
     check(w, torch.from_numpy(q).to(BF), scale=1.0 / (20 * dim ** 0.5))
+
+
+@pytest.mark.parametrize("group", [8, 16, 32, 40, 64])
+def test_weights_above_2_13_of_the_largest_keep_8_bits(group):
+    """Two tokens, the heavier one's value zero: the output is the lighter one's weight, here 2^-13 to 2^-14 of the largest,
+    times its values. Eight significands of those tell within which bounds the weight is, whatever the output's type rounds
+    away. It may be off by 2^-9 (its two terms) + 2^-11 (its fp16 form on the way), and its exponent by the roundings of
+    two scores below 32 and of the exponential."""
+    w = World(48, [2], 16, 1, 64)
+    k = np.zeros((2, 1, 64))
+    k[0, 0, 0] = k[1, 0, 1] = 1.0
+    k[1, 0, 2] = 2.0 ** -4
+    v = np.zeros((2, 1, 64))
+    v[1, 0] = 1.0 + np.arange(64) % 8 / 8
+    contents(w, k, v)
+    q = np.zeros((64, group, 64))
+    q[:, :, 0] = 16.0
+    q[:, :, 1] = 16.0 - w.rng.uniform(9.1, 9.6, size=(64, group))
+    q[:, :, 2] = w.rng.uniform(0, 0.5, size=(64, group))
+    q = torch.from_numpy(q).to(BF)
+    gap = host(q)[:, :, 0] - host(q)[:, :, 1] - host(q)[:, :, 2] / 16
+    out = np.concatenate([host(w.kv.attend(q[i:i + 1].to(DEV), w.batch([1]), scale=1.0)[0]) for i in range(64)])
+    half = 2.0 ** (np.floor(np.log2(out)) - 8)  # half a last place
+    at_least, at_most = ((out - half) / v[1, 0]).max(-1), ((out + half) / v[1, 0]).min(-1)
+    want, off = 1.0 / (1.0 + np.exp(gap)), 2.0 ** -9 + 2.0 ** -11 + 100 * U
+    assert np.all(want >= at_least / (1 + off)) and np.all(want <= at_most / (1 - off))
