@@ -54,14 +54,15 @@ struct RopeView {
 struct KvSeq {
     int64_t row0;  // first row in the call's tensors
     int32_t n, len;
-    bool ok;
+    bool ok, in_order;  // in_order: its offsets are, and within the call's rows
 };
 
 __device__ __forceinline__ KvSeq kv_seq_of(const KvBatchView& b, uint32_t page_shift, int64_t r0, int64_t r1, int32_t len) {
     KvSeq q;
     q.row0 = r0;
     q.len = len;
-    q.ok = r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(b.n_tokens) && len >= 0 &&
+    q.in_order = r0 >= 0 && r1 >= r0 && r1 <= static_cast<int64_t>(b.n_tokens);
+    q.ok = q.in_order && len >= 0 &&
            static_cast<uint64_t>(len) <= (static_cast<uint64_t>(b.max_pages) << page_shift);
     q.n = q.ok ? static_cast<int32_t>(r1 - r0) : 0;
     return q;
@@ -280,6 +281,7 @@ struct SeqPlan {
     uint32_t paired;      // row tiles laid in pairs
     uint32_t weight;      // virtual tiles of a pair or unit
     uint32_t lanes;       // pairs or units per head
+    bool in_order;        // as KvSeq
 };
 
 __device__ __forceinline__ void unit_tiles(const AttnShape& a, const SeqPlan& s, uint32_t j, int32_t* first,
@@ -297,7 +299,7 @@ __device__ __forceinline__ void unit_tiles(const AttnShape& a, const SeqPlan& s,
 __device__ __forceinline__ SeqPlan plan_seq(const AttnShape& a, const KvBatchView& b, uint32_t page_shift, uint32_t s) {
     const KvSeq q = kv_seq(b, page_shift, s);
     SeqPlan p;
-    p.n = q.n, p.len = q.ok ? q.len : 0, p.row0 = q.row0;
+    p.n = q.n, p.len = q.ok ? q.len : 0, p.row0 = q.row0, p.in_order = q.in_order;
     p.p0 = p.len - p.n;
     const uint32_t rows = static_cast<uint32_t>(p.n) * a.group;
     p.nr = (rows + a.rt - 1) / a.rt;
@@ -413,12 +415,13 @@ __device__ __forceinline__ bool next_piece(const AttnShape& a, const KvBatchView
 }
 
 // The line's total and this CTA's start on it: every thread of the block calls (NT threads); `scratch` is NT / 32 + 2
-// shared 64-bit words, `found` takes the plan of the sequence that the CTA starts in. Returns false when the CTA has
-// nothing to do. *ctas: CTAs that share the line.
+// shared 64-bit words, `found` takes the plan of the sequence that the CTA starts in, `disorder` (shared, zero before)
+// whether any sequence's offsets are out of order. Returns false when the CTA has nothing to do. *ctas: CTAs that share the
+// line.
 template <int NT>
 __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView& b, uint32_t page_shift,
-                                          unsigned long long* scratch, SeqPlan* found, PieceWalk* w, uint64_t* total_out,
-                                          uint32_t* ctas) {
+                                          unsigned long long* scratch, SeqPlan* found, uint32_t* disorder, PieceWalk* w,
+                                          uint64_t* total_out, uint32_t* ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr uint64_t kTiles = (1ull << 40) - 1ull;  // tiles in the low 40 bits, units above them
     uint64_t total = 0;
@@ -431,11 +434,12 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
             const uint32_t s = s0 + threadIdx.x;
             uint64_t mine = 0;
             SeqPlan p;
-            bool small = true;
+            bool small = true, in_order = true;
             if (s < b.n_seqs) {
                 p = plan_seq(a, b, page_shift, s);
                 mine = plan_tiles(a, p) | (static_cast<uint64_t>(p.lanes) * a.n_heads << 40);
                 small = !p.paired && p.weight <= kWholeTiles + a.unit_cost;
+                in_order = p.in_order;
             }
             uint64_t incl = mine;
 #pragma unroll
@@ -445,6 +449,7 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
             }
             __syncthreads();
             if (lane == 31) scratch[warp] = incl;
+            if (!in_order) *disorder = 1u;
             if (pass == 0) whole = __syncthreads_and(small && whole) != 0;
             else __syncthreads();
             uint64_t all = 0, prev = 0;

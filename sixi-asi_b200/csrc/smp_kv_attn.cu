@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ unsigned long long scratch[kNT / 32 + 2];
     __shared__ SeqPlan found;
-    __shared__ uint32_t last_flag;
+    __shared__ uint32_t last_flag, disorder;
     __shared__ int32_t ids[kWindow * 4];
     __shared__ uint32_t code[kRt];  // of score_factor
     const uint32_t tid = threadIdx.x, D = a.g.head_dim, row = D + 16u;
@@ -110,15 +110,17 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         sm.m = f, f += kRt;
         sm.l = f;
     }
-    for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
-        const bool ok = kv_offsets_ok(a.b, tid, kNT) && seq_pages_ok(a.shape, a.b, a.g.page_shift, a.g.n_pages, s, tid, kNT);
-        const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
-        if (tid == 0) a.status[s] = a.counter[kAttnMaxCtas] ? SIXI_BACKEND_ERROR : (bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK);
-    }
+    if (tid == 0) disorder = 0u;
     PieceWalk walk;
     uint64_t total;
     uint32_t ctas;
-    if (!walk_init<kNT>(a.shape, a.b, a.g.page_shift, scratch, &found, &walk, &total, &ctas)) return;
+    const bool busy = walk_init<kNT>(a.shape, a.b, a.g.page_shift, scratch, &found, &disorder, &walk, &total, &ctas);
+    for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
+        const bool ok = disorder == 0u && seq_pages_ok(a.shape, a.b, a.g.page_shift, a.g.n_pages, s, tid, kNT);
+        const bool bad = __syncthreads_or(ok ? 0 : 1) != 0;
+        if (tid == 0) a.status[s] = a.counter[kAttnMaxCtas] ? SIXI_BACKEND_ERROR : (bad ? SIXI_OUT_OF_BOUNDS : SIXI_OK);
+    }
+    if (!busy) return;
 
     const uint32_t quads = D / 4u, groups = kNT / quads;
     const uint32_t quad = tid % quads, tg = tid / quads;

@@ -319,7 +319,7 @@ struct Shared {
     SeqPlan found;
     PieceRec piece[kPieces], split[2];
     uint64_t total;
-    uint32_t tmem, gave_up, ctas, pieces_done, split_mask, join_mask;
+    uint32_t tmem, gave_up, ctas, pieces_done, split_mask, join_mask, disorder;
     float kscale[kNV][8], vscale[kNV][8];   // by page of the tile
     // by column of the weights:
     uint32_t frow[kQSlots][R];              // a row's factor from products to scores: score_factor's code
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
             bar_init(&sh.lfull, 4 * G);
             bar_init(&sh.lempty, 4);
             bar_init(&sh.done, 2);
-            sh.gave_up = sh.pieces_done = sh.split_mask = 0u;
+            sh.gave_up = sh.pieces_done = sh.split_mask = sh.disorder = 0u;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
         uint64_t total;
         uint32_t ctas;
         tc_before();
-        const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &sh.found, &walk, &total, &ctas);
+        const bool busy = walk_init<C::kThreads>(a.shape, a.b, shift, sh.scratch, &sh.found, &sh.disorder, &walk, &total, &ctas);
         if (warp == C::kThreads / 32 - 1) {
             Piece pc;
             const bool any = busy && next_piece(a.shape, a.b, shift, walk, &pc);
@@ -1256,7 +1256,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
     if (warp == C::kThreads / 32 - 1) {
         // statuses, over the grid
         for (uint32_t s = blockIdx.x; s < a.b.n_seqs; s += gridDim.x) {
-            const bool ok = kv_offsets_ok(a.b, lane, 32u) && seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
+            const bool ok = sh.disorder == 0u && seq_pages_ok(a.shape, a.b, shift, a.g.n_pages, s, lane, 32u);
             const bool bad = __any_sync(kFull, !ok);
             if (lane == 0) {
                 volatile int32_t* st = a.status + s;
