@@ -5,7 +5,7 @@
  * chunk of a prompt). It has no counterpart in the engine, whose model execution is external.
  *
  * Conventions are those of sixi_smp.h: `extern "C"`, int32 status codes (the engine's ErrorCode
- * values), array arguments are DEVICE pointers, every call is asynchronous on the caller's stream
+ * values), array arguments are DEVICE pointers aligned to their elements, every call is asynchronous on the caller's stream
  * and neither synchronises nor allocates (create excepted), and failures of a single sequence are
  * reported in out_status without affecting the other sequences. A cache handle owns a workspace: its
  * calls are serialised by the caller (one stream, or streams ordered by events). A rotary handle is

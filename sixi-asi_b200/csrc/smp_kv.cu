@@ -706,9 +706,13 @@ bool tensor_ok(const sixi_kv_tensor* t, uint64_t n_tokens) {
     return (reinterpret_cast<uintptr_t>(t->data) & (t->dtype == SIXI_SMP_BF16 ? 1u : 3u)) == 0;
 }
 
+// arrays that kernels read or write by elements of `size` bytes
+bool aligned(const void* p, uintptr_t size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1u)) == 0; }
+
 bool batch_ok(const sixi_kv* h, const sixi_kv_batch* b) {
     if (b == nullptr || b->n_seqs > h->max_seqs || b->n_tokens > 0x7FFFFFFFu) return false;
     if (b->n_seqs == 0) return b->n_tokens == 0;
+    if (!aligned(b->offsets, 8) || !aligned(b->lens, 4) || !aligned(b->page_table, 4)) return false;
     // (positions of a tile's end and of a window's beginning stay within 31 bits)
     return b->offsets != nullptr && b->lens != nullptr && b->page_table != nullptr && b->table_stride >= b->max_pages &&
            b->max_pages > 0 && static_cast<uint64_t>(b->max_pages) * h->g.page_size <= (1ull << 30);
@@ -877,7 +881,7 @@ int32_t sixi_kv_rope_apply(const sixi_kv_rope* r, const sixi_kv_tensor* x, const
         x->n_heads != out->n_heads || head_dim < r->v.rot_dim || head_dim > 65536)
         return SIXI_INVALID_ARGUMENT;
     if (n_tokens == 0) return SIXI_OK;
-    if (positions == nullptr || n_tokens > 0x7FFFFFFFu) return SIXI_INVALID_ARGUMENT;
+    if (positions == nullptr || !aligned(positions, 4) || n_tokens > 0x7FFFFFFFu) return SIXI_INVALID_ARGUMENT;
     KvDeviceGuard guard(r->device);
     RopeView view = r->v;
     if (inverse) view.amp_sin = -view.amp_sin;
@@ -892,7 +896,7 @@ int32_t sixi_kv_append(sixi_kv* h, const sixi_kv_tensor* k, const sixi_kv_tensor
         return SIXI_INVALID_ARGUMENT;
     if (rope != nullptr && (rope->device != h->device || rope->v.rot_dim > h->g.head_dim)) return SIXI_INVALID_ARGUMENT;
     if (b->n_seqs == 0) return SIXI_OK;
-    if (out_status == nullptr) return SIXI_INVALID_ARGUMENT;
+    if (out_status == nullptr || !aligned(out_status, 4)) return SIXI_INVALID_ARGUMENT;
     KvDeviceGuard guard(h->device);
     const RopeView none{nullptr, 1.0f, 1.0f, 0u, 0u};
     return kv_from_cuda(launch_kv_append(h->g, batch_view(b), k, v, rope ? rope->v : none, b->max_new, out_status,
@@ -905,7 +909,7 @@ int32_t sixi_kv_read(sixi_kv* h, const sixi_kv_batch* b, const sixi_kv_tensor* k
         k->dtype != v->dtype || k->n_heads != h->g.n_heads || v->n_heads != h->g.n_heads)
         return SIXI_INVALID_ARGUMENT;
     if (b->n_seqs == 0) return SIXI_OK;
-    if (out_status == nullptr) return SIXI_INVALID_ARGUMENT;
+    if (out_status == nullptr || !aligned(out_status, 4)) return SIXI_INVALID_ARGUMENT;
     KvDeviceGuard guard(h->device);
     return kv_from_cuda(launch_kv_read(h->g, batch_view(b), k, v, out_status, static_cast<cudaStream_t>(stream)));
 }
@@ -924,7 +928,7 @@ int32_t sixi_kv_attend(sixi_kv* h, const sixi_kv_tensor* q, const sixi_kv_batch*
     // the schedule counts tiles (of 64 tokens and 8 rows at least) in 40 bits
     const double units = (b->n_tokens * static_cast<double>(group) / 8 + 2.0 * b->n_seqs) * h->g.n_heads;
     if (units * (b->max_pages * static_cast<double>(h->g.page_size) / 64 + 8) >= 1099511627776.0) return SIXI_INVALID_ARGUMENT;
-    if (out_status == nullptr) return SIXI_INVALID_ARGUMENT;
+    if (out_status == nullptr || !aligned(out_status, 4) || !aligned(out_lse, 4)) return SIXI_INVALID_ARGUMENT;
     KvDeviceGuard guard(h->device);
     AttnArgs a;
     std::memset(&a, 0, sizeof(a));
