@@ -11,7 +11,7 @@ Every step runs, for all streams at once, what a serving loop runs per layer and
 and then moves each stream's length on by what was accepted: rejected drafts stay behind the length and
 are written over. The cache is paged; pages are dealt to streams as they grow, out of one pool.
 
-    python examples/spec_decode_cache.py [--streams 8] [--tokens 48] [--drafts 4] [--plain]
+    python examples/spec_decode_cache.py [--streams 8] [--tokens 48] [--drafts 4] [--vocab 4096] [--plain]
 
 --plain drafts nothing and verifies one token a step. Both print the same tokens: a draft only changes
 how many positions a step covers.
@@ -83,13 +83,14 @@ class Pages:
         return torch.from_numpy(self.table).cuda()
 
 
-def decode(streams=8, tokens=48, drafts=4, prompt=24, seed=0):
+def decode(streams=8, tokens=48, drafts=4, prompt=24, seed=0, vocab=4096):
     """(generated tokens per stream, steps, tokens per step): greedy, so the drafts cannot change the text."""
-    model = Model(seed=seed)
+    model = Model(vocab=vocab, seed=seed)
     rng = np.random.default_rng(seed)
     hist = [list(rng.integers(0, model.vocab, prompt // 2)) * 2 for _ in range(streams)]
     start = len(hist[0])
-    pages = Pages(streams, 512, 32, start + tokens + drafts + 2)
+    stop = start + tokens
+    pages = Pages(streams, 512, 32, stop + drafts)
     smp = S.Sampler(0, streams * (drafts + 1), model.vocab)
     params = torch.from_numpy(S.make_params(streams, temperature=0.0).view(np.uint8)).cuda()
 
@@ -101,8 +102,8 @@ def decode(streams=8, tokens=48, drafts=4, prompt=24, seed=0):
     _, st = model.logits(flat, KvBatch(pages.reach([n] * streams), off, lens, streams * n, n))
     assert (st == 0).all()
 
-    steps = 0
-    while min(len(h) for h in hist) < start + tokens:
+    steps = written = worked = 0
+    while min(len(h) for h in hist) < stop:
         k = drafts
         if k:
             offs = np.concatenate([[0], np.cumsum([len(h) for h in hist])]).astype(np.int64)
@@ -125,12 +126,14 @@ def decode(streams=8, tokens=48, drafts=4, prompt=24, seed=0):
         else:
             tok, _ = smp.greedy_argmax(logits)
             out, count = tok.cpu().numpy()[:, None], np.ones(streams, np.int64)
-        for s in range(streams):  # a stream's length moves on by what was accepted
-            hist[s] += [int(t) for t in out[s, : count[s]]]
+        for s in range(streams):  # a stream's length moves on by what was accepted, up to the end of its text
+            if len(hist[s]) < stop:
+                written, worked = written + int(count[s]), worked + 1
+                hist[s] = (hist[s] + [int(t) for t in out[s, : count[s]]])[:stop]
         steps += 1
-    text = [h[start: start + tokens] for h in hist]
+    text = [h[start:] for h in hist]
     smp.close()
-    return text, steps, sum(len(h) - start for h in hist) / (steps * streams)
+    return text, steps, written / worked
 
 
 def main():
@@ -138,9 +141,10 @@ def main():
     ap.add_argument("--streams", type=int, default=8)
     ap.add_argument("--tokens", type=int, default=48)
     ap.add_argument("--drafts", type=int, default=4)
+    ap.add_argument("--vocab", type=int, default=4096, help="a small one repeats itself, so that drafts are accepted")
     ap.add_argument("--plain", action="store_true")
     a = ap.parse_args()
-    text, steps, rate = decode(a.streams, a.tokens, 0 if a.plain else a.drafts)
+    text, steps, rate = decode(a.streams, a.tokens, 0 if a.plain else a.drafts, vocab=a.vocab)
     print(f"{a.streams} streams x {a.tokens} tokens in {steps} steps, {rate:.2f} tokens a step")
     print("stream 0:", text[0])
 
