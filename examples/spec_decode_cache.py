@@ -13,8 +13,10 @@ are written over. The cache is paged; pages are dealt to streams as they grow, o
 
     python examples/spec_decode_cache.py [--streams 8] [--tokens 48] [--drafts 4] [--vocab 4096] [--plain]
 
---plain drafts nothing and verifies one token a step. Both print the same tokens: a draft only changes
-how many positions a step covers.
+--plain drafts nothing and verifies one token a step. Both choose the same tokens but for near-ties of two
+logits: a draft changes how many positions a step covers, so the order in which products are summed, and
+a rejected draft that was the largest of its page leaves the page's scale raised, and the page's older
+tokens rounded at that.
 """
 
 from __future__ import annotations
@@ -84,7 +86,8 @@ class Pages:
 
 
 def decode(streams=8, tokens=48, drafts=4, prompt=24, seed=0, vocab=4096):
-    """(generated tokens per stream, steps, tokens per step): greedy, so the drafts cannot change the text."""
+    """(generated tokens per stream, steps, tokens per step of a stream that is not done). Greedy: drafts change the
+    text by near-ties only."""
     model = Model(vocab=vocab, seed=seed)
     rng = np.random.default_rng(seed)
     hist = [list(rng.integers(0, model.vocab, prompt // 2)) * 2 for _ in range(streams)]

@@ -67,7 +67,9 @@ typedef struct sixi_kv_tensor {
  * position lens[s] - n_s + i, in page page_table[s * table_stride + position / page_size].
  * The same batch serves an append and the attention that follows it: lens counts the new tokens.
  * After verification has kept a of the k drafted tokens of a stream, its next lens continues from
- * lens - k + a: positions behind it are written over by the next append.
+ * lens - k + a: positions behind it are written over by the next append. What a rejected token leaves is
+ * the scale of its page, where it raised it (see sixi_kv_append): older tokens of that page stay as they
+ * were rounded at it, until the page is written from its first slot again.
  */
 typedef struct sixi_kv_batch {
     const int32_t* page_table;

@@ -10,7 +10,8 @@ A serving step on a batch of streams, before the sampler or the verifier sees it
 
 `batch` names each sequence's last offsets[s + 1] - offsets[s] positions: one token a stream for a
 decode step, 1 + k for speculative verification, a chunk of a prompt. After the verifier has accepted
-a of k drafts, lens for the next batch continues from lens - k + a.
+a of k drafts, lens for the next batch continues from lens - k + a. A rejected draft whose keys or values were
+the largest of its page leaves the page's scale raised, and its older tokens rounded at that.
 
 Calls run on the current stream, or on `stream`: what they allocate then belongs to that stream, and what
 they are given stays as it is until that stream is through with it. Which stream waits for which is the
