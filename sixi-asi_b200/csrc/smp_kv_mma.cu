@@ -145,7 +145,8 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0u;
 }
 // Barrier of a softmax group's four warps. It is not bounded, but its warps cannot miss it: they run through the same
-// tiles whatever happens to the waits, and agree before each piece on whether there is one (group_any).
+// tiles whatever happens to the waits, and agree on whatever they branch on around it (group_any): before each piece on
+// whether there is one, in each tile on whether its scales differ.
 __device__ __forceinline__ void group_sync(uint32_t grp) { asm volatile("bar.sync %0, 128;" ::"r"(2u + grp) : "memory"); }
 __device__ __forceinline__ bool group_any(uint32_t grp, bool x) {
     uint32_t y;
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     er = max(er, __shfl_xor_sync(kFull, er, 4));
                     er = max(er, __shfl_xor_sync(kFull, er, 2));
                     er = max(er, __shfl_xor_sync(kFull, er, 1));
-                    const bool wide = __any_sync(kFull, ep > -127 && ep < er - 4);
+                    const bool differ = __any_sync(kFull, ep > -127 && ep < er - 4);
                     const int ev0 = max(scale_exp_of(sh.vscale[vs][pg0]) - er, -126);
                     const int ev1 = max(scale_exp_of(sh.vscale[vs][pg1]) - er, -126);
                     const bool edge = t * kTile < safe_from || (t + 1) * kTile > reach;
@@ -1064,7 +1065,9 @@ __global__ void __launch_bounds__(Cfg<R, DC, NB, G>::kThreads, 1)
                     fold_lanes<kFold>(mx, lane, max_op);
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) wmax[quad][own + i] = mx[i];
-                    group_sync(grp);
+                    // (the group's warps agree on it: once waits have been given up, they may have read different scales, and
+                    // a warp that went through the two barriers below alone would wait there for good)
+                    const bool wide = group_any(grp, differ);
                     float mt[kOwn];
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i)
