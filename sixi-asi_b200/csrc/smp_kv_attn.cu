@@ -135,26 +135,18 @@ __global__ void __launch_bounds__(kNT, 2) attend_f32_kernel(AttnArgs a) {
         load_ids(a, pc, lo, pc.t0, ids);
         __syncthreads();
         load_tile(a, sm, pc, lo, pc.t0, 0, ids);
-        // queries, turned; then a row is divided by a power of two, which keeps its products with the cached bytes within
-        // fp32's range. A NaN or Inf makes the row NaN.
-        for (uint32_t i = tid; i < kRt * D; i += kNT) {
-            const uint32_t r = i / D, d = i - r * D;
-            float x = 0.0f;
-            if (r < pc.rows) {
-                const uint32_t tok = (r_base + r) / a.shape.group, g = (r_base + r) - tok * a.shape.group;
-                const float* p = static_cast<const float*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
-                             (pc.head * a.shape.group + g) * a.q.head_stride;
-                load_turned<float, 1>(a.rope, p, d, pc.plan.p0 + static_cast<int32_t>(tok), &x);
-            }
-            sm.q[i] = x;
-        }
-        __syncthreads();
+        // Queries, a warp a row: turned, then divided by a power of two, which keeps their products with the cached bytes
+        // within fp32's range. A NaN or Inf makes the row NaN.
         for (uint32_t r = tid >> 5; r < kRt; r += kNT / 32) {
-            const uint32_t lane = tid & 31u;
+            const uint32_t lane = tid & 31u, tok = (r_base + r) / a.shape.group, g = (r_base + r) - tok * a.shape.group;
+            const float* p = static_cast<const float*>(a.q.data) + (pc.plan.row0 + tok) * a.q.token_stride +
+                             (pc.head * a.shape.group + g) * a.q.head_stride;
             float m = 0.0f;
             for (uint32_t d = lane; d < D; d += 32u) {
-                const float ab = fabsf(sm.q[r * D + d]);
-                m = ab < __builtin_huge_valf() ? fmaxf(m, ab) : __builtin_huge_valf();
+                float x = 0.0f;
+                if (r < pc.rows) load_turned<float, 1>(a.rope, p, d, pc.plan.p0 + static_cast<int32_t>(tok), &x);
+                m = fabsf(x) < __builtin_huge_valf() ? fmaxf(m, fabsf(x)) : __builtin_huge_valf();
+                sm.q[r * D + d] = x;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
