@@ -93,7 +93,7 @@ class _Caller:
         if not t.is_cuda or t.get_device() != self.device:
             raise ValueError(f"{what}: on {t.device}, not cuda:{self.device}")
 
-    def view(self, i: int, t, tokens: int, dim: int, what: str) -> int:
+    def view(self, i: int, t, tokens: int, dim: int, what: str, written: bool = False) -> int:
         """Record i filled with t [tokens, heads, dim] (unit stride along dim); its address."""
         dt = self.dtypes.get(t.dtype)
         shape = t.shape
@@ -103,6 +103,8 @@ class _Caller:
         stride = t.stride()
         if stride[2] != 1:
             raise ValueError(f"{what}: the last dimension must have unit stride")
+        if written and ((stride[0] == 0 and shape[0] > 1) or (stride[1] == 0 and shape[1] > 1)):
+            raise ValueError(f"{what}: rows that share their memory cannot be written")
         r = self.records
         v = r.views[i]
         v.data, v.dtype, v.n_heads, v.token_stride, v.head_stride = t.data_ptr(), dt, shape[1], stride[0], stride[1]
@@ -165,7 +167,7 @@ class Rope:
         elif out.shape != x.shape:
             raise ValueError(f"out: {tuple(x.shape)} expected, got {tuple(out.shape)}")
         st = _lib().sixi_kv_rope_apply(self.h, c.view(0, x, n, dim, "x"), positions.data_ptr(), n, dim, 1 if inverse else 0,
-                                       c.view(1, out, n, dim, "out"), c.stream(stream))
+                                       c.view(1, out, n, dim, "out", True), c.stream(stream))
         _check("sixi_kv_rope_apply", st)
         return out
 
@@ -275,8 +277,8 @@ class KvCache:
             k = c.torch.empty((n, self.n_kv_heads, dim), dtype=dt, device=c.dev) if k is None else k
             v = c.torch.empty((n, self.n_kv_heads, dim), dtype=dt, device=c.dev) if v is None else v
         status = self._status(status, batch)
-        st = _lib().sixi_kv_read(self.h, batch.at, c.view(0, k, n, dim, "k"), c.view(1, v, n, dim, "v"), status.data_ptr(),
-                                 c.stream(stream))
+        st = _lib().sixi_kv_read(self.h, batch.at, c.view(0, k, n, dim, "k", True), c.view(1, v, n, dim, "v", True),
+                                 status.data_ptr(), c.stream(stream))
         _check("sixi_kv_read", st)
         return k, v
 
@@ -300,7 +302,7 @@ class KvCache:
         status = self._status(status, batch)
         st = _lib().sixi_kv_attend(self.h, c.view(0, q, n, dim, "q"), batch.at,
                                    dim ** -0.5 if scale is None else scale, min(window, 0xFFFFFFFF),
-                                   0 if causal else ATTEND_ALL, _rope_handle(rope), c.view(1, out, n, dim, "out"),
+                                   0 if causal else ATTEND_ALL, _rope_handle(rope), c.view(1, out, n, dim, "out", True),
                                    lse.data_ptr(), status.data_ptr(), c.stream(stream))
         _check("sixi_kv_attend", st)
         return out, lse, status

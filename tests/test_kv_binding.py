@@ -303,3 +303,26 @@ def test_rope_numbers_beyond_32_bits_are_refused(lib, field, value):
     args = dict(rot_dim=64, scaling="yarn", factor=2.0, original_max_position=4096)
     with pytest.raises(ValueError, match=field):
         K.Rope(device=0, **{**args, field: value})
+
+
+class Expanded(Tensor):
+    """Every row of heads in the same place."""
+
+    def stride(self, i=None):
+        s = (0, 0, 1)
+        return s if i is None else s[i]
+
+
+@pytest.mark.parametrize("name", ["read", "attend", "apply"])
+def test_outputs_whose_rows_share_their_place_are_refused(lib, name):
+    cache, rope, b = make_cache(), make_rope(), batch()
+    q, kv, one = Tensor((3, 4, 32), BF), Tensor((3, 2, 32), BF), Expanded((3, 2, 32), BF)
+    calls = {"read": lambda: cache.read(b, k=kv, v=one, stream=MAIN),
+             "attend": lambda: cache.attend(q, b, out=Expanded((3, 4, 32), BF), stream=MAIN),
+             "apply": lambda: rope.apply(kv, Tensor((3,), I32), out=one, stream=MAIN)}
+    with pytest.raises(ValueError, match="share"):
+        calls[name]()
+    assert not {"sixi_kv_read", "sixi_kv_attend", "sixi_kv_rope_apply"} & set(lib.calls)
+    cache.append(one, one, b, stream=MAIN)  # (as inputs they are rows like others)
+    rope.apply(one, Tensor((3,), I32), stream=MAIN)
+    cache.attend(Expanded((3, 4, 32), BF), b, out=q, stream=MAIN)
