@@ -265,6 +265,7 @@ struct AttnShape {
     // Beginning and ending a unit takes about as long as this many of its tiles: each unit's place on the line is so much
     // longer than its tiles, and CTAs with many short units get fewer tiles.
     uint32_t unit_cost;
+    uint32_t whole_tiles;  // units of at most this many tiles (in every sequence of a call) are not cut
 };
 
 // 64-bit quotient; the 32-bit one, which is much shorter, where it is enough
@@ -353,10 +354,6 @@ struct PieceWalk {
     bool whole;  // the line is one of units, not tiles: no unit is cut
 };
 
-// Units of at most this many tiles (in every sequence of a call) are not cut: joining the pieces costs about as much as
-// four tiles (one token over 700 cached ones, 32 heads on 8, 6 tiles a unit: 13.9 us whole, 15.7 us cut).
-constexpr uint32_t kWholeTiles = 8;
-
 __device__ __forceinline__ bool next_piece(const AttnShape& a, const KvBatchView& b, uint32_t page_shift, PieceWalk& w,
                                            Piece* out) {
     while (w.at < w.stop) {
@@ -438,7 +435,7 @@ __device__ __forceinline__ bool walk_init(const AttnShape& a, const KvBatchView&
             if (s < b.n_seqs) {
                 p = plan_seq(a, b, page_shift, s);
                 mine = plan_tiles(a, p) | (static_cast<uint64_t>(p.lanes) * a.n_heads << 40);
-                small = !p.paired && p.weight <= kWholeTiles + a.unit_cost;
+                small = !p.paired && p.weight <= a.whole_tiles + a.unit_cost;
                 in_order = p.in_order;
             }
             uint64_t incl = mine;

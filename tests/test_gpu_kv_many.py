@@ -66,3 +66,25 @@ def test_time_grows_with_the_sequences_not_with_their_square(dt):
         out, lse, st = kv.attend(q, batch)
         t.append(least_time(lambda: kv.attend(q, batch, out=out, lse=lse, status=st)))
     assert t[1] <= 16 * t[0], t
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_shorter_sequence_does_not_take_longer(dt):
+    """Where units begin to be cut, time may not fall: half the tokens take no more than the whole, but for a fifth."""
+    t = {}
+    for n in (128, 256, 512, 1024):
+        kv = KvCache(n // 16, 16, 3, 80, device=0)
+        for p in (kv.k_pages, kv.v_pages):
+            p.zero_()
+        for p in (kv.k_scales, kv.v_scales):
+            p.fill_(1.0)
+        batch = KvBatch(torch.arange(n // 16, dtype=torch.int32, device=DEV).view(1, -1), torch.tensor([0, 2], device=DEV),
+                        torch.tensor([n], dtype=torch.int32, device=DEV), 2, 2)
+        q = torch.ones((2, 21, 80), dtype=dt, device=DEV)
+        out, lse, st = kv.attend(q, batch)
+        call = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(call):
+            for _ in range(20):
+                kv.attend(q, batch, out=out, lse=lse, status=st)
+        t[n] = least_time(call.replay)
+    assert all(t[n] <= 1.2 * t[2 * n] for n in (128, 256, 512)), t
