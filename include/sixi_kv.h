@@ -165,6 +165,8 @@ SIXI_SMP_API int32_t sixi_kv_read(sixi_kv* h, const sixi_kv_batch* batch, const 
  *             unspecified. SIXI_BACKEND_ERROR for all if a wait inside a kernel ever runs out (and
  *             from then on for every call of the handle)
  * n_tokens * n_q_heads / n_kv_heads < 2^30, and the call's tiles of 8 rows by 64 positions < 2^40.
+ * Queries and keys may have any finite magnitudes whose scores are within fp32's range. Values are
+ * summed before they are divided by the weights' sum: what a row's |v_t| add up to has to stay within it too.
  * Pages that lie wholly before every row's window are not read, and their table entries may be anything.
  * Sums and softmax statistics are fp32. With fp32 queries everything is. With bf16 queries the products
  * run on the tensor cores straight from the cached bytes, and the weights exp(s_t - m) enter theirs

@@ -9,8 +9,9 @@
 //
 // The work is cut over two CTAs per SM as smp_kv.cuh describes. fp32 products have no tensor-core form that
 // keeps 24 bits, so the bound is the fp32 pipes and the shared-memory reads that feed them, and for small
-// calls the chain of steps of a tile: 15 tokens of 6 sequences, up to 3,000 cached ones, 21 heads of 80
-// elements on 3: 39 us (the bytes alone would take 0.4 us at the copy rate).
+// calls what a piece costs whatever its length: a call of one tile takes 17 us, a further tile of a piece 6, and
+// joining 47 pieces some 20. 15 tokens of 6 sequences, up to 3,000 cached ones, 21 heads of 80 elements on 3, cut
+// into pieces of one or two tiles: 40 us (the bytes alone would take 0.4 us at the copy rate).
 #include <cuda_runtime.h>
 
 #include "smp_kernels.cuh"

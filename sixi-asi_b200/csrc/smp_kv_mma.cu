@@ -36,14 +36,14 @@
 // at a time, with the scores of the next ready before one ends, hide it.
 //
 // Bound and measured (one B200, bytes at its copy rate of 6.54 TB/s, products at 1.65 PFLOP/s):
-//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 111 to 117 us, 5.2 to 5.5 TB/s (80 to 84 %
+//   64 sequences, one token, up to 16,000 cached, 32 heads on 8 of 128: 111 to 113 us, 5.4 to 5.5 TB/s (83 to 85 %
 //     of the copy rate)
-//   2 sequences, one token, up to 262,144 cached, 32 on 4 of 128:       93 us, 5.6 TB/s (85 %)
-//   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         177 to 190 us; 26 us of bytes
-//   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       790 to 810 us; 163 us of products
+//   2 sequences, one token, up to 262,144 cached, 32 on 4 of 128:       92 to 95 us, 5.5 to 5.7 TB/s (84 to 87 %)
+//   32 sequences, 9 tokens, up to 8,000 cached, 64 on 8 of 128:         178 to 194 us; 26 us of bytes
+//   3 chunks of up to 2,048 tokens, window 4,096, 16 on 4 of 256:       772 to 794 us; 163 us of products
 //   one token over 700 cached, 32 on 8 of 128:                          14 us, a chain of waits
-// With few rows memory is the bound. With 64 rows a tile it is the softmax's chain of waits for scores, barriers and
-// weights, and instruction fetch: 37 % of the issue slots, 25 % of the ALU and 16 % of the tensor pipe are busy, and code
+// With few rows memory is the bound. With many rows a tile it is the softmax's chain of waits for scores, barriers and
+// weights, and instruction fetch: 40 % of the issue slots, 28 % of the ALU and 17 % of the tensor pipe are busy, and code
 // that is never run moves these times by 3 to 5 %.
 #include <cuda.h>
 #include <cuda_runtime.h>
